@@ -41,7 +41,8 @@ enum {
     LLOOM_HIP_EEXPERT = 4,     /* an expert id >= n_experts                  */
     LLOOM_HIP_EHIP = 5,        /* a HIP runtime call failed                 */
     LLOOM_HIP_ENOMEM = 6,      /* device allocation failed                  */
-    LLOOM_HIP_EDEVICE = 7      /* no gfx950 device at that ordinal          */
+    LLOOM_HIP_EDEVICE = 7,     /* no gfx950 device at that ordinal          */
+    LLOOM_HIP_EPAGE = 8        /* a page, slot or length out of range       */
 };
 
 enum {
@@ -89,8 +90,10 @@ enum { LLOOM_HIP_MMA_F16 = 0, LLOOM_HIP_MMA_INT8 = 1, LLOOM_HIP_MMA_AUTO = 2 };
 int lloom_hip_ctx_set_prefill_mma(lloom_hip_ctx* ctx, int mode);
 
 /* Wait for the device; report a device-side error (an out-of-range expert
- * id seen by a routed matmul, or an out-of-range embedding id) recorded
- * since the last check, and clear it. */
+ * id seen by a routed matmul, or an out-of-range embedding id: EEXPERT; a page,
+ * slot or length that a paged-cache call could not serve: EPAGE) recorded
+ * since the last check, and clear it.  Where both were seen, EEXPERT is
+ * reported and EPAGE by the next call. */
 int lloom_hip_ctx_sync(lloom_hip_ctx* ctx);
 
 /* ---------------------------------------------------------------- memory --
@@ -262,6 +265,65 @@ int lloom_hip_moe_matmul_glu(lloom_hip_ctx* ctx, int ggml_type, const void* w_ga
 int lloom_hip_embedding(lloom_hip_ctx* ctx, int ggml_type, const void* w_dev, int64_t rows,
                         int64_t hidden, const uint32_t* ids_dev, int64_t n_ids, void* y_dev,
                         int out_dtype, int strict, void* stream);
+
+/* ----------------------------------------------------------- paged cache --
+ * Attention over a cache of pages beside the packed projections, for programs
+ * that serve requests of different lengths.  A layer's cache is two f16 arrays,
+ *   k [pages][kv_heads][page_size][head_dim]
+ *   v [pages][kv_heads][head_dim][page_size]
+ * of the caller's, page_size a power of two from 16 to 4096 and head_dim 64, 96,
+ * 128 or 256.  Position p of request b is in page tables[b * table_stride +
+ * p / page_size] at p % page_size.  Lengths, starts and pages are int32 (read as
+ * such), slots int64 (page * page_size + place).  At most 4096 requests a call
+ * (LLOOM_HIP_ESHAPE beyond).  The calls neither synchronize nor copy; what only
+ * the GPU can see (a page or slot out of range, no free page left, lengths that
+ * do not fit) is left out of the result as said below and reported by the next
+ * lloom_hip_ctx_sync as LLOOM_HIP_EPAGE.
+ *
+ * lloom_hip_paged_plan: a step's bookkeeping from each request's cached[b]
+ * tokens and new[b] more.  q_start[requests + 1] = the requests' first rows
+ * among the step's `tokens` (exclusive sums of new), seq_lens = cached + new,
+ * positions[tokens], slots[tokens]; request b takes
+ * ceil(seq / page_size) - ceil(cached / page_size) pages, from free[0 ..] in the
+ * requests' order, which are stored in its table; taken[0] = pages in all.  Rows
+ * past the last request's (a padded batch) get position 0 and slot -1; tokens
+ * that no page is left for slot -1, and -1 in the table. */
+int lloom_hip_paged_plan(lloom_hip_ctx* ctx, const uint32_t* cached_dev, const uint32_t* new_dev, int64_t requests,
+                         int64_t tokens, void* tables_dev, int64_t table_stride, int64_t max_blocks,
+                         const uint32_t* free_dev, int64_t free_count, int64_t page_size, void* q_start_dev,
+                         void* seq_lens_dev, void* positions_dev, void* slots_dev, void* taken_dev, void* stream);
+
+/* Rows k and v [tokens][kv_heads * head_dim] (F32, rounded to nearest even, or
+ * F16; rows k_stride and v_stride elements apart) into the cache at their slots;
+ * a negative slot stores nothing.  No two rows of a call have the same slot.
+ * Rows 16-byte aligned. */
+int lloom_hip_paged_append(lloom_hip_ctx* ctx, int act_dtype, const void* k_dev, int64_t k_stride, const void* v_dev,
+                           int64_t v_stride, const void* slots_dev, int64_t tokens, void* k_cache_dev,
+                           void* v_cache_dev, int64_t pages, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                           void* stream);
+
+/* Causal attention of q [tokens][kv_heads * group][head_dim] (F32 or F16, rows
+ * q_stride elements apart) into out (same type, contiguous).  Rows q_start[b] ..
+ * q_start[b + 1) are request b's last tokens, the last one at position
+ * seq_lens[b] - 1; head h reads key head h / group.  The token at position p sees
+ * position j <= p with window = 0, j > p - window or j < sinks, and its
+ * result is sum_j softmax_j(scale q.k_j) v_j over what it sees: zero where it
+ * sees nothing, where no request owns the row, and nothing of a page out of
+ * [0, pages).  Values that a token does not see may be anything.  Sums and the
+ * softmax are f32.  With F32 q the products take q and the weights as two halves
+ * each (exact to about 2^-22); with F16 the weights are rounded to halves.
+ * max_new: no request has more new tokens (0: not known); only speed depends
+ * on it. */
+int lloom_hip_paged_attention(lloom_hip_ctx* ctx, int act_dtype, const void* q_dev, int64_t q_stride, int64_t tokens,
+                              const void* k_cache_dev, const void* v_cache_dev, int64_t pages, int64_t kv_heads,
+                              int64_t group, int64_t head_dim, int64_t page_size, const void* tables_dev,
+                              int64_t table_stride, int64_t max_blocks, const void* q_start_dev,
+                              const void* seq_lens_dev, int64_t requests, float scale, int64_t window, int64_t sinks,
+                              int64_t max_new, void* out_dev, void* stream);
+
+/* Workspace of an attention call of this shape, to reserve before a capture. */
+int lloom_hip_paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t kv_heads, int64_t group,
+                                              int64_t head_dim, int64_t max_new, size_t* bytes);
 
 /* ------------------------------------------------------- synthetic data --
  * The benchmark/test input generator (not part of the reference): SplitMix64

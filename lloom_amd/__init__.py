@@ -20,3 +20,12 @@ from .quantized import (  # noqa: F401
     synth_normal,
     synth_uniform,
 )
+from .paged import (  # noqa: F401
+    PagedCache,
+    PagedPlan,
+    paged_append,
+    paged_attention,
+    paged_attention_workspace_bytes,
+    paged_check,
+    paged_plan,
+)

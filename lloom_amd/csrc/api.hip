@@ -86,7 +86,7 @@ static WsState try_ws(lloom_hip_ctx* ctx, size_t bytes, hipStream_t s, void** ou
 }
 
 // The same, for a call that cannot do with less.
-static int ensure_ws(lloom_hip_ctx* ctx, size_t bytes, hipStream_t s, void** out) {
+int ensure_ws(lloom_hip_ctx* ctx, size_t bytes, hipStream_t s, void** out) {
     switch (try_ws(ctx, bytes, s, out)) {
         case WS_OK: return LLOOM_HIP_OK;
         case WS_CAPTURING:
@@ -174,12 +174,15 @@ int lloom_hip_ctx_sync(lloom_hip_ctx* ctx) {
     if (!ctx) return fail(LLOOM_HIP_EINVAL, "ctx_sync: null context");
     HIP_OK(hipSetDevice(ctx->device));
     HIP_OK(hipDeviceSynchronize());
-    int flag = 0;
-    HIP_OK(hipMemcpy(&flag, ctx->flags, sizeof(int), hipMemcpyDeviceToHost));
-    if (flag) {
-        int zero = 0;
+    int flag[2] = {0, 0}, zero = 0;
+    HIP_OK(hipMemcpy(flag, ctx->flags, sizeof flag, hipMemcpyDeviceToHost));
+    if (flag[0]) {
         HIP_OK(hipMemcpy(ctx->flags, &zero, sizeof(int), hipMemcpyHostToDevice));
         return fail(LLOOM_HIP_EEXPERT, "a routed matmul or embedding saw an id out of range");
+    }
+    if (flag[1]) {
+        HIP_OK(hipMemcpy(ctx->flags + 1, &zero, sizeof(int), hipMemcpyHostToDevice));
+        return fail(LLOOM_HIP_EPAGE, "a paged-cache call saw a page, slot or length out of range, or no free page left");
     }
     return LLOOM_HIP_OK;
 }

@@ -20,7 +20,7 @@ struct lloom_hip_ctx {
     // earlier, keep reading them, so growth needs no device synchronization.
     // Growth at least doubles, so they hold less than the current one.
     std::vector<void*> retired;
-    int* flags = nullptr;  // [0] sticky id error
+    int* flags = nullptr;  // sticky errors: [0] ids, [1] pages and lengths of the paged cache
     // What a strict call's kernel reports, in host memory: the call reads it
     // when its stream has drained, with no copy (a pageable 4-byte copy took 10
     // us of a 37 us routed call).
@@ -29,6 +29,10 @@ struct lloom_hip_ctx {
     int prefill_mma = lloom::GEMM_AUTO;
     std::mutex mu;
 };
+
+// Workspace of at least `bytes`, as ensured by a call that cannot do with less
+// (0 or the refusal's code); ctx->mu is held.
+int ensure_ws(lloom_hip_ctx* ctx, size_t bytes, hipStream_t s, void** out);
 
 // Records the message of a failure for lloom_hip_last_error; returns code.
 int fail(int code, const char* fmt, ...);

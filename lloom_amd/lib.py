@@ -9,6 +9,7 @@ _lib = None
 
 ERRORS = {
     1: "EINVAL", 2: "EDTYPE", 3: "ESHAPE", 4: "EEXPERT", 5: "EHIP", 6: "ENOMEM", 7: "EDEVICE",
+    8: "EPAGE",
 }
 
 
@@ -70,6 +71,14 @@ def lib():
                 "lloom_hip_moe_matmul_glu": ([vp, i32, vp, vp, i64, i64, i64, vp, i64, i64, vp, i64, vp, i32, vp],
                                              i32),
                 "lloom_hip_embedding": ([vp, i32, vp, i64, i64, vp, i64, vp, i32, i32, vp], i32),
+                "lloom_hip_paged_plan": ([vp, vp, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, vp,
+                                          vp], i32),
+                "lloom_hip_paged_append": ([vp, i32, vp, i64, vp, i64, vp, i64, vp, vp, i64, i64, i64, i64,
+                                            vp], i32),
+                "lloom_hip_paged_attention": ([vp, i32, vp, i64, i64, vp, vp, i64, i64, i64, i64, i64, vp, i64, i64,
+                                               vp, vp, i64, ctypes.c_float, i64, i64, i64, vp, vp], i32),
+                "lloom_hip_paged_attention_workspace_bytes": ([i64, i64, i64, i64, i64, i64,
+                                                               ctypes.POINTER(sz)], i32),
                 "lloom_hip_synth_normal": ([ctypes.c_uint64, ctypes.c_float, ctypes.c_float, vp, i64], i32),
                 "lloom_hip_synth_uniform": ([ctypes.c_uint64, ctypes.c_float, ctypes.c_float, vp, i64], i32),
             }

@@ -32,6 +32,7 @@ pub const LLOOM_HIP_EEXPERT: c_int = 4;
 pub const LLOOM_HIP_EHIP: c_int = 5;
 pub const LLOOM_HIP_ENOMEM: c_int = 6;
 pub const LLOOM_HIP_EDEVICE: c_int = 7;
+pub const LLOOM_HIP_EPAGE: c_int = 8;
 
 // Type ids (GgmlDType::to_u32, mod.rs:505-568).
 pub const LLOOM_HIP_F32: c_int = 0;
@@ -265,6 +266,79 @@ extern "C" {
         out_dtype: c_int,
         strict: c_int,
         stream: *mut c_void,
+    ) -> c_int;
+
+    // The paged cache: a step's block tables and slots, rows into pages, attention.
+    pub fn lloom_hip_paged_plan(
+        ctx: *mut lloom_hip_ctx,
+        cached_dev: *const u32,
+        new_dev: *const u32,
+        requests: i64,
+        tokens: i64,
+        tables_dev: *mut c_void,
+        table_stride: i64,
+        max_blocks: i64,
+        free_dev: *const u32,
+        free_count: i64,
+        page_size: i64,
+        q_start_dev: *mut c_void,
+        seq_lens_dev: *mut c_void,
+        positions_dev: *mut c_void,
+        slots_dev: *mut c_void,
+        taken_dev: *mut c_void,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn lloom_hip_paged_append(
+        ctx: *mut lloom_hip_ctx,
+        act_dtype: c_int,
+        k_dev: *const c_void,
+        k_stride: i64,
+        v_dev: *const c_void,
+        v_stride: i64,
+        slots_dev: *const c_void,
+        tokens: i64,
+        k_cache_dev: *mut c_void,
+        v_cache_dev: *mut c_void,
+        pages: i64,
+        kv_heads: i64,
+        head_dim: i64,
+        page_size: i64,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn lloom_hip_paged_attention(
+        ctx: *mut lloom_hip_ctx,
+        act_dtype: c_int,
+        q_dev: *const c_void,
+        q_stride: i64,
+        tokens: i64,
+        k_cache_dev: *const c_void,
+        v_cache_dev: *const c_void,
+        pages: i64,
+        kv_heads: i64,
+        group: i64,
+        head_dim: i64,
+        page_size: i64,
+        tables_dev: *const c_void,
+        table_stride: i64,
+        max_blocks: i64,
+        q_start_dev: *const c_void,
+        seq_lens_dev: *const c_void,
+        requests: i64,
+        scale: f32,
+        window: i64,
+        sinks: i64,
+        max_new: i64,
+        out_dev: *mut c_void,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn lloom_hip_paged_attention_workspace_bytes(
+        tokens: i64,
+        requests: i64,
+        kv_heads: i64,
+        group: i64,
+        head_dim: i64,
+        max_new: i64,
+        bytes: *mut usize,
     ) -> c_int;
 
     // Host-side synthetic inputs (StdRng-seeded normal / uniform), for benches.
