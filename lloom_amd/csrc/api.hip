@@ -21,6 +21,7 @@
 #include "kernels.hpp"
 #include "kq_common.hpp"
 #include "api_internal.hpp"
+#include "paged.hpp"
 
 using namespace lloom;
 
@@ -57,6 +58,9 @@ static const char* type_name(int t) {
     }
     return "unknown";
 }
+
+// The sticky flags, and from int 64 on the paged attention's counters.
+constexpr size_t CTX_FLAG_BYTES = 256 + PAGED_JOINS * sizeof(int);
 
 // Workspace of at least `bytes`, 256-byte aligned; grows, never shrinks
 // (the CUDA arm's per-device workspace, quantized/fast_mmvq.rs:49-80).  A
@@ -123,7 +127,7 @@ int lloom_hip_ctx_create(int device, lloom_hip_ctx** out) {
         delete c;
         return fail(LLOOM_HIP_EHIP, "ctx_create: stream creation failed");
     }
-    if (hipMalloc(&c->flags, 256) != hipSuccess) {
+    if (hipMalloc(&c->flags, CTX_FLAG_BYTES) != hipSuccess) {
         (void)hipStreamDestroy(c->stream);
         delete c;
         return fail(LLOOM_HIP_ENOMEM, "ctx_create: flag allocation failed");
@@ -134,7 +138,8 @@ int lloom_hip_ctx_create(int device, lloom_hip_ctx** out) {
         delete c;
         return fail(LLOOM_HIP_ENOMEM, "ctx_create: host flag allocation failed");
     }
-    (void)hipMemset(c->flags, 0, 256);
+    c->joins = c->flags + 64;
+    (void)hipMemset(c->flags, 0, CTX_FLAG_BYTES);
     (void)hipDeviceSynchronize();
     *out = c;
     return LLOOM_HIP_OK;
@@ -174,8 +179,13 @@ int lloom_hip_ctx_sync(lloom_hip_ctx* ctx) {
     if (!ctx) return fail(LLOOM_HIP_EINVAL, "ctx_sync: null context");
     HIP_OK(hipSetDevice(ctx->device));
     HIP_OK(hipDeviceSynchronize());
-    int flag[2] = {0, 0}, zero = 0;
+    int flag[CTX_FLAG_BYTES / sizeof(int)], zero = 0;
     HIP_OK(hipMemcpy(flag, ctx->flags, sizeof flag, hipMemcpyDeviceToHost));
+    for (int i = 0; i < PAGED_JOINS; i++)
+        if (flag[64 + i]) {
+            HIP_OK(hipMemset(ctx->joins, 0, PAGED_JOINS * sizeof(int)));
+            break;
+        }
     if (flag[0]) {
         HIP_OK(hipMemcpy(ctx->flags, &zero, sizeof(int), hipMemcpyHostToDevice));
         return fail(LLOOM_HIP_EEXPERT, "a routed matmul or embedding saw an id out of range");

@@ -21,6 +21,9 @@ struct lloom_hip_ctx {
     // Growth at least doubles, so they hold less than the current one.
     std::vector<void*> retired;
     int* flags = nullptr;  // sticky errors: [0] ids, [1] pages and lengths of the paged cache
+    // What the paged attention's workgroups count themselves with: zero between
+    // calls; ctx_sync, with nothing running, clears what a call that was cut off left.
+    int* joins = nullptr;
     // What a strict call's kernel reports, in host memory: the call reads it
     // when its stream has drained, with no copy (a pageable 4-byte copy took 10
     // us of a 37 us routed call).

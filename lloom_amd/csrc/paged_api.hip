@@ -133,9 +133,10 @@ int lloom_hip_paged_attention(lloom_hip_ctx* ctx, int act_dtype, const void* q_d
     if (need)
         if (int rc = ensure_ws(ctx, need, s, &ws)) return rc;
     PagedCall c{q_dev, (const uint16_t*)k_cache_dev, (const uint16_t*)v_cache_dev, out_dev, (const int*)q_start_dev,
-                (const int*)seq_lens_dev, (const int*)tables_dev, ctx->flags + 1, q_stride, table_stride, (int)tokens,
+                (const int*)seq_lens_dev, (const int*)tables_dev, ctx->flags + 1, ctx->joins, q_stride, table_stride, (int)tokens,
                 (int)requests, (int)kv_heads, (int)group, (int)pages, page_shift(page_size), (int)max_blocks,
-                (int)window, (int)sinks, scale * 1.44269504088896340736f};
+                (int)window, (int)sinks, scale * 1.44269504088896340736f,
+                group > 1 ? (uint32_t)(((1ull << 32) + group - 1) / group) : 0u};
     HIP_OK(launch_paged_attention(act_dtype, (int)head_dim, c, (int)max_new, ws, s));
     return LLOOM_HIP_OK;
 }
