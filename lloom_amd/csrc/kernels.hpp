@@ -160,9 +160,14 @@ hipError_t launch_paged_plan(const int* cached, const int* fresh, int requests, 
 hipError_t launch_paged_append(int act, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                                const int64_t* slots, int tokens, void* kc, void* vc, int pages, int kv_heads, int dim,
                                int page_shift, int* flags, hipStream_t s);
-// paged_attn.hip: head dims that paged_dim_fits names; no request has over max_new
-// new tokens (results do not depend on it).
+// paged_attn.hip, paged_tile.hip: head dims that paged_dim_fits names.  A call's
+// requests go to the one kernel or the other by their rows (paged.hpp); no request
+// has over max_new new tokens where that is not 0 (results do not depend on it).
 constexpr bool paged_dim_fits(int64_t d) { return d == 64 || d == 96 || d == 128 || d == 256; }
+hipError_t launch_paged_rows(int act, int dim, const PagedCall& c, int route, int few, void* ws, hipStream_t s);
+size_t paged_rows_workspace_bytes(int kv_heads, int dim);
+hipError_t launch_paged_tiles(int act, int dim, const PagedCall& c, int route, int few, void* ws, hipStream_t s);
+size_t paged_tiles_workspace_bytes(int kv_heads, int dim);
 size_t paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int kv_heads, int group, int dim,
                                        int max_new);
 hipError_t launch_paged_attention(int act, int dim, const PagedCall& c, int max_new, void* ws, hipStream_t s);

@@ -21,6 +21,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "kq_common.hpp"
+
 namespace lloom {
 
 constexpr int PAGED_MAX_REQUESTS = 4096;
@@ -42,12 +44,16 @@ struct PagedCall {
 };
 
 // How a kernel cuts its requests: 2^row_shift rows of a request and 2^unit_shift
-// keys at a time, at least `unit_min` units an item, and about 2^target_shift
-// items in all.  A tile's last token is at most `more` past its first.
+// keys at a time; a tile with more units of keys than a 2^target_shift-th of the
+// call's, and than `unit_min`, is split among several items.  A tile's last token
+// is at most `more` past its first.
 // route: 0 every request, 1 those of at most `few` rows, 2 the others.
 struct PagedCut {
-    int row_shift, unit_shift, unit_min, target_shift, more, route, few, split;
+    int row_shift, unit_shift, unit_min, target_shift, more, route, few;
 };
+// A split tile has more units than a 2^target_shift-th of all, so that there are
+// under 2^target_shift of them and under twice as many items of theirs.
+__host__ __device__ inline int paged_parts(int target_shift) { return 2 << target_shift; }
 
 // The keys that rows at positions lo .. hi see: [first, hi] and the first
 // `sink` tokens before it, as steps of `step` keys.  Step i of the list is
@@ -79,13 +85,25 @@ __host__ __device__ inline int paged_units(int T, int L, const PagedCut& c, int 
     return most < full ? (int)most : full;
 }
 
+// The most items a call has: its tiles, and the splits of the longest ones, of
+// which there are no more than the tables have units of keys for.
+inline int64_t paged_items_most(const PagedCall& c, const PagedCut& cut) {
+    const int64_t rows = (int64_t)1 << cut.row_shift, some = c.requests < c.tokens ? c.requests : c.tokens;
+    int64_t tiles = ((int64_t)c.tokens * c.group >> cut.row_shift) + some;
+    if (cut.route == 1 && tiles > some * ((cut.few + rows - 1) / rows)) tiles = some * ((cut.few + rows - 1) / rows);
+    tiles *= c.kv_heads;
+    const int64_t keys = (int64_t)c.max_blocks << c.page_shift, units = (keys + (1 << cut.unit_shift) - 1) >> cut.unit_shift;
+    const int64_t all = tiles + ((int64_t)1 << cut.target_shift);
+    return units < all && units * tiles < all ? units * tiles : all;
+}
+
 #if defined(__HIPCC__)
 
-// One item: rows row0 .. of request b, split `split` of `splits` of its keys.
+// One item: rows of tile `tile` of request b, split `split` of `splits` of its keys.
 struct PagedItem {
-    int b, T, L, start, tile, split, splits, chunk;  // chunk: units a split
-    int first;                                       // the item of split 0
-    int group_index;                                 // this (request, tile) among the call's
+    int b, T, L, start, tile, split, splits;
+    int part;   // split 0's number among the items of split tiles
+    int joint;  // the tile's number among them
     bool found;
 };
 
@@ -124,6 +142,46 @@ __device__ __forceinline__ int paged_scan(int v) {  // inclusive over the wave
     return v;
 }
 
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ half8_t as_half8(uint4 v) { return __builtin_bit_cast(half8_t, v); }
+
+// x as hi + lo, two halves: exact to 2^-22 of x where x is in half's normal range.
+__device__ __forceinline__ void split8(const float (&x)[8], half8_t& hi, half8_t& lo) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const _Float16 h = (_Float16)x[i];
+        hi[i] = h;
+        lo[i] = (_Float16)(x[i] - (float)h);
+    }
+}
+
+// Zeroes the infinities and NaN among 8 keys' values; bit j of the result: there
+// was one at key j.
+__device__ __forceinline__ uint32_t take_odd(uint4& v) {
+    uint32_t odd = 0;
+    uint32_t* w = (uint32_t*)&v;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if ((w[j] & 0x7c00u) == 0x7c00u) {
+            odd |= 1u << (2 * j);
+            w[j] &= 0xffff0000u;
+        }
+        if ((w[j] & 0x7c000000u) == 0x7c000000u) {
+            odd |= 2u << (2 * j);
+            w[j] &= 0xffffu;
+        }
+    }
+    return odd;
+}
+// Zeroes the values of the keys whose bit is not set.
+__device__ __forceinline__ void keep8(uint4& v, uint32_t bits) {
+    uint32_t* w = (uint32_t*)&v;
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] &= (bits >> (2 * j) & 1) * 0xffffu | (bits >> (2 * j + 1) & 1) * 0xffff0000u;
+}
+
 // A lane's request: its rows' tiles, and the units of keys of one.
 struct PagedLane {
     int start, T, L, tiles, units;
@@ -140,34 +198,40 @@ __device__ __forceinline__ PagedLane paged_lane(const PagedCall& c, const PagedC
     return r;
 }
 
+template <bool F32>
+__device__ __forceinline__ void paged_store4(void* out, int64_t at, float x, float y, float z, float w) {
+    if constexpr (F32) {
+        *(float4*)((float*)out + at) = make_float4(x, y, z, w);
+    } else {
+        *(uint2*)((uint16_t*)out + at) = make_uint2(f32_to_f16(x) | (uint32_t)f32_to_f16(y) << 16,
+                                                    f32_to_f16(z) | (uint32_t)f32_to_f16(w) << 16);
+    }
+}
+
 // Item `want` of the call, found by every wave on its own: the lengths are known
 // on the GPU alone, and 64 requests cost two scans.  No LDS, no barrier.
 __device__ __forceinline__ PagedItem paged_find(const PagedCall& c, const PagedCut& cut, int want) {
     const int lane = __lane_id(), cap = paged_key_cap(c);
     PagedLane at = paged_lane(c, cut, cap, lane);
-    int chunk = 0x7fffffff;  // the units a split takes
-    if (cut.split) {
-        unsigned long long total = (unsigned long long)at.tiles * at.units;
-        for (int b = 64; b < c.requests; b += 64) {
-            const PagedLane more = paged_lane(c, cut, cap, b + lane);
-            total += (unsigned long long)more.tiles * more.units;
-        }
-#pragma unroll
-        for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d, 64);
-        const unsigned long long per = (total * c.kv_heads + (1u << cut.target_shift) - 1) >> cut.target_shift;
-        chunk = (int)min(per > (unsigned)cut.unit_min ? per : (unsigned long long)cut.unit_min, 0x7fffffffull);
+    unsigned long long total = (unsigned long long)at.tiles * at.units;
+    for (int b = 64; b < c.requests; b += 64) {
+        const PagedLane more = paged_lane(c, cut, cap, b + lane);
+        total += (unsigned long long)more.tiles * more.units;
     }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d, 64);
+    const unsigned long long per = (total * c.kv_heads + (1u << cut.target_shift) - 1) >> cut.target_shift;
+    const int chunk = (int)min(per > (unsigned)cut.unit_min ? per : (unsigned long long)cut.unit_min, 0x7fffffffull);
     // every field is the same in all lanes: readlane keeps them scalar
     PagedItem it;
     it.found = false;
-    it.b = it.T = it.L = it.start = it.tile = it.split = it.splits = it.group_index = 0;
-    it.chunk = __builtin_amdgcn_readfirstlane(chunk);
-    int items_before = 0, tiles_before = 0;
+    it.b = it.T = it.L = it.start = it.tile = it.split = it.splits = it.part = it.joint = 0;
+    int items_before = 0, split_before = 0;
     for (int b0 = 0; b0 < c.requests && !it.found; b0 += 64) {
         if (b0) at = paged_lane(c, cut, cap, b0 + lane);
         const int splits = at.units <= chunk ? 1 : (int)(((unsigned)at.units + (unsigned)chunk - 1) / (unsigned)chunk);
-        const int items = at.tiles * splits;
-        const int ie = items_before + paged_scan(items), te = tiles_before + paged_scan(at.tiles);
+        const int items = at.tiles * splits, split = splits > 1 ? items << 16 | at.tiles : 0;
+        const int ie = items_before + paged_scan(items), se = split_before + paged_scan(split);
         const unsigned long long hit = __ballot(want < ie && want >= ie - items);
         if (hit) {
             const int src = __builtin_ctzll(hit);
@@ -177,14 +241,16 @@ __device__ __forceinline__ PagedItem paged_find(const PagedCall& c, const PagedC
             it.T = __builtin_amdgcn_readlane(at.T, src);
             it.L = __builtin_amdgcn_readlane(at.L, src);
             it.splits = __builtin_amdgcn_readlane(splits, src);
-            it.first = __builtin_amdgcn_readlane(ie - items, src);
-            it.tile = (want - it.first) / it.splits;
-            it.first += it.tile * it.splits;
-            it.split = want - it.first;
-            it.group_index = __builtin_amdgcn_readlane(te - at.tiles, src) + it.tile;
+            const int in = want - __builtin_amdgcn_readlane(ie - items, src), tile = in / it.splits;
+            const int before = __builtin_amdgcn_readlane(se - split, src);
+            it.split = in - tile * it.splits;
+            it.part = (before >> 16) + tile * it.splits;
+            it.joint = (before & 0xffff) + tile;
+            // the last tokens, which see the most, first
+            it.tile = __builtin_amdgcn_readlane(at.tiles, src) - 1 - tile;
         }
         items_before = __builtin_amdgcn_readlane(ie, 63);
-        tiles_before = __builtin_amdgcn_readlane(te, 63);
+        split_before = __builtin_amdgcn_readlane(se, 63);
     }
     return it;
 }
@@ -201,6 +267,73 @@ __device__ __forceinline__ bool paged_last(int* counter, int splits) {
     }
     __syncthreads();
     return came == splits - 1;
+}
+
+// The last of a tile's splits joins their parts, each m [ROWS], l [ROWS] and
+// o [ROWS][D] at the reference m: a thread takes 4 dimensions of a row in every
+// `slices`-th split, 8 loads in flight, then the slices are joined in their
+// order.  `lds`: 24 bytes a thread.
+template <int D, bool F32, int ROWS, int THREADS, class Place>
+__device__ __forceinline__ void paged_join(const float* all, int64_t apart, int splits, int nrows, void* lds, void* out,
+                                           Place place) {
+    float4* sum4 = (float4*)lds;
+    float2* stat2 = (float2*)(sum4 + THREADS);
+    const int quads = nrows * (D / 4), slices = max(min(THREADS / quads, splits), 1);
+    for (int q0 = 0; q0 < quads; q0 += THREADS) {
+        const int slice = slices > 1 ? threadIdx.x / quads : 0, e = slices > 1 ? threadIdx.x % quads : q0 + threadIdx.x;
+        const bool on = slice < slices && e < quads;
+        const int rr = on ? e / (D / 4) : 0;
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float top = -INFINITY, sum = 0.0f;
+        for (int s0 = slice; on && s0 < splits; s0 += 8 * slices) {
+            float ms[8], ls[8];
+            float4 vs[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float* p = all + min(s0 + j * slices, splits - 1) * apart;
+                ms[j] = p[rr];
+                ls[j] = p[ROWS + rr];
+                vs[j] = *(const float4*)(p + 2 * ROWS + 4 * e);
+            }
+            float now = top;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (s0 + j * slices >= splits) ms[j] = -INFINITY;
+                now = __builtin_fmaxf(now, ms[j]);
+            }
+            const float base = now == -INFINITY ? 0.0f : now, less = __builtin_amdgcn_exp2f(top - base);
+            top = now;
+            a.x *= less, a.y *= less, a.z *= less, a.w *= less, sum *= less;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (ms[j] == -INFINITY) continue;
+                const float w = __builtin_amdgcn_exp2f(ms[j] - base);
+                a.x += w * vs[j].x, a.y += w * vs[j].y, a.z += w * vs[j].z, a.w += w * vs[j].w, sum += w * ls[j];
+            }
+        }
+        if (slices > 1) {
+            __syncthreads();
+            sum4[threadIdx.x] = a;
+            stat2[threadIdx.x] = make_float2(top, sum);
+            __syncthreads();
+            if (threadIdx.x >= quads) continue;
+            for (int i = 1; i < slices; i++) top = __builtin_fmaxf(top, stat2[i * quads + e].x);
+            const float base = top == -INFINITY ? 0.0f : top;
+            a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            sum = 0.0f;
+            for (int i = 0; i < slices; i++) {
+                const float2 st = stat2[i * quads + e];
+                const float4 v = sum4[i * quads + e];
+                const float w = __builtin_amdgcn_exp2f(st.x - base);
+                a.x += w * v.x, a.y += w * v.y, a.z += w * v.z, a.w += w * v.w, sum += w * st.y;
+            }
+        }
+        if (!on) continue;
+        const float inv = 1.0f / sum;
+        const bool none = sum == 0.0f;
+        paged_store4<F32>(out, place(rr) + 4 * (e % (D / 4)), none ? 0.0f : a.x * inv, none ? 0.0f : a.y * inv,
+                          none ? 0.0f : a.z * inv, none ? 0.0f : a.w * inv);
+    }
 }
 
 // Rows of q that no request owns are zero.

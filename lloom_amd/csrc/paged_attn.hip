@@ -17,9 +17,6 @@
 
 namespace lloom {
 
-typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
 // p is kept times 2^14: halves then hold it down to 2^-38 of the row's largest.
 constexpr float P_SHIFT = 14.0f;
 constexpr int ATT_WAVES = 8, ATT_ROWS = 16, ATT_STEP = 32;
@@ -27,41 +24,6 @@ constexpr int ATT_WAVES = 8, ATT_ROWS = 16, ATT_STEP = 32;
 __device__ __forceinline__ f32x4 mfma16(half8_t a, half8_t b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ half8_t as_half8(uint4 v) { return __builtin_bit_cast(half8_t, v); }
-
-// x as hi + lo, two halves: exact to 2^-22 of x where x is in half's normal range.
-__device__ __forceinline__ void split8(const float (&x)[8], half8_t& hi, half8_t& lo) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const _Float16 h = (_Float16)x[i];
-        hi[i] = h;
-        lo[i] = (_Float16)(x[i] - (float)h);
-    }
-}
-
-// Zeroes the infinities and NaN among N pieces of 8 keys; bit j of the result:
-// there was one at key j.
-template <int N>
-__device__ __forceinline__ uint32_t take_odd(uint4 (&v)[N]) {
-    uint32_t odd = 0;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        uint32_t* w = (uint32_t*)&v[i];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if ((w[j] & 0x7c00u) == 0x7c00u) {
-                odd |= 1u << (2 * j);
-                w[j] &= 0xffff0000u;
-            }
-            if ((w[j] & 0x7c000000u) == 0x7c000000u) {
-                odd |= 2u << (2 * j);
-                w[j] &= 0xffffu;
-            }
-        }
-    }
-    return odd;
-}
-
 template <int D, bool F32>
 __global__ __launch_bounds__(64 * ATT_WAVES) void k_paged_rows(PagedCall c, PagedCut cut, float* parts) {
     constexpr int DC = D / 32, DT = D / 16, PITCH = D + 4;
@@ -124,7 +86,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_paged_rows(PagedCall c, Page
     const auto reach = [&](int p) { return c.window > 0 ? max(max(p, 0) - c.window + 1, 0) : 0; };
     const int win = reach(pos), win_lo = reach(pos_lo);
     const PagedSpan span = paged_span(pos_lo, key_last, c.window, c.sinks, ATT_STEP);
-    const int per = it.splits > 1 ? it.chunk * ATT_WAVES : span.steps;
+    const int per = (span.steps + it.splits - 1) / it.splits;
     const int s_end = (int)min((int64_t)span.steps, (int64_t)(it.split + 1) * per);
     int s = it.split * per + wave;
 
@@ -147,9 +109,10 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_paged_rows(PagedCall c, Page
 
     for (; s < s_end; s += ATT_WAVES) {
         const int v8 = key0 + vk;
-        const bool bad = (unsigned)vp >= (unsigned)c.pages;
+        // a page that no row sees may be none
+        const bool bad = (unsigned)vp >= (unsigned)c.pages && v8 <= key_last && (v8 + 7 >= win_lo || v8 < c.sinks);
         if ((unsigned)kp >= (unsigned)c.pages) kp = 0;
-        if (bad) vp = 0;
+        if ((unsigned)vp >= (unsigned)c.pages) vp = 0;
         bad_page |= bad;
         const uint16_t* kptr = c.k + kp * page_size + head_off + (int64_t)((key0 + kk) & (page - 1)) * D + 8 * g4;
         const uint16_t* vptr = c.v + vp * page_size + head_off + ((int64_t)r << c.page_shift) + (v8 & (page - 1));
@@ -191,21 +154,16 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_paged_rows(PagedCall c, Page
             const uint32_t seen = bad ? 0u : paged_seen8(v8, win, pos_key, c.sinks);
             // keys that some row sees: the others' v may hold anything
             const uint32_t any = bad ? 0u : paged_seen8(v8, win_lo, key_last, c.sinks);
-            uint32_t keep[4];
 #pragma unroll
             for (int j = 0; j < 8; j++) z[j] = seen >> j & 1 ? z[j] : -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 4; j++) keep[j] = (any >> (2 * j) & 1) * 0xffffu | (any >> (2 * j + 1) & 1) * 0xffff0000u;
-#pragma unroll
-            for (int i = 0; i < DT; i++) {
-                vraw[i].x &= keep[0];
-                vraw[i].y &= keep[1];
-                vraw[i].z &= keep[2];
-                vraw[i].w &= keep[3];
-            }
+            for (int i = 0; i < DT; i++) keep8(vraw[i], any);
             // values that are no numbers, where rows of other tokens do not see them:
             // they leave the product (0 times them is no zero) and are added by hand below
-            if (pos_lo != pos_hi) odd = take_odd<DT>(vraw);
+            if (pos_lo != pos_hi) {
+#pragma unroll
+                for (int i = 0; i < DT; i++) odd |= take_odd(vraw[i]);
+            }
         }
         const bool any_odd = edge && __any(odd != 0);
         float top = z[0];
@@ -294,7 +252,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_paged_rows(PagedCall c, Page
     }
     __syncthreads();
     constexpr int PART = ATT_ROWS * (D + 2);
-    float* part = parts + (int64_t)blockIdx.x * PART;
+    float* part = parts + ((int64_t)(it.part + it.split) * c.kv_heads + h) * PART;
     for (int i = threadIdx.x; i < nrows * D; i += 64 * ATT_WAVES) {
         const int rr = i / D, d = i % D;
         float top = stat[0][0][rr];
@@ -321,121 +279,37 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_paged_rows(PagedCall c, Page
             else ((uint16_t*)c.out)[oi] = f32_to_f16(y);
         }
     }
-    if (it.splits <= 1 || !paged_last(c.joins + it.group_index * c.kv_heads + h, it.splits)) return;
-
-    // The last of the splits joins them all: a thread takes 4 dimensions of a row
-    // in every `slices`-th split, 8 loads in flight; then the slices are joined.
-    float4* sum4 = (float4*)&acc[0][0][0];
-    float2* stat2 = (float2*)(sum4 + 64 * ATT_WAVES);
-    const int quads = nrows * (D / 4), slices = max(64 * ATT_WAVES / quads, 1);
-    const float* all = parts + ((int64_t)it.first * c.kv_heads + h) * PART;
-    const int64_t apart = (int64_t)c.kv_heads * PART;
-    for (int q0 = 0; q0 < quads; q0 += 64 * ATT_WAVES) {
-        const int slice = slices > 1 ? threadIdx.x / quads : 0, e = slices > 1 ? threadIdx.x % quads : q0 + threadIdx.x;
-        const bool on = slice < slices && e < quads;
-        const int rr = on ? e / (D / 4) : 0;
-        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float top = -INFINITY, sum = 0.0f;
-        for (int s0 = slice; on && s0 < it.splits; s0 += 8 * slices) {
-            float ms[8], ls[8];
-            float4 vs[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float* p = all + min(s0 + j * slices, it.splits - 1) * apart;
-                ms[j] = p[rr];
-                ls[j] = p[ATT_ROWS + rr];
-                vs[j] = *(const float4*)(p + 2 * ATT_ROWS + 4 * e);
-            }
-            float now = top;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if (s0 + j * slices >= it.splits) ms[j] = -INFINITY;
-                now = __builtin_fmaxf(now, ms[j]);
-            }
-            const float base = now == -INFINITY ? 0.0f : now, less = __builtin_amdgcn_exp2f(top - base);
-            top = now;
-            a.x *= less, a.y *= less, a.z *= less, a.w *= less, sum *= less;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float w = __builtin_amdgcn_exp2f(ms[j] - base);
-                if (ms[j] == -INFINITY) continue;
-                a.x += w * vs[j].x, a.y += w * vs[j].y, a.z += w * vs[j].z, a.w += w * vs[j].w, sum += w * ls[j];
-            }
-        }
-        if (slices > 1) {
-            __syncthreads();
-            sum4[threadIdx.x] = a;
-            stat2[threadIdx.x] = make_float2(top, sum);
-            __syncthreads();
-            if (threadIdx.x >= quads) continue;
-            for (int i = 1; i < slices; i++) top = __builtin_fmaxf(top, stat2[i * quads + e].x);
-            const float base = top == -INFINITY ? 0.0f : top;
-            a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            sum = 0.0f;
-            for (int i = 0; i < slices; i++) {
-                const float2 st = stat2[i * quads + e];
-                const float4 v = sum4[i * quads + e];
-                const float w = __builtin_amdgcn_exp2f(st.x - base);
-                a.x += w * v.x, a.y += w * v.y, a.z += w * v.z, a.w += w * v.w, sum += w * st.y;
-            }
-        }
-        if (!on) continue;
-        const int64_t oi = place(rr) + 4 * (e % (D / 4));
-        const bool none = sum == 0.0f;
-        a.x = none ? 0.0f : a.x / sum, a.y = none ? 0.0f : a.y / sum, a.z = none ? 0.0f : a.z / sum, a.w = none ? 0.0f : a.w / sum;
-        if constexpr (F32) {
-            *(float4*)((float*)c.out + oi) = a;
-        } else {
-            *(uint2*)((uint16_t*)c.out + oi) = make_uint2(f32_to_f16(a.x) | (uint32_t)f32_to_f16(a.y) << 16,
-                                                          f32_to_f16(a.z) | (uint32_t)f32_to_f16(a.w) << 16);
-        }
-    }
+    if (it.splits > 1 && paged_last(c.joins + it.joint * c.kv_heads + h, it.splits))
+        paged_join<D, F32, ATT_ROWS, 64 * ATT_WAVES>(parts + ((int64_t)it.part * c.kv_heads + h) * PART,
+                                                     (int64_t)c.kv_heads * PART, it.splits, nrows, acc, c.out, place);
 }
 
 // One workgroup a CU: a second round costs more than the last of the balance
 // (512: 26.5 against 20.0 us for 32 requests, 62 MB; 119 against 105 us for 537 MB
 // of one request).
-constexpr int ATT_TARGET_SHIFT = 8, ATT_TARGET = 1 << ATT_TARGET_SHIFT;
-
-static int64_t tiles_most(int64_t tokens, int64_t requests, int group, int rows) {
-    return tokens * group / rows + (requests < tokens ? requests : tokens);
-}
-
-static PagedCut rows_cut(const PagedCall& c, int route, int few) {
-    PagedCut cut{4, 8, 1, ATT_TARGET_SHIFT, (ATT_ROWS - 1) / c.group + 1, route, few, 0};
-    cut.split = tiles_most(c.tokens, c.requests, c.group, ATT_ROWS) * c.kv_heads < ATT_TARGET;
-    return cut;
-}
-
-size_t paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int kv_heads, int group, int dim,
-                                       int max_new) {
-    (void)max_new;
-    const int64_t tiles = tiles_most(tokens, requests, group, ATT_ROWS) * kv_heads;
-    if (tiles >= ATT_TARGET) return 0;
-    return (size_t)(ATT_TARGET + tiles) * ATT_ROWS * (dim + 2) * sizeof(float);
-}
+constexpr int ATT_TARGET_SHIFT = 8;
 
 template <int D, bool F32>
-static hipError_t rows_as(const PagedCall& c, const PagedCut& cut, float* parts, hipStream_t s) {
-    const int64_t tiles = tiles_most(c.tokens, c.requests, c.group, ATT_ROWS) * c.kv_heads;
-    // no more items than the tables have units of keys for
-    const int64_t keys = (int64_t)c.max_blocks << c.page_shift, units = (keys + (1 << cut.unit_shift) - 1) >> cut.unit_shift;
-    const int64_t grid = !cut.split ? tiles : units * tiles < ATT_TARGET + tiles ? units * tiles : ATT_TARGET + tiles;
+static hipError_t rows_as(const PagedCall& c, const PagedCut& cut, int64_t grid, float* parts, hipStream_t s) {
     hipLaunchKernelGGL((k_paged_rows<D, F32>), dim3((unsigned)grid), dim3(64 * ATT_WAVES), 0, s, c, cut, parts);
     return hipGetLastError();
 }
 
-hipError_t launch_paged_attention(int act, int dim, const PagedCall& c, int max_new, void* ws, hipStream_t s) {
-    (void)max_new;
-    const PagedCut cut = rows_cut(c, 0, 0);
+hipError_t launch_paged_rows(int act, int dim, const PagedCall& c, int route, int few, void* ws, hipStream_t s) {
+    const PagedCut cut{4, 8, 1, ATT_TARGET_SHIFT, (ATT_ROWS - 1) / c.group + 1, route, few};
+    const int64_t grid = paged_items_most(c, cut);
     float* parts = (float*)ws;
     switch (dim) {
-        case 64: return act == T_F32 ? rows_as<64, true>(c, cut, parts, s) : rows_as<64, false>(c, cut, parts, s);
-        case 96: return act == T_F32 ? rows_as<96, true>(c, cut, parts, s) : rows_as<96, false>(c, cut, parts, s);
-        case 128: return act == T_F32 ? rows_as<128, true>(c, cut, parts, s) : rows_as<128, false>(c, cut, parts, s);
-        case 256: return act == T_F32 ? rows_as<256, true>(c, cut, parts, s) : rows_as<256, false>(c, cut, parts, s);
+        case 64: return act == T_F32 ? rows_as<64, true>(c, cut, grid, parts, s) : rows_as<64, false>(c, cut, grid, parts, s);
+        case 96: return act == T_F32 ? rows_as<96, true>(c, cut, grid, parts, s) : rows_as<96, false>(c, cut, grid, parts, s);
+        case 128: return act == T_F32 ? rows_as<128, true>(c, cut, grid, parts, s) : rows_as<128, false>(c, cut, grid, parts, s);
+        case 256: return act == T_F32 ? rows_as<256, true>(c, cut, grid, parts, s) : rows_as<256, false>(c, cut, grid, parts, s);
     }
     return hipErrorInvalidValue;
+}
+
+size_t paged_rows_workspace_bytes(int kv_heads, int dim) {
+    return ((size_t)paged_parts(ATT_TARGET_SHIFT) + kv_heads) * ATT_ROWS * (dim + 2) * sizeof(float);
 }
 
 }  // namespace lloom

@@ -254,6 +254,36 @@ def test_bad_pages_are_passed_over_and_reported(name, act):
 
 
 @pytest.mark.parametrize("act", [F32, F16])
+@pytest.mark.parametrize("cached,new,dim", [(900, 1, 64), (900, 70, 128), (900, 40, 256), (300, 300, 96)])
+def test_pages_that_no_token_sees_may_be_none(cached, new, dim, act):
+    """A server frees the pages between the first tokens and the window: nothing is read or reported there."""
+    window, sinks, page = 100, 5, 16
+    s = R.case([cached, 20], [new, 3], page, 2, 2, dim, act, device=DEV)
+    want = _run(s, window=window, sinks=sinks)
+    for i in range(len(s["tables"][0])):
+        if i * page >= sinks and (i + 1) * page <= cached - window + 1:
+            s["tables"][0][i] = -1
+    assert -1 in s["tables"][0]
+    s["t_tables"] = _ints(s["tables"])
+    got = _run(s, window=window, sinks=sinks)
+    L.paged_check()
+    assert torch.equal(got, want)
+    _check(s, got, window, sinks)
+
+
+@pytest.mark.parametrize("act", [F32, F16])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("cached,new,page,group", [(0, 1, 16, 64), (63, 65, 16, 1), (1000, 129, 32, 1), (127, 16, 4096, 8),
+                                                   (2500, 33, 128, 4), (5, 260, 16, 3)])
+def test_attention_of_one_chunk(cached, new, page, group, dim, act):
+    """One request, in whichever way its rows and keys are cut: tiles and steps that are just full, and just over."""
+    s = R.case([cached], [new], page, 2, group, dim, act, seed=new, device=DEV)
+    _check(s, _run(s, max_new=new))
+    _check(s, _run(s, window=77, sinks=3), 77, 3)
+    L.paged_check()
+
+
+@pytest.mark.parametrize("act", [F32, F16])
 def test_lengths_past_the_tables_are_reported(act):
     s = R.case([90], [20], 16, 1, 2, 64, act, device=DEV)
     s["tables"] = [s["tables"][0][:3]]
