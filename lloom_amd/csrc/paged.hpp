@@ -50,6 +50,7 @@ struct PagedCall {
 // route: 0 every request, 1 those of at most `few` rows, 2 the others.
 struct PagedCut {
     int row_shift, unit_shift, unit_min, target_shift, more, route, few;
+    int slots;  // workgroups that the card holds at once, two a CU; 0: not told
 };
 // A split tile has more units than a 2^target_shift-th of all, so that there are
 // under 2^target_shift of them and under twice as many items of theirs.
@@ -175,6 +176,12 @@ __device__ __forceinline__ uint32_t take_odd(uint4& v) {
     }
     return odd;
 }
+// Not zero: there is an infinity or a NaN among 8 keys' values.  An exponent of all
+// ones and 1 more is the sign's bit.
+__device__ __forceinline__ uint32_t odd_mark(const uint4& v) {
+    const auto mark = [](uint32_t w) { return (w & 0x7c007c00u) + 0x04000400u; };
+    return (mark(v.x) | mark(v.y) | mark(v.z) | mark(v.w)) & 0x80008000u;
+}
 // Zeroes the values of the keys whose bit is not set.
 __device__ __forceinline__ void keep8(uint4& v, uint32_t bits) {
     uint32_t* w = (uint32_t*)&v;
@@ -232,6 +239,12 @@ __device__ __forceinline__ PagedItem paged_find(const PagedCall& c, const PagedC
         const int splits = at.units <= chunk ? 1 : (int)(((unsigned)at.units + (unsigned)chunk - 1) / (unsigned)chunk);
         const int items = at.tiles * splits, split = splits > 1 ? items << 16 | at.tiles : 0;
         const int ie = items_before + paged_scan(items), se = split_before + paged_scan(split);
+        if (cut.slots && c.requests <= 64) {
+            // Two workgroups a CU, and the longest items come first: the second ones in
+            // turn, so that the longest of them is not with the longest of the first.
+            const int all = __builtin_amdgcn_readlane(ie, 63), first = (cut.slots / 2) / c.kv_heads;
+            if (all * c.kv_heads <= cut.slots && want >= first && want < all) want = first + all - 1 - want;
+        }
         const unsigned long long hit = __ballot(want < ie && want >= ie - items);
         if (hit) {
             const int src = __builtin_ctzll(hit);
@@ -255,84 +268,121 @@ __device__ __forceinline__ PagedItem paged_find(const PagedCall& c, const PagedC
     return it;
 }
 
-// One workgroup's part of a (tile, key head) that several share is written: true
-// in the one that comes last, which then sees the others' parts.  Its counter
-// is zero before and after.
+// The parts of a tile that several workgroups share are stored and loaded at the
+// agent's scope: past the L2, which each XCD has one of.  A release of ordinary
+// stores writes the whole L2 back instead (537 MB of one request's cache 106 us that
+// way, 100 this).
+__device__ __forceinline__ void part_store(float* p, float v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void part_store4(float* p, float x, float y, float z, float w) {
+    uint64_t* q = (uint64_t*)p;
+    const auto two = [](float a, float b) { return (uint64_t)__builtin_bit_cast(uint32_t, b) << 32 | __builtin_bit_cast(uint32_t, a); };
+    __hip_atomic_store(q, two(x, y), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(q + 1, two(z, w), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float part_load(const float* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float4 part_load4(const float* p) {
+    const uint64_t a = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint64_t b = __hip_atomic_load((const uint64_t*)p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float4(__builtin_bit_cast(float, (uint32_t)a), __builtin_bit_cast(float, (uint32_t)(a >> 32)),
+                       __builtin_bit_cast(float, (uint32_t)b), __builtin_bit_cast(float, (uint32_t)(b >> 32)));
+}
+
+// A workgroup's part is stored: true in the last of them to come, which then loads
+// the others'.  Every wave waits until its stores are done before any of them is
+// counted.  The counter is zero before and after.
 __device__ __forceinline__ bool paged_last(int* counter, int splits) {
     __shared__ int came;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
-        came = __hip_atomic_fetch_add(counter, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        came = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (came == splits - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
+    asm volatile("" ::: "memory");
     return came == splits - 1;
 }
 
 // The last of a tile's splits joins their parts, each m [ROWS], l [ROWS] and
-// o [ROWS][D] at the reference m: a thread takes 4 dimensions of a row in every
-// `slices`-th split, 8 loads in flight, then the slices are joined in their
+// o [ROWS][D] at the reference m: a thread takes 4 dimensions of QN rows in every
+// `slices`-th split, QN x SN loads in flight, then the slices are joined in their
 // order.  `lds`: 24 bytes a thread.
-template <int D, bool F32, int ROWS, int THREADS, class Place>
+template <int D, bool F32, int ROWS, int THREADS, int QN, int SN, class Place>
 __device__ __forceinline__ void paged_join(const float* all, int64_t apart, int splits, int nrows, void* lds, void* out,
                                            Place place) {
     float4* sum4 = (float4*)lds;
     float2* stat2 = (float2*)(sum4 + THREADS);
     const int quads = nrows * (D / 4), slices = max(min(THREADS / quads, splits), 1);
-    for (int q0 = 0; q0 < quads; q0 += THREADS) {
-        const int slice = slices > 1 ? threadIdx.x / quads : 0, e = slices > 1 ? threadIdx.x % quads : q0 + threadIdx.x;
-        const bool on = slice < slices && e < quads;
-        const int rr = on ? e / (D / 4) : 0;
-        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float top = -INFINITY, sum = 0.0f;
-        for (int s0 = slice; on && s0 < splits; s0 += 8 * slices) {
-            float ms[8], ls[8];
-            float4 vs[8];
+    for (int q0 = 0; q0 < quads; q0 += QN * THREADS) {
+        const int slice = slices > 1 ? threadIdx.x / quads : 0, e0 = slices > 1 ? threadIdx.x % quads : q0 + threadIdx.x;
+        const bool on = slice < slices && e0 < quads;
+        float4 a[QN];
+        float top[QN], sum[QN];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float* p = all + min(s0 + j * slices, splits - 1) * apart;
-                ms[j] = p[rr];
-                ls[j] = p[ROWS + rr];
-                vs[j] = *(const float4*)(p + 2 * ROWS + 4 * e);
-            }
-            float now = top;
+        for (int i = 0; i < QN; i++) a[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), top[i] = -INFINITY, sum[i] = 0.0f;
+        for (int s0 = slice; on && s0 < splits; s0 += SN * slices) {
+            float ms[QN][SN], ls[QN][SN];
+            float4 vs[QN][SN];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if (s0 + j * slices >= splits) ms[j] = -INFINITY;
-                now = __builtin_fmaxf(now, ms[j]);
-            }
-            const float base = now == -INFINITY ? 0.0f : now, less = __builtin_amdgcn_exp2f(top - base);
-            top = now;
-            a.x *= less, a.y *= less, a.z *= less, a.w *= less, sum *= less;
+            for (int i = 0; i < QN; i++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if (ms[j] == -INFINITY) continue;
-                const float w = __builtin_amdgcn_exp2f(ms[j] - base);
-                a.x += w * vs[j].x, a.y += w * vs[j].y, a.z += w * vs[j].z, a.w += w * vs[j].w, sum += w * ls[j];
+                for (int j = 0; j < SN; j++) {
+                    const int e = min(e0 + i * THREADS, quads - 1), rr = e / (D / 4);
+                    const float* p = all + min(s0 + j * slices, splits - 1) * apart;
+                    ms[i][j] = part_load(p + rr);
+                    ls[i][j] = part_load(p + ROWS + rr);
+                    vs[i][j] = part_load4(p + 2 * ROWS + 4 * e);
+                }
+#pragma unroll
+            for (int i = 0; i < QN; i++) {
+                float now = top[i];
+#pragma unroll
+                for (int j = 0; j < SN; j++) {
+                    if (s0 + j * slices >= splits) ms[i][j] = -INFINITY;
+                    now = __builtin_fmaxf(now, ms[i][j]);
+                }
+                const float base = now == -INFINITY ? 0.0f : now, less = __builtin_amdgcn_exp2f(top[i] - base);
+                top[i] = now;
+                a[i].x *= less, a[i].y *= less, a[i].z *= less, a[i].w *= less, sum[i] *= less;
+#pragma unroll
+                for (int j = 0; j < SN; j++) {
+                    if (ms[i][j] == -INFINITY) continue;
+                    const float w = __builtin_amdgcn_exp2f(ms[i][j] - base);
+                    a[i].x += w * vs[i][j].x, a[i].y += w * vs[i][j].y, a[i].z += w * vs[i][j].z, a[i].w += w * vs[i][j].w;
+                    sum[i] += w * ls[i][j];
+                }
             }
         }
-        if (slices > 1) {
+        if (slices > 1) {  // then one quad a thread
             __syncthreads();
-            sum4[threadIdx.x] = a;
-            stat2[threadIdx.x] = make_float2(top, sum);
+            sum4[threadIdx.x] = a[0];
+            stat2[threadIdx.x] = make_float2(top[0], sum[0]);
             __syncthreads();
             if (threadIdx.x >= quads) continue;
-            for (int i = 1; i < slices; i++) top = __builtin_fmaxf(top, stat2[i * quads + e].x);
-            const float base = top == -INFINITY ? 0.0f : top;
-            a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            sum = 0.0f;
+            for (int i = 1; i < slices; i++) top[0] = __builtin_fmaxf(top[0], stat2[i * quads + e0].x);
+            const float base = top[0] == -INFINITY ? 0.0f : top[0];
+            a[0] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            sum[0] = 0.0f;
             for (int i = 0; i < slices; i++) {
-                const float2 st = stat2[i * quads + e];
-                const float4 v = sum4[i * quads + e];
+                const float2 st = stat2[i * quads + e0];
+                const float4 v = sum4[i * quads + e0];
                 const float w = __builtin_amdgcn_exp2f(st.x - base);
-                a.x += w * v.x, a.y += w * v.y, a.z += w * v.z, a.w += w * v.w, sum += w * st.y;
+                a[0].x += w * v.x, a[0].y += w * v.y, a[0].z += w * v.z, a[0].w += w * v.w, sum[0] += w * st.y;
             }
         }
-        if (!on) continue;
-        const float inv = 1.0f / sum;
-        const bool none = sum == 0.0f;
-        paged_store4<F32>(out, place(rr) + 4 * (e % (D / 4)), none ? 0.0f : a.x * inv, none ? 0.0f : a.y * inv,
-                          none ? 0.0f : a.z * inv, none ? 0.0f : a.w * inv);
+#pragma unroll
+        for (int i = 0; i < QN; i++) {
+            const int e = e0 + i * THREADS;
+            if (!on || e >= quads) continue;
+            const float inv = 1.0f / sum[i];
+            const bool none = sum[i] == 0.0f;
+            paged_store4<F32>(out, place(e / (D / 4)) + 4 * (e % (D / 4)), none ? 0.0f : a[i].x * inv, none ? 0.0f : a[i].y * inv,
+                              none ? 0.0f : a[i].z * inv, none ? 0.0f : a[i].w * inv);
+        }
     }
 }
 

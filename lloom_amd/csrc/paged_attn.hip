@@ -267,10 +267,10 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_paged_rows(PagedCall c, Page
             sum += stat[w][1][rr] * e;
         }
         if (it.splits > 1) {
-            part[2 * ATT_ROWS + i] = v;
+            part_store(part + 2 * ATT_ROWS + i, v);
             if (d == 0) {
-                part[rr] = top;
-                part[ATT_ROWS + rr] = sum;
+                part_store(part + rr, top);
+                part_store(part + ATT_ROWS + rr, sum);
             }
         } else {
             const int64_t oi = place(rr) + d;
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_paged_rows(PagedCall c, Page
         }
     }
     if (it.splits > 1 && paged_last(c.joins + it.joint * c.kv_heads + h, it.splits))
-        paged_join<D, F32, ATT_ROWS, 64 * ATT_WAVES>(parts + ((int64_t)it.part * c.kv_heads + h) * PART,
+        paged_join<D, F32, ATT_ROWS, 64 * ATT_WAVES, 1, 8>(parts + ((int64_t)it.part * c.kv_heads + h) * PART,
                                                      (int64_t)c.kv_heads * PART, it.splits, nrows, acc, c.out, place);
 }
 
@@ -296,7 +296,7 @@ static hipError_t rows_as(const PagedCall& c, const PagedCut& cut, int64_t grid,
 }
 
 hipError_t launch_paged_rows(int act, int dim, const PagedCall& c, int route, int few, void* ws, hipStream_t s) {
-    const PagedCut cut{4, 8, 1, ATT_TARGET_SHIFT, (ATT_ROWS - 1) / c.group + 1, route, few};
+    const PagedCut cut{4, 8, 1, ATT_TARGET_SHIFT, (ATT_ROWS - 1) / c.group + 1, route, few, 0};
     const int64_t grid = paged_items_most(c, cut);
     float* parts = (float*)ws;
     switch (dim) {

@@ -1,8 +1,7 @@
 // paged_tile.hip -- attention of chunks of new tokens over the paged cache.
 //
-// A workgroup takes 128 rows of a request and a key head.  Its waves are 4 groups
-// of 32 rows times KG groups of keys; a step of the workgroup is KG * STEP keys,
-// whose K and V come into LDS by global_load_lds a step ahead of their use.
+// A workgroup takes 128 rows of a request and a key head, 32 a wave; a step is 64
+// keys, whose K and V come into LDS by global_load_lds a step ahead of their use.
 // Both products run transposed on 32x32x16 MFMAs, S^T = K Q^T (A: 32 keys x 16
 // dims) and O^T = V^T P^T (A: 32 dims x 16 keys).  A lane of S^T's result holds
 // of one row the keys 8 (j / 4) + 4 half + j % 4, j = 0 .. 15; with K's rows taken
@@ -15,6 +14,7 @@
 namespace lloom {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void lds_void;
 
 __device__ __forceinline__ f32x16 mfma32(half8_t a, half8_t b, f32x16 c) {
@@ -27,34 +27,29 @@ __device__ __forceinline__ void lds_load16(const void* g, uint8_t* lds_piece) {
 
 template <int D, bool F32>
 struct PagedTile {
-    static constexpr int ROWS = 128, RG = 4;             // rows, and groups of 32 of them
-    static constexpr int STEP = D <= 128 ? 64 : 32;      // keys of a wave in a step
-    static constexpr int KG = D == 256 && F32 ? 1 : 2;   // groups of keys
-    static constexpr int WAVES = RG * KG, THREADS = 64 * WAVES;
-    static constexpr int KEYS = KG * STEP, KEY_SHIFT = KEYS == 128 ? 7 : KEYS == 64 ? 6 : 5;
+    static constexpr int ROWS = 128, WAVES = 4, THREADS = 64 * WAVES;
+    static constexpr int KEYS = 64, KEY_SHIFT = 6;       // of a step
     static constexpr int PIECES = D == 96 ? 16 : D / 8;  // 16-byte pieces of a row of K in LDS (96: a quarter unused)
     static constexpr int K_BYTES = KEYS * PIECES * 16, V_BYTES = KEYS * D * 2, STAGE = K_BYTES + V_BYTES;
-    static constexpr int GROUPS = KEYS / 16, SHARE = WAVES / GROUPS;  // waves that load 16 keys together
-    static constexpr int K_LOADS = PIECES / 4 / SHARE, V_LOADS = D / 32;
-    static constexpr int V_EACH = (V_LOADS + SHARE - 1) / SHARE;
-    static constexpr int JOIN = RG * (D / 32) * 16 * 64 * 4 + RG * 64 * 8;  // the second key group's sums
-    static constexpr int LDS = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
+    static constexpr int K_LOADS = PIECES / 4, V_LOADS = D / 32;  // of 1 KB a wave: 16 keys of K; 8 dims of V each
+    // operands read ahead: tiles of 32 keys of K, runs of 16 keys of V
+    static constexpr int K_AHEAD = F32 || D == 256 ? 1 : 2, V_AHEAD = F32 || D == 256 ? 2 : 4;
     static constexpr int PART = ROWS * (D + 2);
     // p is kept times 2^SHIFT, and the reference it is relative to stands until a
     // row's largest passes it by 2^SLACK: rescaling the sums is then rare.  Halves
-    // hold 2^(SHIFT + SLACK) and, as normal numbers, down to 2^-(14 + SHIFT).
-    static constexpr float SHIFT = F32 ? 12.0f : 8.0f, SLACK = F32 ? 3.0f : 7.0f;
-    static_assert(GROUPS * SHARE == WAVES && (PIECES / 4) % SHARE == 0, "loads by 16 keys");
+    // hold 2^(SHIFT + SLACK), and below 2^-(14 + SHIFT) of the reference they are off
+    // by 2^-33 of it at most.
+    static constexpr float SHIFT = 8.0f, SLACK = 7.0f;
 };
 
 template <int D, bool F32>
-__global__ __launch_bounds__((PagedTile<D, F32>::THREADS)) void k_paged_tile(PagedCall c, PagedCut cut, float* parts) {
+__global__ __launch_bounds__((PagedTile<D, F32>::THREADS), D == 256 ? 1 : 2) void k_paged_tile(PagedCall c, PagedCut cut, float* parts) {
     using C = PagedTile<D, F32>;
-    constexpr int DC = D / 16, DT = D / 32, ST = C::STEP / 32;
-    __shared__ __align__(16) uint8_t lds[C::LDS];
-    __shared__ int bad_group[2][C::GROUPS];
+    constexpr int DC = D / 16, DT = D / 32, ST = 2;
+    __shared__ __align__(16) uint8_t lds[2 * C::STAGE];
+    __shared__ int bad_group[2][4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r = lane & 31, half = lane >> 5, rg = wave % C::RG, kg = wave / C::RG;
+    const int r = lane & 31, half = lane >> 5;
     if (cut.route == 0) paged_zero_tail<F32>(c, D, blockIdx.x, gridDim.x);
     const PagedItem it = paged_find(c, cut, blockIdx.x / c.kv_heads);
     if (!it.found) return;
@@ -71,11 +66,11 @@ __global__ __launch_bounds__((PagedTile<D, F32>::THREADS)) void k_paged_tile(Pag
     const int cap = paged_key_cap(c), key_last = min(pos0 + paged_token(c, row + nrows - 1), cap);
     const auto reach = [&](int p) { return c.window > 0 ? max(max(p, 0) - c.window + 1, 0) : 0; };
     // the lane's row, and the wave's rows
-    const int mine = min(32 * rg + r, nrows - 1), tok = paged_token(c, row + mine), pos = pos0 + tok;
+    const int mine = min(32 * wave + r, nrows - 1), tok = paged_token(c, row + mine), pos = pos0 + tok;
     const int tile_lo = reach(pos0);
-    const bool any_rows = 32 * rg < nrows;
-    const int pos_lo = pos0 + paged_token(c, row + min(32 * rg, nrows - 1));
-    const int pos_hi = pos0 + paged_token(c, row + min(32 * rg + 31, nrows - 1));
+    const bool any_rows = 32 * wave < nrows;
+    const int pos_lo = pos0 + paged_token(c, row + min(32 * wave, nrows - 1));
+    const int pos_hi = pos0 + paged_token(c, row + min(32 * wave + 31, nrows - 1));
     const int pos_key = min(pos, cap), wave_last = min(pos_hi, cap), win = reach(pos), win_lo = reach(pos_lo), win_hi = reach(pos_hi);
 
     // q as B operands, dims 16 c + 8 half .., its sign turned where the scale is negative
@@ -124,44 +119,52 @@ __global__ __launch_bounds__((PagedTile<D, F32>::THREADS)) void k_paged_tile(Pag
     bool bad_page = it.L - 1 > cap;
     const auto first_key = [&](int i) { return C::KEYS * (i < span.sink_steps ? i : span.skip + i); };
 
-    // This wave's loads of a step: K and V of 16 keys (a share of them).  In LDS, K
-    // [key][piece ^ key's low bits] and V [16 keys][dim][the two runs of 8 keys, in
-    // turn every 8 dims]: 16 lanes that read one piece of 16 keys, or one run of 16
-    // dims, hit all banks once.
-    const int group = wave / C::SHARE, share = wave % C::SHARE;
-    uint32_t k_off[C::K_LOADS], v_off[C::V_EACH];
+    // This wave's loads of a step.  In LDS, K [key][piece ^ key's low bits] and V
+    // [64 keys][dim][run of 8 keys ^ dim / 2's low bits]: 16 lanes that read one piece
+    // of 16 keys, or one run of 16 dims, hit all banks once.  A load of V takes whole
+    // runs of 64 keys of a dim from one page, or from as many as hold them: a lane's
+    // run is one of two, by whether its 8 dims are an even or an odd 8.
+    uint32_t k_off[C::K_LOADS];
 #pragma unroll
     for (int i = 0; i < C::K_LOADS; i++) {
-        const int at = (share * C::K_LOADS + i) * 64 + lane, key = at / C::PIECES;
+        const int at = i * 64 + lane, key = at / C::PIECES;
         int piece = (at % C::PIECES) ^ (C::PIECES == 8 ? key >> 1 & 7 : key & 15);
         if (piece >= D / 8) piece -= 4;  // a head of 96: any other
         k_off[i] = key * D * 2 + piece * 16;
     }
-#pragma unroll
-    for (int i = 0; i < C::V_EACH; i++) {
-        const int dim = min(share * C::V_EACH + i, C::V_LOADS - 1) * 32 + (lane >> 1);
-        v_off[i] = (uint32_t)(dim << (c.page_shift + 1)) + ((lane & 1) ^ (dim >> 3 & 1)) * 16;
-    }
-    const auto page_of = [&](int s) { return table[min(first_key(s) + 16 * group, key_last) >> c.page_shift]; };
-    const auto load = [&](int s, int pg, int buf) {
-        const int key = first_key(s) + 16 * group;
-        pg = __builtin_amdgcn_readfirstlane(pg);
+    const int v_first = wave * C::V_LOADS;           // its first 8 dims of V
+    const int run = 8 * ((lane & 7) ^ (lane >> 4));  // its run in an even 8 dims; 32 keys off in an odd 8
+    const uint32_t v_row = (uint32_t)(lane >> 3) << (c.page_shift + 1);
+    struct Pages {
+        int k, v[2];
+    };
+    const auto pages_of = [&](int s) {
+        const int key = first_key(s);
+        const auto of = [&](int k) { return table[min(key + k, key_last) >> c.page_shift]; };
+        return Pages{of(16 * wave), {of(run), of(run ^ 32)}};
+    };
+    const auto load = [&](int s, const Pages& pg, uint8_t* to, int* bad_to) __attribute__((always_inline)) {
+        const int key0 = first_key(s), key = key0 + 16 * wave;
+        int kp = __builtin_amdgcn_readfirstlane(pg.k);
         // a page that no row sees may be none
         const bool seen = key <= key_last && (key + 15 >= tile_lo || key < c.sinks);
-        const bool bad = (unsigned)pg >= (unsigned)c.pages && seen;
-        if ((unsigned)pg >= (unsigned)c.pages) pg = 0;
+        const bool bad = (unsigned)kp >= (unsigned)c.pages && seen;
+        if ((unsigned)kp >= (unsigned)c.pages) kp = 0;
         bad_page |= bad;
-        if (lane == 0) bad_group[buf][group] = bad;
-        const uint8_t* k = (const uint8_t*)(c.k + pg * page_size + head_off + (int64_t)(key & (page - 1)) * D);
-        const uint8_t* v = (const uint8_t*)(c.v + pg * page_size + head_off + (key & (page - 1)));
-        uint8_t* to = lds + buf * C::STAGE;
+        if (lane == 0) bad_to[wave] = bad;
+        const uint8_t* k = (const uint8_t*)(c.k + kp * page_size + head_off + (int64_t)(key & (page - 1)) * D);
 #pragma unroll
         for (int i = 0; i < C::K_LOADS; i++)
-            lds_load16(k + k_off[i], to + (group * (C::PIECES / 4) + share * C::K_LOADS + i) * 1024);
+            lds_load16(k + k_off[i], to + (wave * C::K_LOADS + i) * 1024);
+        const uint8_t* v[2];
 #pragma unroll
-        for (int i = 0; i < C::V_EACH; i++)
-            if (share * C::V_EACH + i < C::V_LOADS)
-                lds_load16(v + v_off[i], to + C::K_BYTES + (group * C::V_LOADS + share * C::V_EACH + i) * 1024);
+        for (int i = 0; i < 2; i++) {
+            const int vp = (unsigned)pg.v[i] >= (unsigned)c.pages ? 0 : pg.v[i];
+            v[i] = (const uint8_t*)(c.v + vp * page_size + head_off + ((key0 + (run ^ (32 * i))) & (page - 1))) + v_row;
+        }
+#pragma unroll
+        for (int i = 0; i < C::V_LOADS; i++)
+            lds_load16(((v_first + i) & 1 ? v[1] : v[0]) + ((uint32_t)(v_first + i) << (c.page_shift + 4)), to + C::K_BYTES + (v_first + i) * 1024);
     };
 
     f32x16 o[DT];
@@ -175,188 +178,275 @@ __global__ __launch_bounds__((PagedTile<D, F32>::THREADS)) void k_paged_tile(Pag
     // + r % 4 of a tile of K, dim r of a tile of V
     const int kkey = (r & 16) + (r >> 2 & 1) * 8 + (r >> 3 & 1) * 4 + (r & 3);
     const uint32_t k_turn = ((uint32_t)(half ^ (C::PIECES == 8 ? kkey >> 1 & 7 : kkey & 15))) << 4;
-    const uint32_t k_base = (uint32_t)(kg * C::STEP + kkey) * C::PIECES * 16;
-    const uint32_t v_base = C::K_BYTES + (uint32_t)kg * C::STEP * D * 2 + (r * 2 + (half ^ (r >> 3 & 1))) * 16;
+    const uint32_t k_base = (uint32_t)kkey * C::PIECES * 16;
+    const uint32_t v_turn = (uint32_t)(half ^ (r >> 1 & 7)) << 4, v_base = C::K_BYTES + r * 128;
+    const auto v_at = [&](const uint8_t* at, int g, int i) { return *(const uint4*)(at + v_base + (v_turn ^ (g << 5)) + i * 4096); };
 
-    // One step of this wave's keys; EDGE: some row does not see some of them.
-    const auto step = [&](const uint8_t* at, int key0, uint32_t bad, auto edge_c) {
-        constexpr bool EDGE = decltype(edge_c)::value;
-        f32x16 z[ST];
-#pragma unroll
-        for (int t = 0; t < ST; t++) {
-#pragma unroll
-            for (int j = 0; j < 16; j++) z[t][j] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < DC; i++) {
-                const half8_t k = as_half8(*(const uint4*)(at + k_base + (k_turn ^ (i << 5)) + t * 32 * C::PIECES * 16));
-                z[t] = mfma32(k, qh[i], z[t]);
-                if constexpr (F32) z[t] = mfma32(k, ql[i], z[t]);
-            }
-        }
-        uint32_t any[2 * ST];  // keys that some row of the wave sees: the others' v may hold anything
-        if constexpr (EDGE) {
-#pragma unroll
-            for (int g = 0; g < 2 * ST; g++) {
-                const int key = key0 + 16 * g + 8 * half;
-                const bool out = bad >> g & 1;
-                const uint32_t seen = out ? 0u : paged_seen8(key, win, pos_key, c.sinks);
-                any[g] = out ? 0u : paged_seen8(key, win_lo, wave_last, c.sinks);
-#pragma unroll
-                for (int j = 0; j < 8; j++) z[g >> 1][8 * (g & 1) + j] = seen >> j & 1 ? z[g >> 1][8 * (g & 1) + j] : -INFINITY;
-            }
-        }
+    const auto k_at = [&](const uint8_t* at, int t, int i) {
+        return as_half8(*(const uint4*)(at + k_base + (k_turn ^ (i << 5)) + t * 32 * C::PIECES * 16));
+    };
+    const auto largest = [&](const f32x16 (&z)[ST]) {
         float top = z[0][0];
 #pragma unroll
         for (int t = 0; t < ST; t++)
 #pragma unroll
             for (int j = 0; j < 16; j++) top = __builtin_fmaxf(top, z[t][j]);
-        top = __builtin_fmaxf(top, partner32(top)) * factor;
-        if (__any(top > m + C::SLACK)) {
-            const float now = __builtin_fmaxf(m, top);
-            const float less = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);
-            m = now;
-            l *= less;
+        return __builtin_fmaxf(top, partner32(top)) * factor;
+    };
+
+    // z = K Q^T of a step.
+    const auto scores = [&](const uint8_t* at, f32x16 (&z)[ST]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < DT; i++)
+        for (int t = 0; t < ST; t++)
 #pragma unroll
-                for (int j = 0; j < 16; j++) o[i][j] *= less;
+            for (int j = 0; j < 16; j++) z[t][j] = 0.0f;
+#pragma unroll
+        for (int t0 = 0; t0 < ST; t0 += C::K_AHEAD) {
+            half8_t kf[C::K_AHEAD][DC];
+#pragma unroll
+            for (int i = 0; i < DC; i++)
+#pragma unroll
+                for (int t = 0; t < C::K_AHEAD; t++) kf[t][i] = k_at(at, t0 + t, i);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < DC; i++)
+#pragma unroll
+                for (int t = 0; t < C::K_AHEAD; t++) {
+                    z[t0 + t] = mfma32(kf[t][i], qh[i], z[t0 + t]);
+                    if constexpr (F32) z[t0 + t] = mfma32(kf[t][i], ql[i], z[t0 + t]);
+                }
         }
-        const float base = m == -INFINITY ? 0.0f : m - C::SHIFT;
+    };
+    // The weights of 16 keys, added to l, as B operands.
+    const auto weights = [&](const f32x16 (&z)[ST], int g, float base, half8_t& ph, half8_t& pl) __attribute__((always_inline)) {
+        float p[8];
 #pragma unroll
-        for (int g = 0; g < 2 * ST; g++) {
-            float p[8];
-            half8_t ph, pl;
+        for (int j = 0; j < 8; j++) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[g >> 1][8 * (g & 1) + j], factor, -base));
+        if constexpr (F32) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[g >> 1][8 * (g & 1) + j], factor, -base));
-                l += p[j];
-            }
-            if constexpr (F32) {
-                split8(p, ph, pl);
-            } else {
+            for (int j = 0; j < 8; j++) l += p[j];
+            split8(p, ph, pl);
+        } else {
+            // the sum of the weights as rounded, which is what the values are summed with
 #pragma unroll
-                for (int j = 0; j < 8; j++) ph[j] = (_Float16)p[j];
-            }
-            uint32_t odd = 0;
-#pragma unroll
-            for (int i = 0; i < DT; i++) {
-                uint4 v = *(const uint4*)(at + v_base + g * D * 32 + i * 1024);
-                if constexpr (EDGE) {
-                    keep8(v, any[g]);
-                    // values that are no numbers, where other rows do not see them: they
-                    // leave the product (0 times them is no zero) and are added below
-                    if (pos_lo != pos_hi) odd |= take_odd(v);
-                }
-                o[i] = mfma32(as_half8(v), ph, o[i]);
-                if constexpr (F32) o[i] = mfma32(as_half8(v), pl, o[i]);
-            }
-            if constexpr (EDGE) {
-                if (!__any(odd)) continue;
-#pragma unroll 1
-                for (int k = 0; k < 16; k++) {
-                    const unsigned long long who = __ballot(odd >> (k & 7) & 1);
-                    if (!(who >> (32 * (k >> 3)) & 0xffffffffu)) continue;
-                    float pk = 0.0f, zk = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        pk = e == (k & 7) ? p[e] : pk;
-                        zk = e == (k & 7) ? z[g >> 1][8 * (g & 1) + e] : zk;
-                    }
-                    pk = __shfl(pk, (k >> 3) * 32 + r, 64);
-                    zk = __shfl(zk, (k >> 3) * 32 + r, 64);
-#pragma unroll
-                    for (int i = 0; i < DT; i++) {
-#pragma unroll
-                        for (int j = 0; j < 16; j++) {
-                            const int dim = 8 * (j >> 2) + 4 * half + (j & 3);
-                            const uint16_t x = *(const uint16_t*)(at + C::K_BYTES + (kg * C::STEP + 16 * g) * D * 2 + i * 1024 +
-                                                                  (dim * 2 + ((k >> 3) ^ (dim >> 3 & 1))) * 16 + (k & 7) * 2);
-                            const bool add = ((x & 0x7c00) == 0x7c00) & (zk != -INFINITY);
-                            o[i][j] += add ? pk * f16_to_f32(x) : 0.0f;
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
+            for (int j = 0; j < 8; j += 2) {
+                const half2_t two = {(_Float16)p[j], (_Float16)p[j + 1]}, one = {(_Float16)1.0f, (_Float16)1.0f};
+                ph[j] = two[0], ph[j + 1] = two[1];
+                l = __builtin_amdgcn_fdot2(two, one, l, false);
             }
         }
     };
 
-    int pg = s0 < s_end ? page_of(s0) : 0;
-    if (s0 < s_end) {
-        load(s0, pg, 0);
-        if (s0 + 1 < s_end) pg = page_of(s0 + 1);
-    }
-    for (int s = s0; s < s_end; s++) {
-        const int buf = (s - s0) & 1;
-        __syncthreads();  // step s is in LDS, and no wave reads the other buffer any more
-        if (s + 1 < s_end) {
-            load(s + 1, pg, buf ^ 1);
-            if (s + 2 < s_end) pg = page_of(s + 2);
-        }
-        const int key0 = first_key(s) + kg * C::STEP, key_end = key0 + C::STEP - 1;
-        // keys that no row of the wave sees
-        if (!any_rows || key0 > wave_last || (c.window > 0 && key_end < win_lo && key0 >= c.sinks)) continue;
-        uint32_t bad = 0;
+    // x, or -inf where bit j is not set (two instructions, and no lane mask held in
+    // scalar registers).
+    const auto hide = [](float x, uint32_t bits, int j) {
+        const uint32_t keep = (uint32_t)((int32_t)(bits << (31 - j)) >> 31);
+        return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) & keep) | (0xff800000u & ~keep));
+    };
+
+    // Any step; edge: some row does not see some of its keys.
+    const auto any_step = [&](const uint8_t* at, int key0, uint32_t bad, bool edge) __attribute__((always_inline)) {
+        f32x16 z[ST];
+        scores(at, z);
+        if (edge) {
 #pragma unroll
-        for (int g = 0; g < 2 * ST; g++) bad |= (uint32_t)bad_group[buf][kg * (C::STEP / 16) + g] << g;
-        bad = __builtin_amdgcn_readfirstlane(bad);
-        const uint8_t* at = lds + buf * C::STAGE;
-        const bool edge = key_end > min(pos_lo, cap) || (c.window > 0 && key0 < win_hi && key_end >= c.sinks) || bad;
-        if (edge) step(at, key0, bad, std::integral_constant<bool, true>());
-        else step(at, key0, 0u, std::integral_constant<bool, false>());
+            for (int g = 0; g < 2 * ST; g++) {
+                const uint32_t seen = bad >> g & 1 ? 0u : paged_seen8(key0 + 16 * g + 8 * half, win, pos_key, c.sinks);
+#pragma unroll
+                for (int j = 0; j < 8; j++) z[g >> 1][8 * (g & 1) + j] = hide(z[g >> 1][8 * (g & 1) + j], seen, j);
+            }
+        }
+        const float now = __builtin_fmaxf(m, largest(z));
+        const float less = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+        m = now;
+        l *= less;
+#pragma unroll
+        for (int i = 0; i < DT; i++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) o[i][j] *= less;
+        const float base = m == -INFINITY ? 0.0f : m - C::SHIFT;
+        // Values that some row does not see may be anything, and 0 times an infinity or a
+        // NaN is no zero: zero times all the values tells whether there are such ones.
+        bool found = false;
+        if (edge) {
+            f32x16 none;
+#pragma unroll
+            for (int j = 0; j < 16; j++) none[j] = 0.0f;
+            const half8_t zero = as_half8(make_uint4(0, 0, 0, 0));
+#pragma unroll
+            for (int g = 0; g < 2 * ST; g++)
+#pragma unroll
+                for (int i = 0; i < DT; i++) none = mfma32(as_half8(v_at(at, g, i)), zero, none);
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; j++) sum += none[j];
+            found = __any(sum != 0.0f);  // a NaN is not zero
+        }
+        if (!found) {
+#pragma unroll
+            for (int g = 0; g < 2 * ST; g++) {
+                half8_t ph, pl;
+                weights(z, g, base, ph, pl);
+#pragma unroll
+                for (int i = 0; i < DT; i++) {
+                    const half8_t v = as_half8(v_at(at, g, i));
+                    o[i] = mfma32(v, ph, o[i]);
+                    if constexpr (F32) o[i] = mfma32(v, pl, o[i]);
+                }
+            }
+            return;
+        }
+        // values that no row of the wave sees become zero; those that only some rows see
+        // leave the product if they are no numbers, and are added by hand
+        uint32_t odd = 0;  // bit 8 g + j: key 16 g + 8 half + j
+#pragma unroll
+        for (int g = 0; g < 2 * ST; g++) {
+            half8_t ph, pl;
+            weights(z, g, base, ph, pl);
+            const uint32_t any = bad >> g & 1 ? 0u : paged_seen8(key0 + 16 * g + 8 * half, win_lo, wave_last, c.sinks);
+#pragma unroll
+            for (int i = 0; i < DT; i++) {
+                uint4 v = v_at(at, g, i);
+                keep8(v, any);
+                odd |= take_odd(v) << (8 * g);
+                o[i] = mfma32(as_half8(v), ph, o[i]);
+                if constexpr (F32) o[i] = mfma32(as_half8(v), pl, o[i]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+#pragma unroll 1
+        for (int k = 0; k < C::KEYS; k++) {
+            const int bit = 8 * (k >> 4) + (k & 7), side = k >> 3 & 1;
+            const unsigned long long who = __ballot(odd >> bit & 1);
+            if (!(who >> (32 * side) & 0xffffffffu)) continue;
+            float zk = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16 * ST; e++) zk = e == bit ? z[e >> 4][e & 15] : zk;
+            zk = __shfl(zk, side * 32 + r, 64);
+            const float pk = __builtin_amdgcn_exp2f(__builtin_fmaf(zk, factor, -base));
+            int side4 = 4 * half;
+            asm volatile("" : "+v"(side4));  // or the main loop carries these reads' addresses
+            const uint8_t* from = at + C::K_BYTES + (k & 7) * 2;
+#pragma unroll
+            for (int i = 0; i < DT; i++) {
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const int dim = 32 * i + 8 * (j >> 2) + side4 + (j & 3);
+                    const uint16_t x = *(const uint16_t*)(from + dim * 128 + (k >> 3 ^ (dim >> 1 & 7)) * 16);
+                    const bool add = ((x & 0x7c00) == 0x7c00) & (zk != -INFINITY);
+                    o[i][j] += add ? pk * f16_to_f32(x) : 0.0f;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+
+    const auto bad_of = [&](const int* from) {
+        const uint32_t bad = from[0] | from[1] << 1 | from[2] << 2 | from[3] << 3;
+        return (uint32_t)__builtin_amdgcn_readfirstlane(bad);
+    };
+    // steps fast0 .. fast1 - 1 of this wave: every row sees all their keys
+    const int whole = min(pos_lo, cap) + 1 - C::KEYS;
+    const int fast0 = max(span.sink_steps, ((win_hi + C::KEYS - 1) >> C::KEY_SHIFT) - span.skip);
+    const int fast1 = any_rows && whole >= 0 ? min(s_end - 1, (whole >> C::KEY_SHIFT) - span.skip + 1) : 0;
+    Pages pg{0, {0, 0}};
+    int s = s0;
+    if (s < s_end) {
+        load(s, pages_of(s), lds, bad_group[0]);
+        pg = pages_of(s + 1);
+    }
+    // a wave's own loads, which a barrier does not wait for, then everyone's
+    const auto arrive = [&]() {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    bool there = false;  // step s is in LDS, and no wave reads the other stage any more
+    while (s < s_end) {
+        // any step
+        const int odd = (s - s0) & 1, key0 = first_key(s), key_end = key0 + C::KEYS - 1;
+        if (!there) arrive();
+        there = false;
+        if (s + 1 < s_end) {
+            load(s + 1, pg, lds + (odd ^ 1) * C::STAGE, bad_group[odd ^ 1]);
+            pg = pages_of(s + 2);
+        }
+        // one with keys that some row of the wave sees
+        if (any_rows && key0 <= wave_last && (c.window <= 0 || key_end >= win_lo || key0 < c.sinks)) {
+            const uint32_t bad = bad_of(bad_group[odd]);
+            any_step(lds + odd * C::STAGE, key0, bad,
+                     bad || key_end > min(pos_lo, cap) || (c.window > 0 && key0 < win_hi && key_end >= c.sinks));
+        }
+        s++;
+        if (s < fast0) continue;
+        // Steps whose keys every row of the wave sees, up to one where a row's largest
+        // passes its reference by more than the slack.  The sums change at the end alone:
+        // else they were held, and moved, in two sets of registers.  The next step's
+        // loads follow this one's last read, as the compiler has every read of LDS wait
+        // for the loads before it.
+        while (s < fast1) {
+            const int now = (s - s0) & 1;
+            const uint8_t* at = lds + now * C::STAGE;
+            arrive();
+            there = true;
+            if (bad_of(bad_group[now])) break;
+            f32x16 z[ST];
+            scores(at, z);
+            half8_t vf[C::V_AHEAD][DT];
+#pragma unroll
+            for (int g = 0; g < C::V_AHEAD; g++)
+#pragma unroll
+                for (int i = 0; i < DT; i++) vf[g][i] = as_half8(v_at(at, g, i));
+            __builtin_amdgcn_sched_barrier(0);
+            if (__any(largest(z) > m + C::SLACK)) break;
+            const float base = m - C::SHIFT;  // m is not -inf: no score passes such a reference by the slack
+#pragma unroll
+            for (int g0 = 0; g0 < 2 * ST; g0 += C::V_AHEAD) {
+                if (g0) {
+#pragma unroll
+                    for (int g = 0; g < C::V_AHEAD; g++)
+#pragma unroll
+                        for (int i = 0; i < DT; i++) vf[g][i] = as_half8(v_at(at, g0 + g, i));
+                }
+                if (g0 + C::V_AHEAD == 2 * ST) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    load(s + 1, pg, lds + (now ^ 1) * C::STAGE, bad_group[now ^ 1]);
+                    pg = pages_of(s + 2);
+                }
+#pragma unroll
+                for (int g = 0; g < C::V_AHEAD; g++) {
+                    half8_t ph, pl;
+                    weights(z, g0 + g, base, ph, pl);
+#pragma unroll
+                    for (int i = 0; i < DT; i++) {
+                        o[i] = mfma32(vf[g][i], ph, o[i]);
+                        if constexpr (F32) o[i] = mfma32(vf[g][i], pl, o[i]);
+                    }
+                }
+            }
+            there = false;
+            s++;
+        }
     }
     if (bad_page && lane == 0) c.flags[0] = 1;
 
-    // the halves of a row's sum, and the two key groups' sums
-    l += partner32(l);
-    if constexpr (C::KG == 2) {
-        float4* sums = (float4*)lds + (rg * DT * 4) * 64 + lane;
-        float2* stat = (float2*)(lds + C::RG * DT * 4 * 64 * 16) + rg * 64 + lane;
-        __syncthreads();
-        if (kg == 1) {
-#pragma unroll
-            for (int i = 0; i < DT; i++)
-#pragma unroll
-                for (int a = 0; a < 4; a++)
-                    sums[(i * 4 + a) * 64] = make_float4(o[i][4 * a], o[i][4 * a + 1], o[i][4 * a + 2], o[i][4 * a + 3]);
-            *stat = make_float2(m, l);
-        }
-        __syncthreads();
-        if (kg == 0) {
-            const float2 other = *stat;
-            const float top = __builtin_fmaxf(m, other.x), base = top == -INFINITY ? 0.0f : top;
-            const float e0 = __builtin_amdgcn_exp2f(m - base), e1 = __builtin_amdgcn_exp2f(other.x - base);
-            m = top;
-            l = l * e0 + other.y * e1;
-#pragma unroll
-            for (int i = 0; i < DT; i++)
-#pragma unroll
-                for (int a = 0; a < 4; a++) {
-                    const float4 v = sums[(i * 4 + a) * 64];
-                    o[i][4 * a] = o[i][4 * a] * e0 + v.x * e1;
-                    o[i][4 * a + 1] = o[i][4 * a + 1] * e0 + v.y * e1;
-                    o[i][4 * a + 2] = o[i][4 * a + 2] * e0 + v.z * e1;
-                    o[i][4 * a + 3] = o[i][4 * a + 3] * e0 + v.w * e1;
-                }
-        }
-    }
-    if (kg == 0 && 32 * rg + r < nrows) {
+    l += partner32(l);  // the halves of a row's sum
+    if (32 * wave + r < nrows) {
         if (it.splits > 1) {
             float* part = parts + ((int64_t)(it.part + it.split) * c.kv_heads + h) * C::PART;
             if (half == 0) {
-                part[32 * rg + r] = m;
-                part[C::ROWS + 32 * rg + r] = l;
+                part_store(part + 32 * wave + r, m);
+                part_store(part + C::ROWS + 32 * wave + r, l);
             }
 #pragma unroll
             for (int i = 0; i < DT; i++)
 #pragma unroll
                 for (int a = 0; a < 4; a++)
-                    *(float4*)(part + 2 * C::ROWS + (32 * rg + r) * D + 32 * i + 8 * a + 4 * half) =
-                        make_float4(o[i][4 * a], o[i][4 * a + 1], o[i][4 * a + 2], o[i][4 * a + 3]);
+                    part_store4(part + 2 * C::ROWS + (32 * wave + r) * D + 32 * i + 8 * a + 4 * half, o[i][4 * a], o[i][4 * a + 1],
+                                o[i][4 * a + 2], o[i][4 * a + 3]);
         } else {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const bool none = l == 0.0f;
-            const int64_t to = place(32 * rg + r) + 4 * half;
+            const int64_t to = place(32 * wave + r) + 4 * half;
 #pragma unroll
             for (int i = 0; i < DT; i++)
 #pragma unroll
@@ -366,17 +456,17 @@ __global__ __launch_bounds__((PagedTile<D, F32>::THREADS)) void k_paged_tile(Pag
         }
     }
     if (it.splits > 1 && paged_last(c.joins + it.joint * c.kv_heads + h, it.splits))
-        paged_join<D, F32, C::ROWS, C::THREADS>(parts + ((int64_t)it.part * c.kv_heads + h) * C::PART,
+        paged_join<D, F32, C::ROWS, C::THREADS, 4, 2>(parts + ((int64_t)it.part * c.kv_heads + h) * C::PART,
                                                 (int64_t)c.kv_heads * C::PART, it.splits, nrows, lds, c.out, place);
 }
 
 // Workgroups that the card holds at once.
-constexpr int TILE_TARGET_SHIFT = 8, TILE_UNIT_MIN = 4;
+constexpr int TILE_TARGET_SHIFT = 9, TILE_UNIT_MIN = 8;
 
 template <int D, bool F32>
 static hipError_t tiles_as(const PagedCall& c, int route, int few, float* parts, hipStream_t s) {
     using C = PagedTile<D, F32>;
-    const PagedCut cut{7, C::KEY_SHIFT, TILE_UNIT_MIN, TILE_TARGET_SHIFT, (C::ROWS - 1) / c.group + 1, route, few};
+    const PagedCut cut{7, C::KEY_SHIFT, TILE_UNIT_MIN, TILE_TARGET_SHIFT, (C::ROWS - 1) / c.group + 1, route, few, D == 256 ? 0 : 512};
     hipLaunchKernelGGL((k_paged_tile<D, F32>), dim3((unsigned)paged_items_most(c, cut)), dim3(C::THREADS), 0, s, c, cut, parts);
     return hipGetLastError();
 }
