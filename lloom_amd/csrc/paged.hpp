@@ -159,29 +159,20 @@ __device__ __forceinline__ void split8(const float (&x)[8], half8_t& hi, half8_t
 }
 
 // Zeroes the infinities and NaN among 8 keys' values; bit j of the result: there
-// was one at key j.
+// was one at key j.  An exponent of all ones and 1 more is the sign's bit.
 __device__ __forceinline__ uint32_t take_odd(uint4& v) {
     uint32_t odd = 0;
     uint32_t* w = (uint32_t*)&v;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        if ((w[j] & 0x7c00u) == 0x7c00u) {
-            odd |= 1u << (2 * j);
-            w[j] &= 0xffff0000u;
-        }
-        if ((w[j] & 0x7c000000u) == 0x7c000000u) {
-            odd |= 2u << (2 * j);
-            w[j] &= 0xffffu;
-        }
+        const uint32_t at = ((w[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+        w[j] &= ~(at | (at - (at >> 15)));
+        odd |= (at >> 15 & 1) << (2 * j) | (at >> 31) << (2 * j + 1);
     }
     return odd;
 }
-// Not zero: there is an infinity or a NaN among 8 keys' values.  An exponent of all
-// ones and 1 more is the sign's bit.
-__device__ __forceinline__ uint32_t odd_mark(const uint4& v) {
-    const auto mark = [](uint32_t w) { return (w & 0x7c007c00u) + 0x04000400u; };
-    return (mark(v.x) | mark(v.y) | mark(v.z) | mark(v.w)) & 0x80008000u;
-}
+// Bit j: an infinity or a NaN at key j of 8 keys' values.
+__device__ __forceinline__ uint32_t odd_keys(uint4 v) { return take_odd(v); }
 // Zeroes the values of the keys whose bit is not set.
 __device__ __forceinline__ void keep8(uint4& v, uint32_t bits) {
     uint32_t* w = (uint32_t*)&v;
@@ -228,7 +219,18 @@ __device__ __forceinline__ PagedItem paged_find(const PagedCall& c, const PagedC
 #pragma unroll
     for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d, 64);
     const unsigned long long per = (total * c.kv_heads + (1u << cut.target_shift) - 1) >> cut.target_shift;
-    const int chunk = (int)min(per > (unsigned)cut.unit_min ? per : (unsigned long long)cut.unit_min, 0x7fffffffull);
+    int chunk = (int)min(per > (unsigned)cut.unit_min ? per : (unsigned long long)cut.unit_min, 0x7fffffffull);
+    // Fewer and longer splits where that lets every item start at once: a second round
+    // of a few items takes as long as the first.
+    if (cut.slots && c.requests <= 64) {
+        const int all = __builtin_amdgcn_readlane(paged_scan(at.tiles), 63) * c.kv_heads;
+        for (int i = 0; i < 6 && all < cut.slots; i++) {
+            const int items = __builtin_amdgcn_readlane(paged_scan(at.tiles * (((unsigned)at.units + chunk - 1) / (unsigned)chunk)), 63) * c.kv_heads;
+            if (items <= cut.slots) break;
+            chunk += max(1, (int)((int64_t)chunk * (items - cut.slots) / cut.slots));
+        }
+        chunk = __builtin_amdgcn_readfirstlane(chunk);
+    }
     // every field is the same in all lanes: readlane keeps them scalar
     PagedItem it;
     it.found = false;

@@ -156,15 +156,21 @@ __global__ __launch_bounds__((PagedTile<D, F32>::THREADS), D == 256 ? 1 : 2) voi
 #pragma unroll
         for (int i = 0; i < C::K_LOADS; i++)
             lds_load16(k + k_off[i], to + (wave * C::K_LOADS + i) * 1024);
+        int shift = c.page_shift;
+        asm volatile("" : "+s"(shift));  // or every load's offset is held in scalar registers
         const uint8_t* v[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int vp = (unsigned)pg.v[i] >= (unsigned)c.pages ? 0 : pg.v[i];
-            v[i] = (const uint8_t*)(c.v + vp * page_size + head_off + ((key0 + (run ^ (32 * i))) & (page - 1))) + v_row;
+            v[i] = (const uint8_t*)(c.v + vp * page_size + head_off + ((key0 + (run ^ (32 * i))) & (page - 1))) + v_row +
+                   ((uint32_t)(i ? v_first | 1 : (v_first + 1) & ~1) << (shift + 4));
         }
 #pragma unroll
-        for (int i = 0; i < C::V_LOADS; i++)
-            lds_load16(((v_first + i) & 1 ? v[1] : v[0]) + ((uint32_t)(v_first + i) << (c.page_shift + 4)), to + C::K_BYTES + (v_first + i) * 1024);
+        for (int i = 0; i < C::V_LOADS; i++) {
+            const int par = (v_first + i) & 1;
+            lds_load16(par ? v[1] : v[0], to + C::K_BYTES + (v_first + i) * 1024);
+            (par ? v[1] : v[0]) += 32 << shift;
+        }
     };
 
     f32x16 o[DT];
@@ -266,8 +272,10 @@ __global__ __launch_bounds__((PagedTile<D, F32>::THREADS), D == 256 ? 1 : 2) voi
             for (int j = 0; j < 16; j++) o[i][j] *= less;
         const float base = m == -INFINITY ? 0.0f : m - C::SHIFT;
         // Values that some row does not see may be anything, and 0 times an infinity or a
-        // NaN is no zero: zero times all the values tells whether there are such ones.
-        bool found = false;
+        // NaN is no zero.  Zero times all the values tells whether there are such ones;
+        // if so, keys that no row sees, and keys that hold such values, leave the product,
+        // and the latter are added by hand to the rows that see them.
+        uint32_t odd = 0, keep = 0xffffffffu;  // bit 8 g + j: key 16 g + 8 half + j
         if (edge) {
             f32x16 none;
 #pragma unroll
@@ -280,63 +288,56 @@ __global__ __launch_bounds__((PagedTile<D, F32>::THREADS), D == 256 ? 1 : 2) voi
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 16; j++) sum += none[j];
-            found = __any(sum != 0.0f);  // a NaN is not zero
-        }
-        if (!found) {
-#pragma unroll
-            for (int g = 0; g < 2 * ST; g++) {
-                half8_t ph, pl;
-                weights(z, g, base, ph, pl);
-#pragma unroll
-                for (int i = 0; i < DT; i++) {
-                    const half8_t v = as_half8(v_at(at, g, i));
-                    o[i] = mfma32(v, ph, o[i]);
-                    if constexpr (F32) o[i] = mfma32(v, pl, o[i]);
+            if (__any(sum != 0.0f)) {  // a NaN is not zero
+#pragma unroll 1
+                for (int g = 0; g < 2 * ST; g++) {
+                    const uint32_t any = bad >> g & 1 ? 0u : paged_seen8(key0 + 16 * g + 8 * half, win_lo, wave_last, c.sinks);
+                    uint32_t marks = 0;
+#pragma unroll 1
+                    for (int i = 0; i < DT; i++) marks |= odd_keys(v_at(at, g, i));
+                    odd |= (marks & any) << (8 * g);
+                    keep &= ~((~any & 0xffu) << (8 * g));
                 }
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) odd |= __shfl_xor(odd, d, 64);
+                keep &= ~odd;
             }
-            return;
         }
-        // values that no row of the wave sees become zero; those that only some rows see
-        // leave the product if they are no numbers, and are added by hand
-        uint32_t odd = 0;  // bit 8 g + j: key 16 g + 8 half + j
 #pragma unroll
         for (int g = 0; g < 2 * ST; g++) {
             half8_t ph, pl;
             weights(z, g, base, ph, pl);
-            const uint32_t any = bad >> g & 1 ? 0u : paged_seen8(key0 + 16 * g + 8 * half, win_lo, wave_last, c.sinks);
 #pragma unroll
             for (int i = 0; i < DT; i++) {
                 uint4 v = v_at(at, g, i);
-                keep8(v, any);
-                odd |= take_odd(v) << (8 * g);
+                if (edge) keep8(v, keep >> (8 * g));
                 o[i] = mfma32(as_half8(v), ph, o[i]);
                 if constexpr (F32) o[i] = mfma32(as_half8(v), pl, o[i]);
-                __builtin_amdgcn_sched_barrier(0);
             }
         }
+        const uint32_t odd2[2] = {(uint32_t)__builtin_amdgcn_readlane(odd, 0), (uint32_t)__builtin_amdgcn_readlane(odd, 32)};
+        for (int side = 0; side < 2; side++) {
 #pragma unroll 1
-        for (int k = 0; k < C::KEYS; k++) {
-            const int bit = 8 * (k >> 4) + (k & 7), side = k >> 3 & 1;
-            const unsigned long long who = __ballot(odd >> bit & 1);
-            if (!(who >> (32 * side) & 0xffffffffu)) continue;
-            float zk = 0.0f;
+            for (uint32_t left = side ? odd2[1] : odd2[0]; left; left &= left - 1) {
+                const int bit = __builtin_ctz(left), k = 16 * (bit >> 3) + 8 * side + (bit & 7);
+                float zk = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 16 * ST; e++) zk = e == bit ? z[e >> 4][e & 15] : zk;
-            zk = __shfl(zk, side * 32 + r, 64);
-            const float pk = __builtin_amdgcn_exp2f(__builtin_fmaf(zk, factor, -base));
-            int side4 = 4 * half;
-            asm volatile("" : "+v"(side4));  // or the main loop carries these reads' addresses
-            const uint8_t* from = at + C::K_BYTES + (k & 7) * 2;
+                for (int e = 0; e < 16 * ST; e++) zk = e == bit ? z[e >> 4][e & 15] : zk;
+                zk = __shfl(zk, side * 32 + r, 64);
+                const float pk = __builtin_amdgcn_exp2f(__builtin_fmaf(zk, factor, -base));
+                int side4 = 4 * half;
+                asm volatile("" : "+v"(side4));  // or the main loop carries these reads' addresses
+                const uint8_t* from = at + C::K_BYTES + (k & 7) * 2;
 #pragma unroll
-            for (int i = 0; i < DT; i++) {
+                for (int i = 0; i < DT; i++) {
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const int dim = 32 * i + 8 * (j >> 2) + side4 + (j & 3);
-                    const uint16_t x = *(const uint16_t*)(from + dim * 128 + (k >> 3 ^ (dim >> 1 & 7)) * 16);
-                    const bool add = ((x & 0x7c00) == 0x7c00) & (zk != -INFINITY);
-                    o[i][j] += add ? pk * f16_to_f32(x) : 0.0f;
+                    for (int j = 0; j < 16; j++) {
+                        const int dim = 32 * i + 8 * (j >> 2) + side4 + (j & 3);
+                        const uint16_t x = *(const uint16_t*)(from + dim * 128 + (k >> 3 ^ (dim >> 1 & 7)) * 16);
+                        o[i][j] += zk != -INFINITY ? pk * f16_to_f32(x) : 0.0f;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
         }
     };
