@@ -53,7 +53,8 @@ struct PagedCut {
     int slots;  // workgroups that the card holds at once, two a CU; 0: not told
 };
 // A split tile has more units than a 2^target_shift-th of all, so that there are
-// under 2^target_shift of them and under twice as many items of theirs.
+// under 2^target_shift of them and under twice as many items of theirs; where
+// shorter splits fit there are no more than `slots` items.
 __host__ __device__ inline int paged_parts(int target_shift) { return 2 << target_shift; }
 
 // The keys that rows at positions lo .. hi see: [first, hi] and the first
@@ -94,7 +95,8 @@ inline int64_t paged_items_most(const PagedCall& c, const PagedCut& cut) {
     if (cut.route == 1 && tiles > some * ((cut.few + rows - 1) / rows)) tiles = some * ((cut.few + rows - 1) / rows);
     tiles *= c.kv_heads;
     const int64_t keys = (int64_t)c.max_blocks << c.page_shift, units = (keys + (1 << cut.unit_shift) - 1) >> cut.unit_shift;
-    const int64_t all = tiles + ((int64_t)1 << cut.target_shift);
+    int64_t all = tiles + ((int64_t)1 << cut.target_shift);
+    if (all < cut.slots) all = cut.slots;  // where shorter splits fit
     return units < all && units * tiles < all ? units * tiles : all;
 }
 
@@ -220,16 +222,16 @@ __device__ __forceinline__ PagedItem paged_find(const PagedCall& c, const PagedC
     for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d, 64);
     const unsigned long long per = (total * c.kv_heads + (1u << cut.target_shift) - 1) >> cut.target_shift;
     int chunk = (int)min(per > (unsigned)cut.unit_min ? per : (unsigned long long)cut.unit_min, 0x7fffffffull);
-    // Fewer and longer splits where that lets every item start at once: a second round
-    // of a few items takes as long as the first.
-    if (cut.slots && c.requests <= 64) {
-        const int all = __builtin_amdgcn_readlane(paged_scan(at.tiles), 63) * c.kv_heads;
-        for (int i = 0; i < 6 && all < cut.slots; i++) {
-            const int items = __builtin_amdgcn_readlane(paged_scan(at.tiles * (((unsigned)at.units + chunk - 1) / (unsigned)chunk)), 63) * c.kv_heads;
+    // Shorter ones, down to half of that, if every item still starts at once: a second
+    // round of a few items takes as long as the first.
+    if (cut.slots && c.requests <= 64 && __builtin_amdgcn_readlane(paged_scan(at.tiles), 63) * c.kv_heads < cut.slots) {
+        int less = max((chunk + 1) / 2, cut.unit_min);
+        while (less < chunk) {
+            const int items = __builtin_amdgcn_readlane(paged_scan(at.tiles * (int)(((unsigned)at.units + less - 1) / (unsigned)less)), 63) * c.kv_heads;
             if (items <= cut.slots) break;
-            chunk += max(1, (int)((int64_t)chunk * (items - cut.slots) / cut.slots));
+            less += max(less / 8, (int)((int64_t)less * (items - cut.slots) / cut.slots)) + 1;
         }
-        chunk = __builtin_amdgcn_readfirstlane(chunk);
+        chunk = __builtin_amdgcn_readfirstlane(min(chunk, less));
     }
     // every field is the same in all lanes: readlane keeps them scalar
     PagedItem it;

@@ -461,8 +461,8 @@ __global__ __launch_bounds__((PagedTile<D, F32>::THREADS), D == 256 ? 1 : 2) voi
                                                 (int64_t)c.kv_heads * C::PART, it.splits, nrows, lds, c.out, place);
 }
 
-// Workgroups that the card holds at once.
-constexpr int TILE_TARGET_SHIFT = 9, TILE_UNIT_MIN = 8;
+// A tile is split past what a CU would take of the whole call (two workgroups').
+constexpr int TILE_TARGET_SHIFT = 8, TILE_UNIT_MIN = 8;
 
 template <int D, bool F32>
 static hipError_t tiles_as(const PagedCall& c, int route, int few, float* parts, hipStream_t s) {

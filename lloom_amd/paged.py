@@ -18,7 +18,7 @@ from typing import NamedTuple
 import torch
 
 from .lib import LloomHipError, check, lib
-from .quantized import _ACT_IDS, _ctx, _dev_index, _stream
+from .quantized import _ACT_IDS, _ctx, _ctxs, _stream_of
 
 HEAD_DIMS = (64, 96, 128, 256)
 
@@ -38,36 +38,42 @@ def _need(ok, code, msg):
         raise LloomHipError(code, msg)
 
 
-def _ints(t, what, dtype, dim, device):
-    if t.dtype != dtype or t.dim() != dim or t.device != device or (t.numel() and t.stride(-1) != 1):
-        raise LloomHipError(1, f"{what}: {tuple(t.shape)} {t.dtype} on {t.device} is not a {dtype} tensor of {dim} "
-                               f"dimension(s) on {device}, dense in its last")
+def _ints(index, dtype, **tensors):
+    """Each tensor (by its argument's name, with its dimensions) is of dtype, on GPU `index`, dense in its last."""
+    for what, (t, dim) in tensors.items():
+        if t.dtype is not dtype or t.dim() != dim or t.get_device() != index or (t.stride(-1) != 1 and t.numel()):
+            raise LloomHipError(1, f"{what}: {tuple(t.shape)} {t.dtype} on {t.device} is not a {dtype} tensor of {dim} "
+                                   f"dimension(s), dense in its last, on GPU {index}")
+
+
+def _gpu(t, what):
+    """The GPU that t is on, and the handle of its context."""
+    i = t.get_device()
+    if i < 0:
+        raise LloomHipError(1, f"{what}: the cache is not on a HIP device")
+    return i, _ctxs.get(i) or _ctx(i)
 
 
 def paged_plan(cached, new, tokens, block_tables, free_pages, page_size):
     """Block tables, slots and positions of a step from the requests' lengths: cached [requests] tokens each has in the
     cache, new [requests] more, `tokens` rows in all (more than their sum: a padded batch).  block_tables [requests,
     max_blocks] is updated in place with pages from the front of free_pages; all int32 on one GPU."""
-    dev = cached.device
-    i = _dev_index(cached)
-    _ints(cached, "paged_plan cached", torch.int32, 1, dev)
-    _ints(new, "paged_plan new", torch.int32, 1, dev)
-    _ints(block_tables, "paged_plan block_tables", torch.int32, 2, dev)
-    _ints(free_pages, "paged_plan free_pages", torch.int32, 1, dev)
+    i, ctx = _gpu(cached, "paged_plan")
+    _ints(i, torch.int32, cached=(cached, 1), new=(new, 1), block_tables=(block_tables, 2), free_pages=(free_pages, 1))
     n = cached.shape[0]
     _need(new.shape[0] == n and block_tables.shape[0] == n, 3,
           f"paged_plan: {n} cached lengths, {new.shape[0]} new ones and {block_tables.shape[0]} tables")
     # one allocation for the five small outputs, the slots (8 bytes each) first
     at = 2 * tokens
-    buf = torch.empty(at + tokens + 2 * n + 2, dtype=torch.int32, device=dev)
+    buf = cached.new_empty(at + tokens + 2 * n + 2)
     base = buf.data_ptr()
     p_pos = base + 4 * at
     p_start = p_pos + 4 * tokens
     p_seq = p_start + 4 * (n + 1)
-    check(lib().lloom_hip_paged_plan(_ctx(i), cached.data_ptr(), new.data_ptr(), n, tokens, block_tables.data_ptr(),
+    check(lib().lloom_hip_paged_plan(ctx, cached.data_ptr(), new.data_ptr(), n, tokens, block_tables.data_ptr(),
                                      _table_stride(block_tables), block_tables.shape[1], free_pages.data_ptr(),
                                      free_pages.shape[0], page_size, p_start, p_seq, p_pos, base, p_seq + 4 * n,
-                                     _stream(cached)))
+                                     _stream_of(i)))
     slots, positions, q_start, seq_lens, taken = buf.split((at, tokens, n + 1, n, 1))
     return PagedPlan(q_start, seq_lens, positions, slots.view(torch.int64), taken, block_tables)
 
@@ -78,9 +84,9 @@ def _table_stride(t):
 
 def _cache_dims(k_cache, v_cache, what):
     pages, heads, page, dim = k_cache.shape if k_cache.dim() == 4 else (0, 0, 0, 0)
-    if (k_cache.dtype != torch.float16 or v_cache.dtype != torch.float16 or not k_cache.is_contiguous()
+    if (k_cache.dtype is not torch.float16 or v_cache.dtype is not torch.float16 or not k_cache.is_contiguous()
             or not v_cache.is_contiguous() or v_cache.shape != (pages, heads, dim, page)
-            or v_cache.device != k_cache.device):
+            or v_cache.get_device() != k_cache.get_device()):
         raise LloomHipError(3, f"{what}: k {tuple(k_cache.shape)} {k_cache.dtype} and v {tuple(v_cache.shape)} "
                                f"{v_cache.dtype} are not one cache: contiguous f16 [pages, heads, page, dim] and "
                                f"[pages, heads, dim, page]")
@@ -105,17 +111,20 @@ def paged_append(k_cache, v_cache, k, v, slots):
     """Rows k and v [tokens, kv_heads, head_dim] (f32 or f16) into the cache at slots [tokens] (int64; negative: not
     stored).  No two rows of a call share a slot."""
     pages, heads, page, dim = _cache_dims(k_cache, v_cache, "paged_append")
+    i = k_cache.get_device()
     k, v = _rows(k, heads, dim, "paged_append k"), _rows(v, heads, dim, "paged_append v")
-    _ints(slots, "paged_append slots", torch.int64, 1, k_cache.device)
-    _need(k.dtype == v.dtype and k.device == v.device == k_cache.device, 2,
-          f"paged_append: k {k.dtype} on {k.device} and v {v.dtype} on {v.device} differ, or the cache is on "
-          f"{k_cache.device}")
+    _ints(i, torch.int64, slots=(slots, 1))
+    if k.dtype is not v.dtype or k.get_device() != i or v.get_device() != i:
+        raise LloomHipError(2, f"paged_append: k {k.dtype} on {k.device} and v {v.dtype} on {v.device} differ, or the cache "
+                               f"is on {k_cache.device}")
     n = slots.shape[0]
-    _need(k.shape[0] == n and v.shape[0] == n, 3, f"paged_append: {k.shape[0]} and {v.shape[0]} rows, {n} slots")
-    check(lib().lloom_hip_paged_append(_ctx(_dev_index(k_cache)), _ACT_IDS[k.dtype], k.data_ptr(),
+    if k.shape[0] != n or v.shape[0] != n:
+        raise LloomHipError(3, f"paged_append: {k.shape[0]} and {v.shape[0]} rows, {n} slots")
+    i, ctx = _gpu(k_cache, "paged_append")
+    check(lib().lloom_hip_paged_append(ctx, _ACT_IDS[k.dtype], k.data_ptr(),
                                        max(k.stride(0), heads * dim), v.data_ptr(), max(v.stride(0), heads * dim),
                                        slots.data_ptr(), n, k_cache.data_ptr(), v_cache.data_ptr(), pages, heads, dim,
-                                       page, _stream(k_cache)))
+                                       page, _stream_of(i)))
 
 
 def paged_attention(q, k_cache, v_cache, block_tables, q_start, seq_lens, scale=None, window=0, sinks=0, max_new=None,
@@ -130,27 +139,25 @@ def paged_attention(q, k_cache, v_cache, block_tables, q_start, seq_lens, scale=
         raise LloomHipError(3, f"paged_attention: q {tuple(q.shape)} is not [tokens, heads, {dim}] with a multiple of "
                                f"{heads} heads")
     q = _rows(q, q.shape[1], dim, "paged_attention q")
-    dev = k_cache.device
-    _ints(block_tables, "paged_attention block_tables", torch.int32, 2, dev)
-    _ints(q_start, "paged_attention q_start", torch.int32, 1, dev)
-    _ints(seq_lens, "paged_attention seq_lens", torch.int32, 1, dev)
-    n, tokens, group = seq_lens.shape[0], q.shape[0], q.shape[1] // heads
-    _need(q_start.shape[0] == n + 1 and block_tables.shape[0] == n and q.device == dev, 3,
-          f"paged_attention: {n} lengths, {q_start.shape[0]} starts, {block_tables.shape[0]} tables; q on {q.device}, "
-          f"cache on {dev}")
+    i = k_cache.get_device()
+    _ints(i, torch.int32, block_tables=(block_tables, 2), q_start=(q_start, 1), seq_lens=(seq_lens, 1))
+    n, (tokens, all_heads, _) = seq_lens.shape[0], q.shape
+    if q_start.shape[0] != n + 1 or block_tables.shape[0] != n or q.get_device() != i:
+        raise LloomHipError(3, f"paged_attention: {n} lengths, {q_start.shape[0]} starts, {block_tables.shape[0]} tables; q "
+                               f"on {q.device}, cache on {k_cache.device}")
+    i, ctx = _gpu(k_cache, "paged_attention")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    else:
-        _need(out.dtype == q.dtype and out.shape == q.shape and out.is_contiguous() and out.device == dev, 3,
-              f"paged_attention: out {tuple(out.shape)} {out.dtype} does not fit the contiguous {q.dtype} output "
-              f"{tuple(q.shape)}")
-    check(lib().lloom_hip_paged_attention(_ctx(_dev_index(k_cache)), _ACT_IDS[q.dtype], q.data_ptr(),
-                                          max(q.stride(0), q.shape[1] * dim), tokens, k_cache.data_ptr(),
-                                          v_cache.data_ptr(), pages, heads, group, dim, page, block_tables.data_ptr(),
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.dtype is not q.dtype or out.shape != q.shape or not out.is_contiguous() or out.get_device() != i:
+        raise LloomHipError(3, f"paged_attention: out {tuple(out.shape)} {out.dtype} does not fit the contiguous {q.dtype} "
+                               f"output {tuple(q.shape)}")
+    check(lib().lloom_hip_paged_attention(ctx, _ACT_IDS[q.dtype], q.data_ptr(),
+                                          max(q.stride(0), all_heads * dim), tokens, k_cache.data_ptr(),
+                                          v_cache.data_ptr(), pages, heads, all_heads // heads, dim, page, block_tables.data_ptr(),
                                           _table_stride(block_tables), block_tables.shape[1],
                                           q_start.data_ptr(), seq_lens.data_ptr(), n,
                                           1.0 / math.sqrt(dim) if scale is None else scale, window, sinks,
-                                          max_new or 0, out.data_ptr(), _stream(k_cache)))
+                                          max_new or 0, out.data_ptr(), _stream_of(i)))
     return out
 
 

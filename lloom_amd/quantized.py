@@ -92,10 +92,14 @@ def _dev_index(t):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _stream(t):
+def _stream_of(index):
     if _raw_stream is not None:
-        return _raw_stream(_dev_index(t))
-    return torch.cuda.current_stream(t.device).cuda_stream
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+def _stream(t):
+    return _stream_of(_dev_index(t))
 
 
 def _ptr(t):

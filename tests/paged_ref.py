@@ -60,6 +60,28 @@ def attention(q, k_cache, v_cache, tables, q_start, seq_lens, scale, window, sin
     return out, mass, reach, count
 
 
+def dense(s, request):
+    """`attention` of one request that sees everything before it, on the tensors' device (for lengths that take too long a
+    token at a time)."""
+    first, end, length = s["q_start"][request], s["q_start"][request + 1], s["seq_lens"][request]
+    key = torch.arange(length, device=s["q"].device)
+    pages, kv_heads, page, dim = s["k"].shape
+    home = s["t_tables"][request].long()[key // page]
+    pos = torch.arange(length - (end - first), length, device=key.device)
+    q = s["q"][first:end].double()
+    heads = q.shape[1]
+    out, mass = torch.empty_like(q), torch.empty_like(q)
+    reach, count = torch.empty(end - first, heads), (pos + 1).float().cpu()[:, None].expand(-1, heads)
+    for h in range(heads):
+        j = h // (heads // kv_heads)
+        k, v = s["k"][home, j, key % page].double(), s["v"][home, j, :, key % page].double()
+        z = s["scale"] * torch.mm(q[:, h], k.t().contiguous())
+        w = torch.softmax(z.masked_fill(key > pos[:, None], -math.inf), 1)
+        out[:, h], mass[:, h] = torch.mm(w, v), torch.mm(w, v.abs())
+        reach[:, h] = s["scale"] * torch.mm(q[:, h].abs(), k.abs().t().contiguous()).amax(1).cpu()
+    return out.cpu(), mass.cpu(), reach, count
+
+
 def bound(out, mass, reach, count, act, dim):
     """How far a kernel may be from `out`: a score is off by its sum's roundings (dim + 2 of half an f32 step of
     sum |q| |k|), by a few more where it is scaled and has the maximum taken off, and with f32 q by what two halves leave

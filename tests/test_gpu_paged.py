@@ -283,6 +283,30 @@ def test_attention_of_one_chunk(cached, new, page, group, dim, act):
     L.paged_check()
 
 
+#                   cached, new, page, kv_heads, group, dim
+LONG = {
+    "tiles_and_splits": ([6000], [512], 64, 4, 4, 64), "splits_of_a_few_rows": ([30000], [9], 16, 1, 4, 128),
+    "one_long_among_short": ([20000, 40, 0, 700], [300, 64, 129, 1], 32, 2, 4, 64),
+    "more_tiles_than_the_card_holds": ([0, 900], [3000, 1100], 128, 8, 4, 64),
+    "long_and_short_tokens": ([60000, 3, 900, 33], [1, 1, 1, 1], 16, 2, 8, 128),
+}
+
+
+@pytest.mark.parametrize("act", [F32, F16])
+@pytest.mark.parametrize("name", LONG)
+def test_long_requests_in_splits(name, act):
+    """Every way a call's tiles and splits are dealt out, each request against the definition, and the same twice."""
+    s = R.case(*LONG[name], act, device=DEV)
+    got = _run(s)
+    L.paged_check()
+    assert torch.equal(_run(s), got)
+    for b in range(len(s["seq_lens"])):
+        out, *rest = R.dense(s, b)
+        tol = R.bound(out, *rest, act, s["q"].shape[-1])
+        off = (got[s["q_start"][b]:s["q_start"][b + 1]].double().cpu() - out).abs()
+        assert (off <= tol).all(), (b, (off / tol).max())
+
+
 @pytest.mark.parametrize("act", [F32, F16])
 def test_lengths_past_the_tables_are_reported(act):
     s = R.case([90], [20], 16, 1, 2, 64, act, device=DEV)
