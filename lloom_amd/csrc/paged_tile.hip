@@ -9,7 +9,7 @@
 // product's B operand as they stand, and P never leaves its lane.
 #include "kernels.hpp"
 #include "kq_common.hpp"
-#include "paged.hpp"
+#include "paged_rows.hpp"
 
 namespace lloom {
 
@@ -42,18 +42,18 @@ struct PagedTile {
     static constexpr float SHIFT = 8.0f, SLACK = 7.0f;
 };
 
+// Workgroup `wg`; lds: two stages, then bad_group.
 template <int D, bool F32>
-__global__ __launch_bounds__((PagedTile<D, F32>::THREADS), D == 256 ? 1 : 2) void k_paged_tile(PagedCall c, PagedCut cut, float* parts) {
+__device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& cut, float* parts, int wg, int wgs, uint8_t* lds,
+                                           int (*bad_group)[4]) {
     using C = PagedTile<D, F32>;
     constexpr int DC = D / 16, DT = D / 32, ST = 2;
-    __shared__ __align__(16) uint8_t lds[2 * C::STAGE];
-    __shared__ int bad_group[2][4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 31, half = lane >> 5;
-    if (cut.route == 0) paged_zero_tail<F32>(c, D, blockIdx.x, gridDim.x);
-    const PagedItem it = paged_find(c, cut, blockIdx.x / c.kv_heads);
+    if (cut.route == 0) paged_zero_tail<F32>(c, D, wg, wgs);
+    const PagedItem it = paged_find(c, cut, wg / c.kv_heads);
     if (!it.found) return;
-    const int h = blockIdx.x % c.kv_heads, page = 1 << c.page_shift;
+    const int h = wg % c.kv_heads, page = 1 << c.page_shift;
 
     const int row0 = it.tile * C::ROWS, nrows = min(it.T * c.group - row0, C::ROWS);
     const int tok0 = row0 / c.group, row = row0 - tok0 * c.group;  // the tile's first token, and its row 0 from there
@@ -461,24 +461,48 @@ __global__ __launch_bounds__((PagedTile<D, F32>::THREADS), D == 256 ? 1 : 2) voi
                                                 (int64_t)c.kv_heads * C::PART, it.splits, nrows, lds, c.out, place);
 }
 
+// The tiles of the requests with many rows, and after them in the same launch the
+// requests with few.
+template <int D, bool F32>
+__global__ __launch_bounds__((PagedTile<D, F32>::THREADS), D == 256 ? 1 : 2) void k_paged_tile(PagedCall c, PagedCut tiles, float* tile_parts,
+                                                                                            PagedCut rows, float* row_parts, int tile_wgs) {
+    using C = PagedTile<D, F32>;
+    union Lds {
+        struct {
+            uint8_t stages[2 * C::STAGE];
+            int bad_group[2][4];
+        } t;
+        RowsLds<D, C::WAVES> r;
+    };
+    __shared__ __align__(16) Lds lds;
+    const int wg = blockIdx.x;
+    if (wg < tile_wgs) paged_tile<D, F32>(c, tiles, tile_parts, wg, tile_wgs, lds.t.stages, lds.t.bad_group);
+    else paged_rows<D, F32, C::WAVES>(c, rows, row_parts, wg - tile_wgs, gridDim.x - tile_wgs, lds.r.acc, lds.r.stat);
+}
+
 // A tile is split past what a CU would take of the whole call (two workgroups').
 constexpr int TILE_TARGET_SHIFT = 8, TILE_UNIT_MIN = 8;
+// Rows beside tiles: two workgroups of 4 waves a CU.
+constexpr int ROWS_TARGET_SHIFT = 8;
 
 template <int D, bool F32>
-static hipError_t tiles_as(const PagedCall& c, int route, int few, float* parts, hipStream_t s) {
+static hipError_t tiles_as(const PagedCall& c, int few, float* tile_parts, float* row_parts, hipStream_t s) {
     using C = PagedTile<D, F32>;
-    const PagedCut cut{7, C::KEY_SHIFT, TILE_UNIT_MIN, TILE_TARGET_SHIFT, (C::ROWS - 1) / c.group + 1, route, few, D == 256 ? 0 : 512};
-    hipLaunchKernelGGL((k_paged_tile<D, F32>), dim3((unsigned)paged_items_most(c, cut)), dim3(C::THREADS), 0, s, c, cut, parts);
+    const PagedCut tiles{7, C::KEY_SHIFT, TILE_UNIT_MIN, TILE_TARGET_SHIFT, (C::ROWS - 1) / c.group + 1, few ? 2 : 0, few, D == 256 ? 256 : 512};
+    const PagedCut rows{4, 7, 2, ROWS_TARGET_SHIFT, (ATT_ROWS - 1) / c.group + 1, 1, few, 0};
+    const int tile_wgs = (int)paged_items_most(c, tiles), row_wgs = few ? (int)paged_items_most(c, rows) : 0;
+    hipLaunchKernelGGL((k_paged_tile<D, F32>), dim3(tile_wgs + row_wgs), dim3(C::THREADS), 0, s, c, tiles, tile_parts, rows, row_parts, tile_wgs);
     return hipGetLastError();
 }
 
-hipError_t launch_paged_tiles(int act, int dim, const PagedCall& c, int route, int few, void* ws, hipStream_t s) {
-    float* parts = (float*)ws;
+// few: requests of at most so many rows are served by rows; 0: all by tiles.
+hipError_t launch_paged_tiles(int act, int dim, const PagedCall& c, int few, void* tile_ws, void* row_ws, hipStream_t s) {
+    float *t = (float*)tile_ws, *r = (float*)row_ws;
     switch (dim) {
-        case 64: return act == T_F32 ? tiles_as<64, true>(c, route, few, parts, s) : tiles_as<64, false>(c, route, few, parts, s);
-        case 96: return act == T_F32 ? tiles_as<96, true>(c, route, few, parts, s) : tiles_as<96, false>(c, route, few, parts, s);
-        case 128: return act == T_F32 ? tiles_as<128, true>(c, route, few, parts, s) : tiles_as<128, false>(c, route, few, parts, s);
-        case 256: return act == T_F32 ? tiles_as<256, true>(c, route, few, parts, s) : tiles_as<256, false>(c, route, few, parts, s);
+        case 64: return act == T_F32 ? tiles_as<64, true>(c, few, t, r, s) : tiles_as<64, false>(c, few, t, r, s);
+        case 96: return act == T_F32 ? tiles_as<96, true>(c, few, t, r, s) : tiles_as<96, false>(c, few, t, r, s);
+        case 128: return act == T_F32 ? tiles_as<128, true>(c, few, t, r, s) : tiles_as<128, false>(c, few, t, r, s);
+        case 256: return act == T_F32 ? tiles_as<256, true>(c, few, t, r, s) : tiles_as<256, false>(c, few, t, r, s);
     }
     return hipErrorInvalidValue;
 }
@@ -499,11 +523,9 @@ size_t paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int kv_
 
 hipError_t launch_paged_attention(int act, int dim, const PagedCall& c, int max_new, void* ws, hipStream_t s) {
     const int64_t longest = max_new > 0 && max_new < c.tokens ? max_new : c.tokens;
-    if (longest * c.group <= PAGED_FEW) return launch_paged_rows(act, dim, c, 0, 0, ws, s);
-    void* tiles_ws = (char*)ws + paged_rows_workspace_bytes(c.kv_heads, dim);
-    if (c.requests == 1) return launch_paged_tiles(act, dim, c, 0, 0, tiles_ws, s);
-    const hipError_t e = launch_paged_rows(act, dim, c, 1, PAGED_FEW, ws, s);
-    return e != hipSuccess ? e : launch_paged_tiles(act, dim, c, 2, PAGED_FEW, tiles_ws, s);
+    if (longest * c.group <= PAGED_FEW) return launch_paged_rows(act, dim, c, ws, s);
+    void* tile_ws = (char*)ws + paged_rows_workspace_bytes(c.kv_heads, dim);
+    return launch_paged_tiles(act, dim, c, c.requests == 1 ? 0 : PAGED_FEW, tile_ws, ws, s);
 }
 
 }  // namespace lloom
