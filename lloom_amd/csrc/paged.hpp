@@ -21,6 +21,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "kq_common.hpp"
 
 namespace lloom {
@@ -136,14 +138,23 @@ __device__ __forceinline__ uint32_t paged_seen8(int key, int lo, int hi, int sin
     return under(hi + 1) & (~under(lo) | under(sinks));
 }
 
-__device__ __forceinline__ int paged_scan(int v) {  // inclusive over the wave
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(v, d, 64);
-        if ((int)__lane_id() >= d) v += o;
-    }
+// Inclusive sums over the wave, in 6 DPP additions (shuffles: 6 passes through LDS).
+template <class T>
+__device__ __forceinline__ T paged_scan(T v) {
+    const auto from = [](T x, auto ctrl, auto rows) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+    };
+    using std::integral_constant;
+    using All = integral_constant<int, 0xf>;
+    v += from(v, integral_constant<int, 0x111>(), All());  // row_shr:1
+    v += from(v, integral_constant<int, 0x112>(), All());
+    v += from(v, integral_constant<int, 0x114>(), All());
+    v += from(v, integral_constant<int, 0x118>(), All());
+    v += from(v, integral_constant<int, 0x142>(), integral_constant<int, 0xa>());  // row_bcast:15
+    v += from(v, integral_constant<int, 0x143>(), integral_constant<int, 0xc>());  // row_bcast:31
     return v;
 }
+__device__ __forceinline__ int paged_sum(int v) { return __builtin_amdgcn_readlane(paged_scan(v), 63); }
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -213,26 +224,28 @@ __device__ __forceinline__ void paged_store4(void* out, int64_t at, float x, flo
 __device__ __forceinline__ PagedItem paged_find(const PagedCall& c, const PagedCut& cut, int want) {
     const int lane = __lane_id(), cap = paged_key_cap(c);
     PagedLane at = paged_lane(c, cut, cap, lane);
-    unsigned long long total = (unsigned long long)at.tiles * at.units;
+    // in f32: exact under 2^24, and rounded up from there
+    float total = (float)at.tiles * at.units;
     for (int b = 64; b < c.requests; b += 64) {
         const PagedLane more = paged_lane(c, cut, cap, b + lane);
-        total += (unsigned long long)more.tiles * more.units;
+        total += (float)more.tiles * more.units;
     }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d, 64);
-    const unsigned long long per = (total * c.kv_heads + (1u << cut.target_shift) - 1) >> cut.target_shift;
-    int chunk = (int)min(per > (unsigned)cut.unit_min ? per : (unsigned long long)cut.unit_min, 0x7fffffffull);
+    total = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, paged_scan(total)), 63)) * c.kv_heads;
+    if (total >= 16777216.0f) total *= 1.0f + 1.0f / 65536;
+    const float per = __builtin_ceilf(__builtin_ldexpf(total, -cut.target_shift));
+    int chunk = max((int)__builtin_fminf(per, 1e9f), cut.unit_min);
     // Shorter ones, down to half of that, if every item still starts at once: a second
     // round of a few items takes as long as the first.
-    if (cut.slots && c.requests <= 64 && __builtin_amdgcn_readlane(paged_scan(at.tiles), 63) * c.kv_heads < cut.slots) {
+    if (cut.slots && c.requests <= 64 && paged_sum(at.tiles) * c.kv_heads < cut.slots) {
         int less = max((chunk + 1) / 2, cut.unit_min);
         while (less < chunk) {
-            const int items = __builtin_amdgcn_readlane(paged_scan(at.tiles * (int)(((unsigned)at.units + less - 1) / (unsigned)less)), 63) * c.kv_heads;
+            const int items = paged_sum(at.tiles * (int)(((unsigned)at.units + less - 1) / (unsigned)less)) * c.kv_heads;
             if (items <= cut.slots) break;
             less += max(less / 8, (int)((int64_t)less * (items - cut.slots) / cut.slots)) + 1;
         }
-        chunk = __builtin_amdgcn_readfirstlane(min(chunk, less));
+        chunk = min(chunk, less);
     }
+    chunk = __builtin_amdgcn_readfirstlane(chunk);
     // every field is the same in all lanes: readlane keeps them scalar
     PagedItem it;
     it.found = false;
@@ -258,7 +271,7 @@ __device__ __forceinline__ PagedItem paged_find(const PagedCall& c, const PagedC
             it.T = __builtin_amdgcn_readlane(at.T, src);
             it.L = __builtin_amdgcn_readlane(at.L, src);
             it.splits = __builtin_amdgcn_readlane(splits, src);
-            const int in = want - __builtin_amdgcn_readlane(ie - items, src), tile = in / it.splits;
+            const int in = want - __builtin_amdgcn_readlane(ie - items, src), tile = it.splits == 1 ? in : in < it.splits ? 0 : in / it.splits;
             const int before = __builtin_amdgcn_readlane(se - split, src);
             it.split = in - tile * it.splits;
             it.part = (before >> 16) + tile * it.splits;

@@ -11,7 +11,7 @@ constexpr int ATT_WAVES = 8;
 template <int D, bool F32>
 __global__ __launch_bounds__(64 * ATT_WAVES) void k_paged_rows(PagedCall c, PagedCut cut, float* parts) {
     __shared__ float acc[ATT_WAVES][ATT_ROWS][D + 4], stat[ATT_WAVES][2][ATT_ROWS];
-    paged_rows<D, F32, ATT_WAVES>(c, cut, parts, blockIdx.x, gridDim.x, acc, stat);
+    paged_rows<D, F32, ATT_WAVES>(c, cut, parts, blockIdx.x, gridDim.x, acc, stat, c.joins);
 }
 
 // One workgroup a CU: a second round costs more than the last of the balance

@@ -36,7 +36,7 @@ struct RowsLds {
 // Workgroup `wg` of `wgs`, of W waves.
 template <int D, bool F32, int W>
 __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& cut, float* parts, int wg, int wgs,
-                                           float (&acc)[W][ATT_ROWS][D + 4], float (&stat)[W][2][ATT_ROWS]) {
+                                           float (&acc)[W][ATT_ROWS][D + 4], float (&stat)[W][2][ATT_ROWS], int* joins) {
     constexpr int DC = D / 32, DT = D / 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g4 = lane >> 4;
     if (cut.route != 2) paged_zero_tail<F32>(c, D, wg, wgs);
@@ -46,7 +46,7 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
 
     // the lane's row: token and head in group
     const int row0 = it.tile * ATT_ROWS, nrows = min(it.T * c.group - row0, ATT_ROWS);
-    const int tok0 = row0 / c.group, row = row0 - tok0 * c.group;  // the tile's first token, and its row 0 from there
+    const int tok0 = row0 ? row0 / c.group : 0, row = row0 - tok0 * c.group;  // the tile's first token, and its row 0 from there
     const int tok = paged_token(c, row + min(r, nrows - 1)), head = h * c.group + row + min(r, nrows - 1) - tok * c.group;
     const int pos_lo = it.L - it.T + tok0, pos = pos_lo + tok, pos_hi = pos_lo + paged_token(c, row + nrows - 1);
     // row i's place in out
@@ -167,14 +167,19 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
             for (int j = 0; j < 8; j++) z[j] = seen >> j & 1 ? z[j] : -INFINITY;
 #pragma unroll
             for (int i = 0; i < DT; i++) keep8(vraw[i], any);
-            // values that are no numbers, where rows of other tokens do not see them:
-            // they leave the product (0 times them is no zero) and are added by hand below
+            // 0 times an infinity or a NaN is no zero: where rows of other tokens do not see
+            // them, keys that hold such values leave the product and are added by hand below
             if (pos_lo != pos_hi) {
 #pragma unroll
-                for (int i = 0; i < DT; i++) odd |= take_odd(vraw[i]);
+                for (int i = 0; i < DT; i++) odd |= odd_keys(vraw[i]);
+                if (__any(odd != 0)) {
+#pragma unroll
+                    for (int d = 1; d < 16; d <<= 1) odd |= __shfl_xor(odd, d, 64);
+#pragma unroll
+                    for (int i = 0; i < DT; i++) keep8(vraw[i], ~odd);
+                }
             }
         }
-        const bool any_odd = edge && __any(odd != 0);
         float top = z[0];
 #pragma unroll
         for (int j = 1; j < 8; j++) top = __builtin_fmaxf(top, z[j]);
@@ -209,20 +214,17 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
             o[i] = mfma16(as_half8(vraw[i]), ph, o[i]);
             if constexpr (F32) o[i] = mfma16(as_half8(vraw[i]), pl, o[i]);
         }
-        if (any_odd) {
+        if (__any(odd != 0)) {
 #pragma unroll 1
             for (int j = 0; j < 8; j++) {
                 const unsigned long long who = __ballot(odd >> j & 1);
-                float pj = 0.0f, zj = 0.0f;
+                float zj = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    pj = e == j ? p[e] : pj;
-                    zj = e == j ? z[e] : zj;
-                }
+                for (int e = 0; e < 8; e++) zj = e == j ? z[e] : zj;
 #pragma unroll 1
                 for (int g = 0; g < 4; g++) {
                     if (!(who >> (16 * g) & 0xffff)) continue;
-                    const float pr = __shfl(pj, 16 * g + r, 64), zr = __shfl(zj, 16 * g + r, 64);
+                    const float zr = __shfl(zj, 16 * g + r, 64), pr = __builtin_amdgcn_exp2f(zr - base);
                     const int pg = __shfl(vp, 16 * g, 64);
                     int shift = c.page_shift;
                     asm volatile("" : "+s"(shift));  // or the main loop carries these loads' addresses
@@ -233,9 +235,7 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
                         const uint16_t* at = src;
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const uint16_t x = *at;
-                            const bool add = ((x & 0x7c00) == 0x7c00) & (zr != -INFINITY);
-                            o[i][e] += add ? pr * f16_to_f32(x) : 0.0f;
+                            o[i][e] += zr != -INFINITY ? pr * f16_to_f32(*at) : 0.0f;
                             at += 1 << shift;
                         }
                         src += 16 << shift;
@@ -288,7 +288,7 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
             else ((uint16_t*)c.out)[oi] = f32_to_f16(y);
         }
     }
-    if (it.splits > 1 && paged_last(c.joins + it.joint * c.kv_heads + h, it.splits))
+    if (it.splits > 1 && paged_last(joins + it.joint * c.kv_heads + h, it.splits))
         paged_join<D, F32, ATT_ROWS, 64 * W, 1, 8>(parts + ((int64_t)it.part * c.kv_heads + h) * PART,
                                                      (int64_t)c.kv_heads * PART, it.splits, nrows, acc, c.out, place);
 }

@@ -462,7 +462,8 @@ __device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& c
 }
 
 // The tiles of the requests with many rows, and after them in the same launch the
-// requests with few.
+// requests with few, whose splits count themselves with the other half of the
+// counters.
 template <int D, bool F32>
 __global__ __launch_bounds__((PagedTile<D, F32>::THREADS), D == 256 ? 1 : 2) void k_paged_tile(PagedCall c, PagedCut tiles, float* tile_parts,
                                                                                             PagedCut rows, float* row_parts, int tile_wgs) {
@@ -477,7 +478,7 @@ __global__ __launch_bounds__((PagedTile<D, F32>::THREADS), D == 256 ? 1 : 2) voi
     __shared__ __align__(16) Lds lds;
     const int wg = blockIdx.x;
     if (wg < tile_wgs) paged_tile<D, F32>(c, tiles, tile_parts, wg, tile_wgs, lds.t.stages, lds.t.bad_group);
-    else paged_rows<D, F32, C::WAVES>(c, rows, row_parts, wg - tile_wgs, gridDim.x - tile_wgs, lds.r.acc, lds.r.stat);
+    else paged_rows<D, F32, C::WAVES>(c, rows, row_parts, wg - tile_wgs, gridDim.x - tile_wgs, lds.r.acc, lds.r.stat, c.joins + PAGED_JOINS / 2);
 }
 
 // A tile is split past what a CU would take of the whole call (two workgroups').
