@@ -166,7 +166,7 @@ hipError_t launch_paged_append(int act, const void* k, int64_t k_stride, const v
 constexpr bool paged_dim_fits(int64_t d) { return d == 64 || d == 96 || d == 128 || d == 256; }
 hipError_t launch_paged_rows(int act, int dim, const PagedCall& c, void* ws, hipStream_t s);
 size_t paged_rows_workspace_bytes(int kv_heads, int dim);
-hipError_t launch_paged_tiles(int act, int dim, const PagedCall& c, int few, void* tile_ws, void* row_ws, hipStream_t s);
+hipError_t launch_paged_tiles(int act, int dim, const PagedCall& c, void* tile_ws, void* row_ws, hipStream_t s);
 size_t paged_tiles_workspace_bytes(int kv_heads, int dim);
 size_t paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int kv_heads, int group, int dim,
                                        int max_new);

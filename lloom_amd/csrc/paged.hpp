@@ -49,11 +49,21 @@ struct PagedCall {
 // keys at a time; a tile with more units of keys than a 2^target_shift-th of the
 // call's, and than `unit_min`, is split among several items.  A tile's last token
 // is at most `more` past its first.
-// route: 0 every request, 1 those of at most `few` rows, 2 the others.
+// route: 0 every request, 1 those with few rows (paged_few), 2 the others.
 struct PagedCut {
-    int row_shift, unit_shift, unit_min, target_shift, more, route, few;
+    int row_shift, unit_shift, unit_min, target_shift, more, route;
     int slots;  // workgroups that the card holds at once, two a CU; 0: not told
 };
+// Whether a request is one of few rows, which are served 16 at a time, each 16
+// reading its keys.  Measured with 16 requests of up to 8191 tokens (heads of 128, 4
+// key heads of 4, f16), the kernel of few rows against that of many: 16 rows each
+// 18 and 28 us, 64 22 and 37; two of 30000 tokens, 76 rows 64 and 105, 140 rows 175
+// and 114; eight of 300 tokens, 200 rows 8 and 13, 500 rows 16 and 15.
+constexpr int PAGED_FEW = 96, PAGED_FEW_SHORT = 256, PAGED_SHORT = 1024;
+__host__ __device__ inline bool paged_few(int64_t rows, int64_t length) {
+    return rows <= PAGED_FEW || (rows <= PAGED_FEW_SHORT && length <= PAGED_SHORT);
+}
+
 // A split tile has more units than a 2^target_shift-th of all, so that there are
 // under 2^target_shift of them and under twice as many items of theirs; where
 // shorter splits fit there are no more than `slots` items.
@@ -94,7 +104,7 @@ __host__ __device__ inline int paged_units(int T, int L, const PagedCut& c, int 
 inline int64_t paged_items_most(const PagedCall& c, const PagedCut& cut) {
     const int64_t rows = (int64_t)1 << cut.row_shift, some = c.requests < c.tokens ? c.requests : c.tokens;
     int64_t tiles = ((int64_t)c.tokens * c.group >> cut.row_shift) + some;
-    if (cut.route == 1 && tiles > some * ((cut.few + rows - 1) / rows)) tiles = some * ((cut.few + rows - 1) / rows);
+    if (cut.route == 1 && tiles > some * (PAGED_FEW_SHORT / rows)) tiles = some * (PAGED_FEW_SHORT / rows);
     tiles *= c.kv_heads;
     const int64_t keys = (int64_t)c.max_blocks << c.page_shift, units = (keys + (1 << cut.unit_shift) - 1) >> cut.unit_shift;
     int64_t all = tiles + ((int64_t)1 << cut.target_shift);
@@ -202,7 +212,7 @@ __device__ __forceinline__ PagedLane paged_lane(const PagedCall& c, const PagedC
     if (b >= c.requests) return r;
     paged_request(c, b, &r.start, &r.T, &r.L);
     const int rows = r.T * c.group;
-    if (r.T > 0 && (cut.route == 0 || (rows <= cut.few) == (cut.route == 1))) {
+    if (r.T > 0 && (cut.route == 0 || paged_few(rows, r.L) == (cut.route == 1))) {
         r.tiles = (rows + (1 << cut.row_shift) - 1) >> cut.row_shift;
         r.units = paged_units(r.T, min(r.L - 1, cap) + 1, cut, c.window, c.sinks);
     }

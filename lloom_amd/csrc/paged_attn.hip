@@ -26,7 +26,7 @@ static hipError_t rows_as(const PagedCall& c, const PagedCut& cut, int64_t grid,
 }
 
 hipError_t launch_paged_rows(int act, int dim, const PagedCall& c, void* ws, hipStream_t s) {
-    const PagedCut cut{4, 8, 1, ATT_TARGET_SHIFT, (ATT_ROWS - 1) / c.group + 1, 0, 0, 0};
+    const PagedCut cut{4, 8, 1, ATT_TARGET_SHIFT, (ATT_ROWS - 1) / c.group + 1, 0, 0};
     const int64_t grid = paged_items_most(c, cut);
     float* parts = (float*)ws;
     switch (dim) {

@@ -11,6 +11,15 @@
 // of a 32-key step leave 8 consecutive keys in a lane, which is B's operand of
 // the second product as it stands: P never leaves its lane, and K and V come
 // straight from the cache in 16-byte pieces, with no LDS.
+//
+// Bound by reading the cache: one request of 131072 tokens (8 key heads of 128, 537
+// MB) takes 98 us, 5.5 TB/s where a large read reaches 6.4.  With less to read,
+// latencies in a row are what it takes: of the 10 us of one request of 641 tokens
+// (1.3 MB) the search for the item is 1.2, the page table and a wave's first K and
+// V 2, the second four waves' another 1.7 (a CU's 32 KB of L1 hold what is in
+// flight: 24 B a clock), the waves' sums 0.5, the counter 0.8, the parts' join 1.5,
+// the launch the rest.  Loads a step ahead of the products are there already: eight
+// waves' 16 KB each.
 #pragma once
 
 #include "kernels.hpp"
@@ -39,7 +48,7 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
                                            float (&acc)[W][ATT_ROWS][D + 4], float (&stat)[W][2][ATT_ROWS], int* joins) {
     constexpr int DC = D / 32, DT = D / 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g4 = lane >> 4;
-    if (cut.route != 2) paged_zero_tail<F32>(c, D, wg, wgs);
+    paged_zero_tail<F32>(c, D, wg, wgs);
     const PagedItem it = paged_find(c, cut, wg / c.kv_heads);
     if (!it.found) return;
     const int h = wg % c.kv_heads, page = 1 << c.page_shift;

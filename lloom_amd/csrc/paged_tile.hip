@@ -7,6 +7,17 @@
 // of one row the keys 8 (j / 4) + 4 half + j % 4, j = 0 .. 15; with K's rows taken
 // in the order that makes them 16 (j / 8) + 8 half + j % 8 they are the second
 // product's B operand as they stand, and P never leaves its lane.
+//
+// Two workgroups a CU: the one's waits and prologue run beside the other's products
+// (one of 8 waves, which share a step's 128 keys: 119 against 116 us for a prompt of
+// 4096 tokens, 16 heads of 128 in f16, and 100 against 64 for two chunks of 2048 with
+// a window of 1024).  The prompt runs at 610 TFLOP/s in 113 us, a large library
+// product at 1300; with f32 q and p in two halves each, so twice the matrix
+// instructions, four chunks of 509 over 8000 take 131 us (760 TFLOP/s of them).
+// Issue and waits bound it, no unit: a step of a wave is 32 MFMAs (1024 clocks) among
+// 370 instructions, and a long tile that is left alone on its CU takes 3900 clocks
+// for it.  Left out by turns, loads are 24 us of the prompt's 111 (without the check
+// of the reference, which is 10), the products with V 13, the weights 13.
 #include "kernels.hpp"
 #include "kq_common.hpp"
 #include "paged_rows.hpp"
@@ -50,7 +61,6 @@ __device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& c
     constexpr int DC = D / 16, DT = D / 32, ST = 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 31, half = lane >> 5;
-    if (cut.route == 0) paged_zero_tail<F32>(c, D, wg, wgs);
     const PagedItem it = paged_find(c, cut, wg / c.kv_heads);
     if (!it.found) return;
     const int h = wg % c.kv_heads, page = 1 << c.page_shift;
@@ -482,28 +492,29 @@ __global__ __launch_bounds__((PagedTile<D, F32>::THREADS), D == 256 ? 1 : 2) voi
 }
 
 // A tile is split past what a CU would take of the whole call (two workgroups').
+// Splits of tiles that fill the card by themselves cost more than they level (two
+// parts for each of 512 tiles: 64 -> 116 us).
 constexpr int TILE_TARGET_SHIFT = 8, TILE_UNIT_MIN = 8;
 // Rows beside tiles: two workgroups of 4 waves a CU.
 constexpr int ROWS_TARGET_SHIFT = 8;
 
 template <int D, bool F32>
-static hipError_t tiles_as(const PagedCall& c, int few, float* tile_parts, float* row_parts, hipStream_t s) {
+static hipError_t tiles_as(const PagedCall& c, float* tile_parts, float* row_parts, hipStream_t s) {
     using C = PagedTile<D, F32>;
-    const PagedCut tiles{7, C::KEY_SHIFT, TILE_UNIT_MIN, TILE_TARGET_SHIFT, (C::ROWS - 1) / c.group + 1, few ? 2 : 0, few, D == 256 ? 256 : 512};
-    const PagedCut rows{4, 7, 2, ROWS_TARGET_SHIFT, (ATT_ROWS - 1) / c.group + 1, 1, few, 0};
-    const int tile_wgs = (int)paged_items_most(c, tiles), row_wgs = few ? (int)paged_items_most(c, rows) : 0;
+    const PagedCut tiles{7, C::KEY_SHIFT, TILE_UNIT_MIN, TILE_TARGET_SHIFT, (C::ROWS - 1) / c.group + 1, 2, D == 256 ? 256 : 512};
+    const PagedCut rows{4, 7, 2, ROWS_TARGET_SHIFT, (ATT_ROWS - 1) / c.group + 1, 1, 0};
+    const int tile_wgs = (int)paged_items_most(c, tiles), row_wgs = (int)paged_items_most(c, rows);
     hipLaunchKernelGGL((k_paged_tile<D, F32>), dim3(tile_wgs + row_wgs), dim3(C::THREADS), 0, s, c, tiles, tile_parts, rows, row_parts, tile_wgs);
     return hipGetLastError();
 }
 
-// few: requests of at most so many rows are served by rows; 0: all by tiles.
-hipError_t launch_paged_tiles(int act, int dim, const PagedCall& c, int few, void* tile_ws, void* row_ws, hipStream_t s) {
+hipError_t launch_paged_tiles(int act, int dim, const PagedCall& c, void* tile_ws, void* row_ws, hipStream_t s) {
     float *t = (float*)tile_ws, *r = (float*)row_ws;
     switch (dim) {
-        case 64: return act == T_F32 ? tiles_as<64, true>(c, few, t, r, s) : tiles_as<64, false>(c, few, t, r, s);
-        case 96: return act == T_F32 ? tiles_as<96, true>(c, few, t, r, s) : tiles_as<96, false>(c, few, t, r, s);
-        case 128: return act == T_F32 ? tiles_as<128, true>(c, few, t, r, s) : tiles_as<128, false>(c, few, t, r, s);
-        case 256: return act == T_F32 ? tiles_as<256, true>(c, few, t, r, s) : tiles_as<256, false>(c, few, t, r, s);
+        case 64: return act == T_F32 ? tiles_as<64, true>(c, t, r, s) : tiles_as<64, false>(c, t, r, s);
+        case 96: return act == T_F32 ? tiles_as<96, true>(c, t, r, s) : tiles_as<96, false>(c, t, r, s);
+        case 128: return act == T_F32 ? tiles_as<128, true>(c, t, r, s) : tiles_as<128, false>(c, t, r, s);
+        case 256: return act == T_F32 ? tiles_as<256, true>(c, t, r, s) : tiles_as<256, false>(c, t, r, s);
     }
     return hipErrorInvalidValue;
 }
@@ -512,21 +523,20 @@ size_t paged_tiles_workspace_bytes(int kv_heads, int dim) {
     return ((size_t)paged_parts(TILE_TARGET_SHIFT) + kv_heads) * 128 * (dim + 2) * sizeof(float);
 }
 
-// Requests of at most this many rows go to the kernel of few rows.
-constexpr int PAGED_FEW = 32;
+// Few rows in every request, as far as the host can see.
+static bool all_few(int64_t tokens, int64_t group, int64_t max_new, int64_t keys) {
+    return paged_few((max_new > 0 && max_new < tokens ? max_new : tokens) * group, keys);
+}
 
 size_t paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int kv_heads, int group, int dim, int max_new) {
     (void)requests;
-    const int64_t longest = max_new > 0 && max_new < tokens ? max_new : tokens;
     const size_t rows = paged_rows_workspace_bytes(kv_heads, dim);
-    return longest * group <= PAGED_FEW ? rows : rows + paged_tiles_workspace_bytes(kv_heads, dim);
+    return all_few(tokens, group, max_new, PAGED_SHORT + 1) ? rows : rows + paged_tiles_workspace_bytes(kv_heads, dim);
 }
 
 hipError_t launch_paged_attention(int act, int dim, const PagedCall& c, int max_new, void* ws, hipStream_t s) {
-    const int64_t longest = max_new > 0 && max_new < c.tokens ? max_new : c.tokens;
-    if (longest * c.group <= PAGED_FEW) return launch_paged_rows(act, dim, c, ws, s);
-    void* tile_ws = (char*)ws + paged_rows_workspace_bytes(c.kv_heads, dim);
-    return launch_paged_tiles(act, dim, c, c.requests == 1 ? 0 : PAGED_FEW, tile_ws, ws, s);
+    if (all_few(c.tokens, c.group, max_new, (int64_t)c.max_blocks << c.page_shift)) return launch_paged_rows(act, dim, c, ws, s);
+    return launch_paged_tiles(act, dim, c, (char*)ws + paged_rows_workspace_bytes(c.kv_heads, dim), ws, s);
 }
 
 }  // namespace lloom

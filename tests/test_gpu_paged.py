@@ -159,6 +159,7 @@ SHAPES = {
     "few_new": ([40, 100], [3, 5], 16, 2, 3, 64), "prompt": ([0], [130], 16, 1, 2, 64),
     "ragged": ([0, 50, 0, 200], [67, 1, 0, 33], 16, 2, 1, 128), "odd_group": ([60], [41], 32, 1, 5, 96),
     "chunk_256": ([90, 10], [37, 64], 16, 1, 2, 256), "many": ([3 * i for i in range(70)], [1] * 70, 16, 1, 2, 64),
+    "many_chunks": ([5 * i for i in range(80)], [1 + 40 * (i % 3 == 1) for i in range(80)], 16, 2, 2, 64),
     "chunk_long": ([1100], [140], 64, 1, 2, 128), "mixed": ([500, 0, 90, 7], [1, 200, 1, 1], 16, 1, 4, 128),
 }
 
@@ -462,3 +463,20 @@ def test_prompt_in_chunks_and_then_tokens():
     s = {"q": q, "k": cache.k, "v": cache.v, "tables": tables.tolist(), "q_start": [0, n], "seq_lens": [n],
          "scale": 1 / math.sqrt(dim)}
     _check(s, torch.cat(got))
+
+
+def test_a_layer_of_packed_projections_over_the_cache():
+    """The example's server: chunks of prompts beside decoding requests, against each whole request at once.  Scores of
+    unit normal q and k are off by at most sum |q||k| / sqrt(128) (about 7.2) times 136 half f32 steps and 2^-21 (see
+    paged_ref.bound), 6e-5, on either side: outputs by d = 1.2e-4 of their size.  The output projection takes them in 8-bit
+    blocks, of steps s = 1/127 of a block's largest, about 3 / 127 of its size: a value changes its step with a
+    probability of d / s and then by s, so that the norm is off by sqrt(d s) = 1.7e-3 at most."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_layer.py")
+    spec = importlib.util.spec_from_file_location("paged_layer", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    worst, us = example.run(prompts=(300, 37, 130, 1), steps=12, chunk=128)
+    assert us is not None and worst < 1.7e-3
