@@ -249,7 +249,7 @@ hipError_t launch_paged_append(int act, const void* k, int64_t k_stride, const v
                  tokens, kv_heads, dim, page_shift};
     // heads of 128 in f16, 8 tokens a workgroup against 64: 64 tokens of 8 heads 3.3 and
     // 6.9 us, 2048 7.5 and 8.8, 4096 12.0 and 10.7, 8192 20.1 and 15.9
-    const bool few = (int64_t)tokens * kv_heads < 24576;
+    const bool few = (int64_t)tokens * kv_heads < 20480;
     if (act == T_F32) few ? append_as<true, 8>(a, s) : append_as<true, 64>(a, s);
     else few ? append_as<false, 8>(a, s) : append_as<false, 64>(a, s);
     return hipGetLastError();
