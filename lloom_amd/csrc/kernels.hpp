@@ -164,9 +164,13 @@ hipError_t launch_paged_append(int act, const void* k, int64_t k_stride, const v
 // requests go to the one kernel or the other by their rows (paged.hpp); no request
 // has over max_new new tokens where that is not 0 (results do not depend on it).
 constexpr bool paged_dim_fits(int64_t d) { return d == 64 || d == 96 || d == 128 || d == 256; }
-hipError_t launch_paged_rows(int act, int dim, const PagedCall& c, void* ws, hipStream_t s);
+// With over 64 requests a launch before sums what they are cut into (c.index).
+struct PagedCut;
+size_t paged_index_workspace_bytes(int64_t requests);
+hipError_t launch_paged_index(PagedCall& c, const PagedCut* cuts, int count, int* to, hipStream_t s);
+hipError_t launch_paged_rows(int act, int dim, PagedCall c, int* index, void* ws, hipStream_t s);
 size_t paged_rows_workspace_bytes(int kv_heads, int dim);
-hipError_t launch_paged_tiles(int act, int dim, const PagedCall& c, void* tile_ws, void* row_ws, hipStream_t s);
+hipError_t launch_paged_tiles(int act, int dim, const PagedCall& c, int* index, void* tile_ws, void* row_ws, hipStream_t s);
 size_t paged_tiles_workspace_bytes(int kv_heads, int dim);
 size_t paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int kv_heads, int group, int dim,
                                        int max_new);

@@ -43,6 +43,10 @@ struct PagedCall {
     int window, sinks;
     float scale;  // log2(e) * the caller's
     uint32_t group_magic;  // 2^32 / group, rounded up (0 for a group of one)
+    // Over 64 requests: where a launch before (k_paged_index) left the splits' length
+    // and every request's sums, of route 1 behind the others'; 64 requests fit a wave,
+    // which finds them itself.
+    const int* index;
 };
 
 // How a kernel cuts its requests: 2^row_shift rows of a request and 2^unit_shift
@@ -54,6 +58,7 @@ struct PagedCut {
     int row_shift, unit_shift, unit_min, target_shift, more, route;
     int slots;  // workgroups that the card holds at once, two a CU; 0: not told
 };
+constexpr int PAGED_INDEX = 16 + 2 * PAGED_MAX_REQUESTS;  // integers of a cut: chunk, then items and splits summed
 // Whether a request is one of few rows, which are served 16 at a time, each 16
 // reading its keys.  Measured with 16 requests of up to 8191 tokens (heads of 128, 4
 // key heads of 4, f16), the kernel of few rows against that of many: 16 rows each
@@ -229,69 +234,89 @@ __device__ __forceinline__ void paged_store4(void* out, int64_t at, float x, flo
     }
 }
 
+// What the requests of a wave's lanes are cut into: items, and items and tiles of
+// split tiles.
+struct PagedCount {
+    int splits, items, split;
+};
+__device__ __forceinline__ PagedCount paged_count(const PagedLane& at, int chunk) {
+    PagedCount n;
+    n.splits = at.units <= chunk ? 1 : (int)(((unsigned)at.units + (unsigned)chunk - 1) / (unsigned)chunk);
+    n.items = at.tiles * n.splits;
+    n.split = n.splits > 1 ? n.items << 16 | at.tiles : 0;
+    return n;
+}
+// The units a split takes, from all requests' tiles x units: in f32, which is exact
+// under 2^24, and rounded up from there.
+__device__ __forceinline__ int paged_chunk(const PagedCall& c, const PagedCut& cut, float total) {
+    total *= c.kv_heads;
+    if (total >= 16777216.0f) total *= 1.0f + 1.0f / 65536;
+    return max((int)__builtin_fminf(__builtin_ceilf(__builtin_ldexpf(total, -cut.target_shift)), 1e9f), cut.unit_min);
+}
+
 // Item `want` of the call, found by every wave on its own: the lengths are known
-// on the GPU alone, and 64 requests cost two scans.  No LDS, no barrier.
+// on the GPU alone.  No LDS, no barrier.
 __device__ __forceinline__ PagedItem paged_find(const PagedCall& c, const PagedCut& cut, int want) {
     const int lane = __lane_id(), cap = paged_key_cap(c);
-    PagedLane at = paged_lane(c, cut, cap, lane);
-    // in f32: exact under 2^24, and rounded up from there
-    float total = (float)at.tiles * at.units;
-    for (int b = 64; b < c.requests; b += 64) {
-        const PagedLane more = paged_lane(c, cut, cap, b + lane);
-        total += (float)more.tiles * more.units;
-    }
-    total = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, paged_scan(total)), 63)) * c.kv_heads;
-    if (total >= 16777216.0f) total *= 1.0f + 1.0f / 65536;
-    const float per = __builtin_ceilf(__builtin_ldexpf(total, -cut.target_shift));
-    int chunk = max((int)__builtin_fminf(per, 1e9f), cut.unit_min);
-    // Shorter ones, down to half of that, if every item still starts at once: a second
-    // round of a few items takes as long as the first.
-    if (cut.slots && c.requests <= 64 && paged_sum(at.tiles) * c.kv_heads < cut.slots) {
-        int less = max((chunk + 1) / 2, cut.unit_min);
-        while (less < chunk) {
-            const int items = paged_sum(at.tiles * (int)(((unsigned)at.units + less - 1) / (unsigned)less)) * c.kv_heads;
-            if (items <= cut.slots) break;
-            less += max(less / 8, (int)((int64_t)less * (items - cut.slots) / cut.slots)) + 1;
-        }
-        chunk = min(chunk, less);
-    }
-    chunk = __builtin_amdgcn_readfirstlane(chunk);
-    // every field is the same in all lanes: readlane keeps them scalar
     PagedItem it;
     it.found = false;
     it.b = it.T = it.L = it.start = it.tile = it.split = it.splits = it.part = it.joint = 0;
-    int items_before = 0, split_before = 0;
-    for (int b0 = 0; b0 < c.requests && !it.found; b0 += 64) {
-        if (b0) at = paged_lane(c, cut, cap, b0 + lane);
-        const int splits = at.units <= chunk ? 1 : (int)(((unsigned)at.units + (unsigned)chunk - 1) / (unsigned)chunk);
-        const int items = at.tiles * splits, split = splits > 1 ? items << 16 | at.tiles : 0;
-        const int ie = items_before + paged_scan(items), se = split_before + paged_scan(split);
-        if (cut.slots && c.requests <= 64) {
+    PagedLane at;
+    PagedCount n;
+    int b0 = 0, ie, se;  // the lanes' first request; their sums
+    if (c.index) {
+        const int* index = c.index + (cut.route == 1 ? PAGED_INDEX : 0);
+        const int *sums = index + 16, last = c.requests - 1;
+        const int end = 64 * lane <= last ? sums[min(64 * lane + 63, last)] : 0x7fffffff;
+        const unsigned long long past = __ballot(want < end && end != 0x7fffffff);
+        if (!past) return it;
+        b0 = 64 * __builtin_ctzll(past);
+        at = paged_lane(c, cut, cap, b0 + lane);
+        n = paged_count(at, __builtin_amdgcn_readfirstlane(index[0]));
+        ie = sums[min(b0 + lane, last)];
+        se = sums[PAGED_MAX_REQUESTS + min(b0 + lane, last)];
+    } else {
+        at = paged_lane(c, cut, cap, lane);
+        const float total = paged_scan((float)at.tiles * at.units);
+        int chunk = paged_chunk(c, cut, __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, total), 63)));
+        // Shorter ones, down to half of that, if every item still starts at once: a second
+        // round of a few items takes as long as the first.
+        if (cut.slots && paged_sum(at.tiles) * c.kv_heads < cut.slots) {
+            int less = max((chunk + 1) / 2, cut.unit_min);
+            while (less < chunk) {
+                const int items = paged_sum(at.tiles * (int)(((unsigned)at.units + less - 1) / (unsigned)less)) * c.kv_heads;
+                if (items <= cut.slots) break;
+                less += max(less / 8, (int)((int64_t)less * (items - cut.slots) / cut.slots)) + 1;
+            }
+            chunk = min(chunk, less);
+        }
+        n = paged_count(at, __builtin_amdgcn_readfirstlane(chunk));
+        ie = paged_scan(n.items);
+        se = paged_scan(n.split);
+        if (cut.slots) {
             // Two workgroups a CU, and the longest items come first: the second ones in
             // turn, so that the longest of them is not with the longest of the first.
             const int all = __builtin_amdgcn_readlane(ie, 63), first = (cut.slots / 2) / c.kv_heads;
             if (all * c.kv_heads <= cut.slots && want >= first && want < all) want = first + all - 1 - want;
         }
-        const unsigned long long hit = __ballot(want < ie && want >= ie - items);
-        if (hit) {
-            const int src = __builtin_ctzll(hit);
-            it.found = true;
-            it.b = b0 + src;
-            it.start = __builtin_amdgcn_readlane(at.start, src);
-            it.T = __builtin_amdgcn_readlane(at.T, src);
-            it.L = __builtin_amdgcn_readlane(at.L, src);
-            it.splits = __builtin_amdgcn_readlane(splits, src);
-            const int in = want - __builtin_amdgcn_readlane(ie - items, src), tile = it.splits == 1 ? in : in < it.splits ? 0 : in / it.splits;
-            const int before = __builtin_amdgcn_readlane(se - split, src);
-            it.split = in - tile * it.splits;
-            it.part = (before >> 16) + tile * it.splits;
-            it.joint = (before & 0xffff) + tile;
-            // the last tokens, which see the most, first
-            it.tile = __builtin_amdgcn_readlane(at.tiles, src) - 1 - tile;
-        }
-        items_before = __builtin_amdgcn_readlane(ie, 63);
-        split_before = __builtin_amdgcn_readlane(se, 63);
     }
+    const unsigned long long hit = __ballot(want < ie && want >= ie - n.items);
+    if (!hit) return it;
+    // every field is the same in all lanes: readlane keeps them scalar
+    const int src = __builtin_ctzll(hit);
+    it.found = true;
+    it.b = b0 + src;
+    it.start = __builtin_amdgcn_readlane(at.start, src);
+    it.T = __builtin_amdgcn_readlane(at.T, src);
+    it.L = __builtin_amdgcn_readlane(at.L, src);
+    it.splits = __builtin_amdgcn_readlane(n.splits, src);
+    const int in = want - __builtin_amdgcn_readlane(ie - n.items, src), tile = it.splits == 1 ? in : in < it.splits ? 0 : in / it.splits;
+    const int before = __builtin_amdgcn_readlane(se - n.split, src);
+    it.split = in - tile * it.splits;
+    it.part = (before >> 16) + tile * it.splits;
+    it.joint = (before & 0xffff) + tile;
+    // the last tokens, which see the most, first
+    it.tile = __builtin_amdgcn_readlane(at.tiles, src) - 1 - tile;
     return it;
 }
 

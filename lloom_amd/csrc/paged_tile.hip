@@ -499,22 +499,23 @@ constexpr int TILE_TARGET_SHIFT = 8, TILE_UNIT_MIN = 8;
 constexpr int ROWS_TARGET_SHIFT = 8;
 
 template <int D, bool F32>
-static hipError_t tiles_as(const PagedCall& c, float* tile_parts, float* row_parts, hipStream_t s) {
+static hipError_t tiles_as(PagedCall c, int* index, float* tile_parts, float* row_parts, hipStream_t s) {
     using C = PagedTile<D, F32>;
-    const PagedCut tiles{7, C::KEY_SHIFT, TILE_UNIT_MIN, TILE_TARGET_SHIFT, (C::ROWS - 1) / c.group + 1, 2, D == 256 ? 256 : 512};
-    const PagedCut rows{4, 7, 2, ROWS_TARGET_SHIFT, (ATT_ROWS - 1) / c.group + 1, 1, 0};
-    const int tile_wgs = (int)paged_items_most(c, tiles), row_wgs = (int)paged_items_most(c, rows);
-    hipLaunchKernelGGL((k_paged_tile<D, F32>), dim3(tile_wgs + row_wgs), dim3(C::THREADS), 0, s, c, tiles, tile_parts, rows, row_parts, tile_wgs);
+    const PagedCut cuts[2] = {{7, C::KEY_SHIFT, TILE_UNIT_MIN, TILE_TARGET_SHIFT, (C::ROWS - 1) / c.group + 1, 2, D == 256 ? 256 : 512},
+                              {4, 7, 2, ROWS_TARGET_SHIFT, (ATT_ROWS - 1) / c.group + 1, 1, 0}};
+    if (const hipError_t e = launch_paged_index(c, cuts, 2, index, s)) return e;
+    const int tile_wgs = (int)paged_items_most(c, cuts[0]), row_wgs = (int)paged_items_most(c, cuts[1]);
+    hipLaunchKernelGGL((k_paged_tile<D, F32>), dim3(tile_wgs + row_wgs), dim3(C::THREADS), 0, s, c, cuts[0], tile_parts, cuts[1], row_parts, tile_wgs);
     return hipGetLastError();
 }
 
-hipError_t launch_paged_tiles(int act, int dim, const PagedCall& c, void* tile_ws, void* row_ws, hipStream_t s) {
+hipError_t launch_paged_tiles(int act, int dim, const PagedCall& c, int* index, void* tile_ws, void* row_ws, hipStream_t s) {
     float *t = (float*)tile_ws, *r = (float*)row_ws;
     switch (dim) {
-        case 64: return act == T_F32 ? tiles_as<64, true>(c, t, r, s) : tiles_as<64, false>(c, t, r, s);
-        case 96: return act == T_F32 ? tiles_as<96, true>(c, t, r, s) : tiles_as<96, false>(c, t, r, s);
-        case 128: return act == T_F32 ? tiles_as<128, true>(c, t, r, s) : tiles_as<128, false>(c, t, r, s);
-        case 256: return act == T_F32 ? tiles_as<256, true>(c, t, r, s) : tiles_as<256, false>(c, t, r, s);
+        case 64: return act == T_F32 ? tiles_as<64, true>(c, index, t, r, s) : tiles_as<64, false>(c, index, t, r, s);
+        case 96: return act == T_F32 ? tiles_as<96, true>(c, index, t, r, s) : tiles_as<96, false>(c, index, t, r, s);
+        case 128: return act == T_F32 ? tiles_as<128, true>(c, index, t, r, s) : tiles_as<128, false>(c, index, t, r, s);
+        case 256: return act == T_F32 ? tiles_as<256, true>(c, index, t, r, s) : tiles_as<256, false>(c, index, t, r, s);
     }
     return hipErrorInvalidValue;
 }
@@ -529,14 +530,14 @@ static bool all_few(int64_t tokens, int64_t group, int64_t max_new, int64_t keys
 }
 
 size_t paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int kv_heads, int group, int dim, int max_new) {
-    (void)requests;
-    const size_t rows = paged_rows_workspace_bytes(kv_heads, dim);
+    const size_t rows = paged_index_workspace_bytes(requests) + paged_rows_workspace_bytes(kv_heads, dim);
     return all_few(tokens, group, max_new, PAGED_SHORT + 1) ? rows : rows + paged_tiles_workspace_bytes(kv_heads, dim);
 }
 
 hipError_t launch_paged_attention(int act, int dim, const PagedCall& c, int max_new, void* ws, hipStream_t s) {
-    if (all_few(c.tokens, c.group, max_new, (int64_t)c.max_blocks << c.page_shift)) return launch_paged_rows(act, dim, c, ws, s);
-    return launch_paged_tiles(act, dim, c, (char*)ws + paged_rows_workspace_bytes(c.kv_heads, dim), ws, s);
+    char* row_ws = (char*)ws + paged_index_workspace_bytes(c.requests);
+    if (all_few(c.tokens, c.group, max_new, (int64_t)c.max_blocks << c.page_shift)) return launch_paged_rows(act, dim, c, (int*)ws, row_ws, s);
+    return launch_paged_tiles(act, dim, c, (int*)ws, row_ws + paged_rows_workspace_bytes(c.kv_heads, dim), row_ws, s);
 }
 
 }  // namespace lloom

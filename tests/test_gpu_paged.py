@@ -196,6 +196,10 @@ def test_attention_arguments(act):
     n, heads, dim = s["q"].shape
     _check(s, _run(s, scale=0.3), scale=0.3)
     _check(s, _run(s, scale=-0.2), scale=-0.2)
+    _check(s, _run(s, scale=0.0), scale=0.0)
+    many = R.case([500], [70], 16, 1, 2, 64, act, device=DEV)
+    for scale in (0.0, -0.3):
+        _check(many, _run(many, scale=scale), scale=scale)
     q, same = s["q"], _run(s)
     fused = torch.zeros(n, 2 * heads * dim, dtype=act, device=DEV)
     fused[:, :heads * dim] = q.reshape(n, -1)
@@ -290,6 +294,8 @@ LONG = {
     "one_long_among_short": ([20000, 40, 0, 700], [300, 64, 129, 1], 32, 2, 4, 64),
     "more_tiles_than_the_card_holds": ([0, 900], [3000, 1100], 128, 8, 4, 64),
     "splits_of_rows_beside_splits_of_tiles": ([30000, 20000, 25000, 9000], [1, 300, 2, 1], 32, 2, 4, 64),
+    "many_requests": ([(911 * i) % 1500 for i in range(321)], [0 if i % 7 == 3 else 1 for i in range(321)], 32, 1, 4, 64),
+    "many_requests_and_chunks": ([20000] + [(577 * i) % 900 for i in range(129)], [90 if i % 16 == 0 else 1 for i in range(130)], 32, 1, 4, 64),
     "long_and_short_tokens": ([60000, 3, 900, 33], [1, 1, 1, 1], 16, 2, 8, 128),
 }
 
