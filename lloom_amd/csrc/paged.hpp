@@ -29,6 +29,10 @@ namespace lloom {
 
 constexpr int PAGED_MAX_REQUESTS = 4096;
 constexpr int PAGED_JOINS = 2048;
+// The least reference of a row that has seen a key: so a row's reference is -inf exactly
+// where it has seen none, and its sums are zero there.  A row whose scores are all -inf
+// or NaN has this reference, and sums that make it NaN.
+constexpr float PAGED_LOWEST = -3.402823466e38f;
 
 // A call's arguments as the kernels see them.
 struct PagedCall {
@@ -404,7 +408,7 @@ __device__ __forceinline__ void paged_join(const float* all, int64_t apart, int 
                 a[i].x *= less, a[i].y *= less, a[i].z *= less, a[i].w *= less, sum[i] *= less;
 #pragma unroll
                 for (int j = 0; j < SN; j++) {
-                    if (ms[i][j] == -INFINITY) continue;
+                    if (ms[i][j] == -INFINITY) continue;  // saw no key, or is no split
                     const float w = __builtin_amdgcn_exp2f(ms[i][j] - base);
                     a[i].x += w * vs[i][j].x, a[i].y += w * vs[i][j].y, a[i].z += w * vs[i][j].z, a[i].w += w * vs[i][j].w;
                     sum[i] += w * ls[i][j];
@@ -433,7 +437,7 @@ __device__ __forceinline__ void paged_join(const float* all, int64_t apart, int 
             const int e = e0 + i * THREADS;
             if (!on || e >= quads) continue;
             const float inv = 1.0f / sum[i];
-            const bool none = sum[i] == 0.0f;
+            const bool none = top[i] == -INFINITY;
             paged_store4<F32>(out, place(e / (D / 4)) + 4 * (e % (D / 4)), none ? 0.0f : a[i].x * inv, none ? 0.0f : a[i].y * inv,
                               none ? 0.0f : a[i].z * inv, none ? 0.0f : a[i].w * inv);
         }

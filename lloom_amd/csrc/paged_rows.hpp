@@ -167,9 +167,9 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
         // a step that some row does not see whole
         const bool edge = key0 + ATT_STEP - 1 > min(pos_lo, cap) ||
                           (c.window > 0 && key0 <= pos_hi - c.window && key0 + ATT_STEP > c.sinks) || __any(bad);
-        uint32_t odd = 0;
+        uint32_t odd = 0, seen = 0xffu;
         if (edge) {
-            const uint32_t seen = bad ? 0u : paged_seen8(v8, win, pos_key, c.sinks);
+            seen = bad ? 0u : paged_seen8(v8, win, pos_key, c.sinks);
             // keys that some row sees: the others' v may hold anything
             const uint32_t any = bad ? 0u : paged_seen8(v8, win_lo, key_last, c.sinks);
 #pragma unroll
@@ -189,9 +189,9 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
                 }
             }
         }
-        float top = z[0];
+        float top = seen ? PAGED_LOWEST : -INFINITY;
 #pragma unroll
-        for (int j = 1; j < 8; j++) top = __builtin_fmaxf(top, z[j]);
+        for (int j = 0; j < 8; j++) top = __builtin_fmaxf(top, z[j]);
         top = __builtin_fmaxf(top, partner16(top));
         top = __builtin_fmaxf(top, partner32(top));
         if (__any(top > m)) {
@@ -292,7 +292,7 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
             }
         } else {
             const int64_t oi = place(rr) + d;
-            const float y = sum == 0.0f ? 0.0f : v / sum;
+            const float y = top == -INFINITY ? 0.0f : v / sum;
             if constexpr (F32) ((float*)c.out)[oi] = y;
             else ((uint16_t*)c.out)[oi] = f32_to_f16(y);
         }

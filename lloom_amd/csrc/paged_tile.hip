@@ -264,15 +264,20 @@ __device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& c
     const auto any_step = [&](const uint8_t* at, int key0, uint32_t bad, bool edge) __attribute__((always_inline)) {
         f32x16 z[ST];
         scores(at, z);
+        float low = PAGED_LOWEST;
         if (edge) {
+            uint32_t some = 0;
 #pragma unroll
             for (int g = 0; g < 2 * ST; g++) {
                 const uint32_t seen = bad >> g & 1 ? 0u : paged_seen8(key0 + 16 * g + 8 * half, win, pos_key, c.sinks);
 #pragma unroll
                 for (int j = 0; j < 8; j++) z[g >> 1][8 * (g & 1) + j] = hide(z[g >> 1][8 * (g & 1) + j], seen, j);
+                some |= seen;
             }
+            low = some ? PAGED_LOWEST : -INFINITY;
+            low = __builtin_fmaxf(low, partner32(low));
         }
-        const float now = __builtin_fmaxf(m, largest(z));
+        const float now = __builtin_fmaxf(__builtin_fmaxf(m, low), largest(z));
         const float less = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);
         m = now;
         l *= less;
@@ -408,8 +413,8 @@ __device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& c
 #pragma unroll
                 for (int i = 0; i < DT; i++) vf[g][i] = as_half8(v_at(at, g, i));
             __builtin_amdgcn_sched_barrier(0);
-            if (__any(largest(z) > m + C::SLACK)) break;
-            const float base = m - C::SHIFT;  // m is not -inf: no score passes such a reference by the slack
+            if (__any(__builtin_fmaxf(largest(z), PAGED_LOWEST) > m + C::SLACK)) break;
+            const float base = m - C::SHIFT;  // m is not -inf: the lowest passes such a reference
 #pragma unroll
             for (int g0 = 0; g0 < 2 * ST; g0 += C::V_AHEAD) {
                 if (g0) {
@@ -455,8 +460,8 @@ __device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& c
                     part_store4(part + 2 * C::ROWS + (32 * wave + r) * D + 32 * i + 8 * a + 4 * half, o[i][4 * a], o[i][4 * a + 1],
                                 o[i][4 * a + 2], o[i][4 * a + 3]);
         } else {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const bool none = l == 0.0f;
+            const float inv = 1.0f / l;
+            const bool none = m == -INFINITY;
             const int64_t to = place(32 * wave + r) + 4 * half;
 #pragma unroll
             for (int i = 0; i < DT; i++)

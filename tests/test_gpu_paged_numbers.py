@@ -1,0 +1,80 @@
+"""Attention over the paged cache where q, keys or values hold infinities or NaN: a row is what the definition makes of
+what it sees, whether its keys are split among workgroups or not, and the other rows are left alone."""
+import math
+
+import pytest
+import torch
+
+import lloom_amd as L
+
+from . import paged_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F16, F32 = torch.float16, torch.float32
+
+#            cached, new, page, kv_heads, group
+WAYS = {
+    "first_token": ([0], [1], 16, 2, 4), "few_rows": ([40, 300], [3, 1], 16, 2, 3),
+    "few_rows_split": ([9, 30000], [1, 3], 64, 1, 4), "tiles": ([300, 5], [130, 1], 32, 1, 2),
+    "tiles_split": ([6000], [90], 64, 1, 2), "many_requests": ([3 * i for i in range(70)], [1 + 60 * (i == 9) for i in range(70)], 16, 1, 2),
+}
+
+
+def _run(s, **kw):
+    return L.paged_attention(s["q"], s["k"], s["v"], s["t_tables"], s["t_start"], s["t_lens"], **kw)
+
+
+def _check(s, got, window=0, sinks=0):
+    """got is the definition's: NaN in the same places, within the bound elsewhere.  Scores' bounds are those of the keys
+    before any was spoilt (s["whole"])."""
+    args = s["tables"], s["q_start"], s["seq_lens"], s["scale"], window, sinks
+    want, mass, reach, count = R.attention(s["q"], s["k"], s["v"], *args)
+    if "whole" in s:
+        reach = R.attention(s["q"], s["whole"], s["v"], *args)[2]
+    tol = R.bound(want, mass, reach, count, s["q"].dtype, s["q"].shape[-1])
+    got = got.double().cpu()
+    nan = want.isnan()
+    assert torch.equal(got.isnan(), nan)
+    assert ((got - want).abs() <= tol)[~nan].all()
+    return nan
+
+
+@pytest.mark.parametrize("act", [F32, F16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("way", WAYS)
+def test_a_query_that_is_no_number(way, dim, bad, act):
+    s = R.case(*WAYS[way], dim, act, device=DEV)
+    spoilt = [(0, 1), (s["q"].shape[0] - 1, 0), (s["q"].shape[0] // 2, s["q"].shape[1] - 1)]
+    for row, head in spoilt:
+        s["q"][row, head, (row + 7 * head) % dim] = bad
+    nan = _check(s, _run(s))
+    assert all(nan[at].all() for at in spoilt) and int(nan.sum()) == len(set(spoilt)) * dim
+    L.paged_check()
+
+
+SPOILT = [(0, 1), (0, 150), (70, 75), (0, 10 ** 6)]
+
+
+def _minus_infinity(way, first, last, act):
+    """Keys first .. last - 1 of every request have scores of -inf."""
+    s = R.case(*WAYS[way], 64, act, device=DEV)
+    s["q"][..., 5] = s["q"][..., 5].abs() + 0.5
+    page = s["k"].shape[2]
+    s["whole"] = s["k"].clone()
+    for b, length in enumerate(s["seq_lens"]):
+        for p in range(first, min(last, length)):
+            s["k"][s["tables"][b][p // page], :, p % page, 5] = -math.inf
+    return s
+
+
+@pytest.mark.parametrize("first,last", SPOILT)
+@pytest.mark.parametrize("way", WAYS)
+def test_keys_whose_scores_are_minus_infinity(way, first, last):
+    """They get no weight; a row that sees no others has no softmax: NaN."""
+    s = _minus_infinity(way, first, last, F16)
+    nan = _check(s, _run(s))
+    assert last < 10 ** 6 or nan.all()
+    _check(s, _run(s, window=40), 40)
+    _check(s, _run(s, window=40, sinks=3), 40, 3)
