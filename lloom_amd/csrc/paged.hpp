@@ -444,16 +444,18 @@ __device__ __forceinline__ void paged_join(const float* all, int64_t apart, int 
     }
 }
 
-// Rows of q that no request owns are zero.
+// Rows of out that no request owns are zero: those before the first's and past the last's.
 template <bool F32>
-__device__ __forceinline__ void paged_zero_tail(const PagedCall& c, int dim, int wg, int wgs) {
-    const int end = min(max(c.q_start[c.requests], 0), c.tokens);
-    const int per = c.kv_heads * c.group * dim;
-    for (int n = end + wg; n < c.tokens; n += wgs)
+__device__ __forceinline__ void paged_zero_rest(const PagedCall& c, int dim, int wg, int wgs) {
+    const int head = min(max(c.q_start[0], 0), c.tokens), end = min(max(c.q_start[c.requests], head), c.tokens);
+    const int per = c.kv_heads * c.group * dim, rest = c.tokens - (end - head);
+    for (int n = wg; n < rest; n += wgs) {
+        const int64_t row = n < head ? n : n + (end - head);
         for (int i = threadIdx.x; i < per; i += blockDim.x) {
-            if (F32) ((float*)c.out)[(int64_t)n * per + i] = 0.0f;
-            else ((uint16_t*)c.out)[(int64_t)n * per + i] = 0;
+            if (F32) ((float*)c.out)[row * per + i] = 0.0f;
+            else ((uint16_t*)c.out)[row * per + i] = 0;
         }
+    }
 }
 
 #endif

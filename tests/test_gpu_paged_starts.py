@@ -1,0 +1,51 @@
+"""Attention over the paged cache: which rows of q a request owns, where q_start is not simply 0 .. tokens."""
+import pytest
+import torch
+
+import lloom_amd as L
+from lloom_amd.lib import LloomHipError
+
+from . import paged_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F16, F32 = torch.float16, torch.float32
+
+#            cached, new, page, kv_heads, group, dim
+WAYS = {
+    "few_rows": ([40, 0, 300], [3, 1, 1], 16, 2, 3, 64), "few_rows_split": ([9, 30000], [1, 3], 64, 1, 4, 64),
+    "tiles": ([300, 5], [130, 1], 32, 1, 2, 128), "tiles_split": ([6000, 0], [90, 70], 64, 1, 2, 64),
+    "many_requests": ([3 * i for i in range(70)], [1 + 60 * (i == 9) for i in range(70)], 16, 1, 2, 96),
+}
+
+
+def _ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def _run(s, **kw):
+    out = torch.full_like(s["q"], 7.0)
+    return L.paged_attention(s["q"], s["k"], s["v"], s["t_tables"], s["t_start"], s["t_lens"], out=out, **kw)
+
+
+def _check(s, got):
+    """got is the definition's within the bound, zero where no request owns the row."""
+    want, *rest = R.attention(s["q"], s["k"], s["v"], s["tables"], s["q_start"], s["seq_lens"], s["scale"], 0, 0)
+    tol = R.bound(want, *rest, s["q"].dtype, s["q"].shape[-1])
+    assert ((got.double().cpu() - want).abs() <= tol).all()
+    owned = torch.zeros(got.shape[0], dtype=torch.bool)
+    owned[s["q_start"][0]:s["q_start"][-1]] = True
+    assert (got[~owned] == 0).all()
+
+
+@pytest.mark.parametrize("act", [F32, F16])
+@pytest.mark.parametrize("before,after", [(1, 0), (5, 3), (300, 0)])
+@pytest.mark.parametrize("way", WAYS)
+def test_rows_before_the_first_request(way, before, after, act):
+    """A part of a longer step's starts, with all of its rows."""
+    s = R.case(*WAYS[way], act, pad=before + after, device=DEV)
+    s["q_start"] = [before + n for n in s["q_start"]]
+    s["t_start"] = _ints(s["q_start"])
+    _check(s, _run(s))
+    _check(s, _run(s, max_new=max(WAYS[way][1])))
+    L.paged_check()
