@@ -62,7 +62,8 @@ struct PagedCut {
     int row_shift, unit_shift, unit_min, target_shift, more, route;
     int slots;  // workgroups that the card holds at once, two a CU; 0: not told
 };
-constexpr int PAGED_INDEX = 16 + 2 * PAGED_MAX_REQUESTS;  // integers of a cut: chunk, then items and splits summed
+// integers of a cut: chunk, whether the call is refused, then from 16 on items and splits summed
+constexpr int PAGED_INDEX = 16 + 2 * PAGED_MAX_REQUESTS;
 // Whether a request is one of few rows, which are served 16 at a time, each 16
 // reading its keys.  Measured with 16 requests of up to 8191 tokens (heads of 128, 4
 // key heads of 4, f16), the kernel of few rows against that of many: 16 rows each
@@ -129,15 +130,21 @@ struct PagedItem {
     int part;   // split 0's number among the items of split tiles
     int joint;  // the tile's number among them
     bool found;
+    bool refused;  // q_start falls or is negative: the call has no items
 };
 
-__device__ __forceinline__ void paged_request(const PagedCall& c, int b, int* start, int* T, int* L) {
+// False where its rows' ends are in no order: rows that two requests own were cut
+// into more items than the grid is sized for, and a split that no workgroup serves
+// would never be counted.
+__device__ __forceinline__ bool paged_request(const PagedCall& c, int b, int* start, int* T, int* L) {
     int s = c.q_start[b], e = c.q_start[b + 1];
+    const bool order = s >= 0 && e >= s;
     s = min(max(s, 0), c.tokens);
     e = min(max(e, s), c.tokens);
     *start = s;
     *T = e - s;
     *L = max(c.seq_lens[b], 0);
+    return order;
 }
 // The last key that a table has a place for.
 __device__ __forceinline__ int paged_key_cap(const PagedCall& c) {
@@ -215,11 +222,12 @@ __device__ __forceinline__ void keep8(uint4& v, uint32_t bits) {
 // A lane's request: its rows' tiles, and the units of keys of one.
 struct PagedLane {
     int start, T, L, tiles, units;
+    bool order;
 };
 __device__ __forceinline__ PagedLane paged_lane(const PagedCall& c, const PagedCut& cut, int cap, int b) {
-    PagedLane r{0, 0, 0, 0, 0};
+    PagedLane r{0, 0, 0, 0, 0, true};
     if (b >= c.requests) return r;
-    paged_request(c, b, &r.start, &r.T, &r.L);
+    r.order = paged_request(c, b, &r.start, &r.T, &r.L);
     const int rows = r.T * c.group;
     if (r.T > 0 && (cut.route == 0 || paged_few(rows, r.L) == (cut.route == 1))) {
         r.tiles = (rows + (1 << cut.row_shift) - 1) >> cut.row_shift;
@@ -263,7 +271,7 @@ __device__ __forceinline__ int paged_chunk(const PagedCall& c, const PagedCut& c
 __device__ __forceinline__ PagedItem paged_find(const PagedCall& c, const PagedCut& cut, int want) {
     const int lane = __lane_id(), cap = paged_key_cap(c);
     PagedItem it;
-    it.found = false;
+    it.found = it.refused = false;
     it.b = it.T = it.L = it.start = it.tile = it.split = it.splits = it.part = it.joint = 0;
     int b0 = 0, ie = 0, se = 0, chunk = 0;  // the lanes' first request; their sums
     if (c.index) {
@@ -279,6 +287,8 @@ __device__ __forceinline__ PagedItem paged_find(const PagedCall& c, const PagedC
     // the one place of both ways: with two, the f32 tiles spilled 8 registers and not 5
     // (128.1 against 125.8 us for 50 GFLOP)
     const PagedLane at = paged_lane(c, cut, cap, b0 + lane);
+    it.refused = c.index ? c.index[1] != 0 : __any(!at.order);
+    if (it.refused) return it;
     if (!c.index) {
         const float total = paged_scan((float)at.tiles * at.units);
         chunk = paged_chunk(c, cut, __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, total), 63)));
@@ -444,10 +454,15 @@ __device__ __forceinline__ void paged_join(const float* all, int64_t apart, int 
     }
 }
 
-// Rows of out that no request owns are zero: those before the first's and past the last's.
+// Rows of out that no request owns are zero: those before the first's and past the last's,
+// and all of a refused call's, which is reported.
 template <bool F32>
-__device__ __forceinline__ void paged_zero_rest(const PagedCall& c, int dim, int wg, int wgs) {
-    const int head = min(max(c.q_start[0], 0), c.tokens), end = min(max(c.q_start[c.requests], head), c.tokens);
+__device__ __forceinline__ void paged_zero_rest(const PagedCall& c, int dim, int wg, int wgs, int first, int last, bool refused) {
+    if (refused) {
+        first = last = c.tokens;
+        if (wg == 0 && threadIdx.x == 0) c.flags[0] = 1;
+    }
+    const int head = min(max(first, 0), c.tokens), end = min(max(last, head), c.tokens);
     const int per = c.kv_heads * c.group * dim, rest = c.tokens - (end - head);
     for (int n = wg; n < rest; n += wgs) {
         const int64_t row = n < head ? n : n + (end - head);

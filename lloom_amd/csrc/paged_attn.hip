@@ -29,14 +29,16 @@ __global__ __launch_bounds__(INDEX_WG) void k_paged_index(PagedCall c, PagedCut 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cap = paged_key_cap(c), b = threadIdx.x * INDEX_EACH;
     PagedLane at[INDEX_EACH];
     float mine = 0.0f;
+    bool order = true;
 #pragma unroll
     for (int i = 0; i < INDEX_EACH; i++) {
         at[i] = paged_lane(c, cut, cap, b + i);
+        order &= at[i].order;
         mine += (float)at[i].tiles * at[i].units;
     }
     mine = paged_scan(mine);
     if (lane == 63) part[wave] = mine;
-    __syncthreads();
+    const int refused = __syncthreads_or(!order);
     float total = 0.0f;
     for (int w = 0; w < INDEX_WG / 64; w++) total += part[w];
     const int chunk = paged_chunk(c, cut, total);
@@ -62,7 +64,10 @@ __global__ __launch_bounds__(INDEX_WG) void k_paged_index(PagedCall c, PagedCut 
             to[16 + PAGED_MAX_REQUESTS + b + i] = se;
         }
     }
-    if (threadIdx.x == 0) to[0] = chunk;
+    if (threadIdx.x == 0) {
+        to[0] = chunk;
+        to[1] = refused;
+    }
 }
 
 size_t paged_index_workspace_bytes(int64_t requests) { return requests > 64 ? 2 * PAGED_INDEX * sizeof(int) : 0; }

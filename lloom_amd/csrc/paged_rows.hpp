@@ -48,8 +48,9 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
                                            float (&acc)[W][ATT_ROWS][D + 4], float (&stat)[W][2][ATT_ROWS], int* joins) {
     constexpr int DC = D / 32, DT = D / 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g4 = lane >> 4;
-    paged_zero_rest<F32>(c, D, wg, wgs);
+    const int first = c.q_start[0], last = c.q_start[c.requests];
     const PagedItem it = paged_find(c, cut, wg / c.kv_heads);
+    paged_zero_rest<F32>(c, D, wg, wgs, first, last, it.refused);
     if (!it.found) return;
     const int h = wg % c.kv_heads, page = 1 << c.page_shift;
 

@@ -49,3 +49,31 @@ def test_rows_before_the_first_request(way, before, after, act):
     _check(s, _run(s))
     _check(s, _run(s, max_new=max(WAYS[way][1])))
     L.paged_check()
+
+
+def _reported():
+    with pytest.raises(LloomHipError) as e:
+        L.paged_check()
+    assert e.value.name == "EPAGE"
+    L.paged_check()
+
+
+@pytest.mark.parametrize("act", [F32, F16])
+@pytest.mark.parametrize("way", WAYS)
+def test_starts_that_fall_leave_the_call_out(way, act):
+    """Zeros and a report, and the next call's splits are joined as ever."""
+    s = R.case(*WAYS[way], act, device=DEV)
+    want = _run(s)
+    n, good = s["q"].shape[0], s["t_start"]
+    for start in ([n, 0], [0, n, 0, n], [0, n - 1, n - 2, n], [-1, n], [-n, 0, n], [-2 ** 31, 2 ** 31 - 1], [2 ** 31 - 1, -2 ** 31]):
+        # the requests beyond: in place in the middle of the others, so that more than one wave's worth is looked at
+        q_start = (start + [start[-1]] * len(s["seq_lens"]))[:len(s["seq_lens"]) + 1]
+        if len(s["seq_lens"]) > 64:
+            q_start = [0] * (len(s["seq_lens"]) + 1 - len(start)) + start
+        if all(a <= b for a, b in zip(q_start, q_start[1:])) and q_start[0] >= 0:
+            continue
+        s["t_start"] = _ints(q_start)
+        assert (_run(s) == 0).all(), q_start
+        s["t_start"] = good
+        assert torch.equal(_run(s), want), q_start
+        _reported()
