@@ -311,7 +311,8 @@ int lloom_hip_paged_append(lloom_hip_ctx* ctx, int act_dtype, const void* k_dev,
  * sees nothing, where no request owns the row, and nothing of a page out of
  * [0, pages).  Values that a token does not see may be anything, and pages that
  * none sees any number (a server's freed ones before a window).  A q_start that
- * falls anywhere or is negative leaves the whole call out: out is zero, EPAGE.  Sums
+ * falls anywhere or is negative leaves the whole call out: out is zero, EPAGE.  Where
+ * it passes `tokens`, the rows that there are keep their positions, EPAGE too.  Sums
  * and the softmax are f32.  With F32 q the products take q and the weights as two halves
  * each (exact to about 2^-22); with F16 the weights are rounded to halves.
  * max_new: no request has more new tokens (0: not known); only speed depends

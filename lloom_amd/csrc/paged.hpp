@@ -135,15 +135,17 @@ struct PagedItem {
 
 // False where its rows' ends are in no order: rows that two requests own were cut
 // into more items than the grid is sized for, and a split that no workgroup serves
-// would never be counted.
+// would never be counted.  Rows past the call's are left out, as if the request ended
+// with the last one that there is.
 __device__ __forceinline__ bool paged_request(const PagedCall& c, int b, int* start, int* T, int* L) {
     int s = c.q_start[b], e = c.q_start[b + 1];
     const bool order = s >= 0 && e >= s;
+    const int past = order ? e - max(s, min(e, c.tokens)) : 0;
     s = min(max(s, 0), c.tokens);
     e = min(max(e, s), c.tokens);
     *start = s;
     *T = e - s;
-    *L = max(c.seq_lens[b], 0);
+    *L = max(c.seq_lens[b], 0) - past;
     return order;
 }
 // The last key that a table has a place for.
@@ -455,13 +457,11 @@ __device__ __forceinline__ void paged_join(const float* all, int64_t apart, int 
 }
 
 // Rows of out that no request owns are zero: those before the first's and past the last's,
-// and all of a refused call's, which is reported.
+// and all of a refused call's.  Reports that, and requests with rows past the call's.
 template <bool F32>
 __device__ __forceinline__ void paged_zero_rest(const PagedCall& c, int dim, int wg, int wgs, int first, int last, bool refused) {
-    if (refused) {
-        first = last = c.tokens;
-        if (wg == 0 && threadIdx.x == 0) c.flags[0] = 1;
-    }
+    if ((refused || last > c.tokens) && wg == 0 && threadIdx.x == 0) c.flags[0] = 1;
+    if (refused) first = last = c.tokens;
     const int head = min(max(first, 0), c.tokens), end = min(max(last, head), c.tokens);
     const int per = c.kv_heads * c.group * dim, rest = c.tokens - (end - head);
     for (int n = wg; n < rest; n += wgs) {

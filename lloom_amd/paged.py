@@ -132,7 +132,8 @@ def paged_attention(q, k_cache, v_cache, block_tables, q_start, seq_lens, scale=
     """Causal attention of q [tokens, heads, head_dim] (f32 or f16) over the cache; out is of q's type and shape.  Rows
     q_start[b] .. q_start[b + 1] are request b's last tokens, the last at position seq_lens[b] - 1; query head h reads key
     head h // (heads // kv_heads).  The token at position p sees position j <= p with window = 0, j > p - window or
-    j < sinks.  A q_start that falls anywhere or is negative leaves the call out (out is zero, paged_check() raises).  scale: 1 / sqrt(head_dim) by default.  max_new: the most new tokens of any request, where the caller
+    j < sinks.  A q_start that falls anywhere or is negative leaves the call out (out is zero, paged_check() raises);
+    one that passes the number of rows leaves out those that are not there (paged_check() raises).  scale: 1 / sqrt(head_dim) by default.  max_new: the most new tokens of any request, where the caller
     knows it (1 for a decode step): only speed depends on it."""
     pages, heads, page, dim = _cache_dims(k_cache, v_cache, "paged_attention")
     if q.dim() != 3 or heads == 0 or q.shape[1] == 0 or q.shape[1] % heads:

@@ -77,3 +77,25 @@ def test_starts_that_fall_leave_the_call_out(way, act):
         s["t_start"] = good
         assert torch.equal(_run(s), want), q_start
         _reported()
+
+
+@pytest.mark.parametrize("act", [F32, F16])
+@pytest.mark.parametrize("cut", [1, 3, 64])
+@pytest.mark.parametrize("way", WAYS)
+def test_rows_that_are_not_there(way, cut, act):
+    """q without the last rows of the step: the others are at the positions that they had, and the call is reported."""
+    s = R.case(*WAYS[way], act, device=DEV)
+    cut = min(cut, s["q"].shape[0] - 1)
+    want, *rest = R.attention(s["q"], s["k"], s["v"], s["tables"], s["q_start"], s["seq_lens"], s["scale"], 0, 0)
+    tol = R.bound(want, *rest, act, s["q"].shape[-1])
+    _run(s)
+    L.paged_check()
+    s["q"] = s["q"][:-cut]
+    got = _run(s)
+    assert ((got.double().cpu() - want[:-cut]).abs() <= tol[:-cut]).all()
+    _reported()
+    # as a plan for fewer rows than there are new tokens says
+    cached, new = WAYS[way][:2]
+    plan = L.paged_plan(_ints(cached), _ints(new), s["q"].shape[0], s["t_tables"], _ints([0] * 4096), WAYS[way][2])
+    assert plan.q_start.tolist() == s["q_start"] and plan.seq_lens.tolist() == s["seq_lens"]
+    _reported()
