@@ -182,10 +182,7 @@ int lloom_hip_ctx_sync(lloom_hip_ctx* ctx) {
     int flag[CTX_FLAG_BYTES / sizeof(int)], zero = 0;
     HIP_OK(hipMemcpy(flag, ctx->flags, sizeof flag, hipMemcpyDeviceToHost));
     for (int i = 0; i < PAGED_JOINS; i++)
-        if (flag[64 + i]) {
-            HIP_OK(hipMemset(ctx->joins, 0, PAGED_JOINS * sizeof(int)));
-            break;
-        }
+        if (flag[64 + i]) ctx->joins_left = true;
     if (flag[0]) {
         HIP_OK(hipMemcpy(ctx->flags, &zero, sizeof(int), hipMemcpyHostToDevice));
         return fail(LLOOM_HIP_EEXPERT, "a routed matmul or embedding saw an id out of range");

@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <mutex>
 #include <vector>
 
@@ -22,8 +23,11 @@ struct lloom_hip_ctx {
     std::vector<void*> retired;
     int* flags = nullptr;  // sticky errors: [0] ids, [1] pages and lengths of the paged cache
     // What the paged attention's workgroups count themselves with: zero between
-    // calls; ctx_sync, with nothing running, clears what a call that was cut off left.
+    // calls.  Where ctx_sync has seen others (a call that was cut off, or one that
+    // another thread has launched since), the next attention call clears them first, on
+    // its own stream: ctx_sync could clear them only under a call that is running.
     int* joins = nullptr;
+    std::atomic<bool> joins_left{false};
     // What a strict call's kernel reports, in host memory: the call reads it
     // when its stream has drained, with no copy (a pageable 4-byte copy took 10
     // us of a 37 us routed call).

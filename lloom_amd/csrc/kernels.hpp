@@ -166,6 +166,7 @@ hipError_t launch_paged_append(int act, const void* k, int64_t k_stride, const v
 constexpr bool paged_dim_fits(int64_t d) { return d == 64 || d == 96 || d == 128 || d == 256; }
 // With over 64 requests a launch before sums what they are cut into (c.index).
 struct PagedCut;
+hipError_t launch_paged_clear(int* joins, hipStream_t s);
 size_t paged_index_workspace_bytes(int64_t requests);
 hipError_t launch_paged_index(PagedCall& c, const PagedCut* cuts, int count, int* to, hipStream_t s);
 hipError_t launch_paged_rows(int act, int dim, PagedCall c, int* index, void* ws, hipStream_t s);

@@ -132,6 +132,14 @@ int lloom_hip_paged_attention(lloom_hip_ctx* ctx, int act_dtype, const void* q_d
         paged_attention_workspace_bytes(tokens, requests, (int)kv_heads, (int)group, (int)head_dim, (int)max_new);
     if (need)
         if (int rc = ensure_ws(ctx, need, s, &ws)) return rc;
+    if (ctx->joins_left.exchange(false)) {
+        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+        const hipError_t e = launch_paged_clear(ctx->joins, s);
+        // recorded into a graph, it has not been done
+        if (e != hipSuccess || hipStreamIsCapturing(s, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone)
+            ctx->joins_left = true;
+        HIP_OK(e);
+    }
     PagedCall c{q_dev, (const uint16_t*)k_cache_dev, (const uint16_t*)v_cache_dev, out_dev, (const int*)q_start_dev,
                 (const int*)seq_lens_dev, (const int*)tables_dev, ctx->flags + 1, ctx->joins, q_stride, table_stride, (int)tokens,
                 (int)requests, (int)kv_heads, (int)group, (int)pages, page_shift(page_size), (int)max_blocks,

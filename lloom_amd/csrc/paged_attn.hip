@@ -70,6 +70,15 @@ __global__ __launch_bounds__(INDEX_WG) void k_paged_index(PagedCall c, PagedCut 
     }
 }
 
+__global__ __launch_bounds__(INDEX_WG) void k_paged_clear(int* joins) {
+    for (int i = threadIdx.x; i < PAGED_JOINS; i += INDEX_WG) joins[i] = 0;
+}
+
+hipError_t launch_paged_clear(int* joins, hipStream_t s) {
+    hipLaunchKernelGGL(k_paged_clear, dim3(1), dim3(INDEX_WG), 0, s, joins);
+    return hipGetLastError();
+}
+
 size_t paged_index_workspace_bytes(int64_t requests) { return requests > 64 ? 2 * PAGED_INDEX * sizeof(int) : 0; }
 
 hipError_t launch_paged_index(PagedCall& c, const PagedCut* cuts, int count, int* to, hipStream_t s) {
