@@ -79,8 +79,8 @@ __host__ __device__ inline bool paged_few(int64_t rows, int64_t length) {
 // shorter splits fit there are no more than `slots` items.
 __host__ __device__ inline int paged_parts(int target_shift) { return 2 << target_shift; }
 
-// The keys that rows at positions lo .. hi see: [first, hi] and the first
-// `sink` tokens before it, as steps of `step` keys.  Step i of the list is
+// The keys that rows at positions lo .. see, up to key hi: [first, hi] and the
+// first `sink` tokens before it, as steps of `step` keys.  Step i of the list is
 // step i of the cache while i < sink_steps, then step skip + i.
 struct PagedSpan {
     int first, sink_steps, skip, steps;
@@ -88,9 +88,10 @@ struct PagedSpan {
 __host__ __device__ inline PagedSpan paged_span(int lo, int hi, int window, int sinks, int step) {
     PagedSpan s;
     s.first = window > 0 && lo >= window ? lo - window + 1 : 0;
-    const int sink = sinks < s.first ? sinks : s.first;
+    // no keys past hi, where a length passes its table
+    const int keys = hi < 0 ? 0 : hi + 1, before = keys < s.first ? keys : s.first, sink = sinks < before ? sinks : before;
     const int fs = s.first / step;
-    s.sink_steps = (sink + step - 1) / step;
+    s.sink_steps = sink / step + (sink % step != 0);
     if (s.sink_steps > fs) s.sink_steps = fs;
     s.skip = fs - s.sink_steps;
     s.steps = hi < 0 ? 0 : hi / step + 1 - s.skip;
@@ -148,9 +149,9 @@ __device__ __forceinline__ bool paged_request(const PagedCall& c, int b, int* st
     *L = max(c.seq_lens[b], 0) - past;
     return order;
 }
-// The last key that a table has a place for.
+// The last key that a table has a place for; two steps of keys past it are in 32 bits too.
 __device__ __forceinline__ int paged_key_cap(const PagedCall& c) {
-    return (int)min(((int64_t)c.max_blocks << c.page_shift) - 1, (int64_t)0x7fffffff);
+    return (int)min(((int64_t)c.max_blocks << c.page_shift) - 1, (int64_t)0x7fffffff - 128);
 }
 
 // n / group for n < 2^32 / group: the magic's error, under group / 2^32, times n
