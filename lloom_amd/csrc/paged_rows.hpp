@@ -234,7 +234,8 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
 #pragma unroll 1
                 for (int g = 0; g < 4; g++) {
                     if (!(who >> (16 * g) & 0xffff)) continue;
-                    const float zr = __shfl(zj, 16 * g + r, 64), pr = __builtin_amdgcn_exp2f(zr - base);
+                    const float pr = __builtin_amdgcn_exp2f(__shfl(zj, 16 * g + r, 64) - base);
+                    const bool sees = __shfl(seen, 16 * g + r, 64) >> j & 1;  // zero times it is no zero either
                     const int pg = __shfl(vp, 16 * g, 64);
                     int shift = c.page_shift;
                     asm volatile("" : "+s"(shift));  // or the main loop carries these loads' addresses
@@ -245,7 +246,7 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
                         const uint16_t* at = src;
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            o[i][e] += zr != -INFINITY ? pr * f16_to_f32(*at) : 0.0f;
+                            o[i][e] += sees ? pr * f16_to_f32(*at) : 0.0f;
                             at += 1 << shift;
                         }
                         src += 16 << shift;

@@ -340,6 +340,8 @@ __device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& c
                 for (int e = 0; e < 16 * ST; e++) zk = e == bit ? z[e >> 4][e & 15] : zk;
                 zk = __shfl(zk, side * 32 + r, 64);
                 const float pk = __builtin_amdgcn_exp2f(__builtin_fmaf(zk, factor, -base));
+                // zero times it is no zero either
+                if (key0 + k > pos_key || (key0 + k < win && key0 + k >= c.sinks)) continue;
                 int side4 = 4 * half;
                 asm volatile("" : "+v"(side4));  // or the main loop carries these reads' addresses
                 const uint8_t* from = at + C::K_BYTES + (k & 7) * 2;
@@ -349,7 +351,7 @@ __device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& c
                     for (int j = 0; j < 16; j++) {
                         const int dim = 32 * i + 8 * (j >> 2) + side4 + (j & 3);
                         const uint16_t x = *(const uint16_t*)(from + dim * 128 + (k >> 3 ^ (dim >> 1 & 7)) * 16);
-                        o[i][j] += zk != -INFINITY ? pk * f16_to_f32(x) : 0.0f;
+                        o[i][j] += pk * f16_to_f32(x);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }

@@ -78,3 +78,19 @@ def test_keys_whose_scores_are_minus_infinity(way, first, last):
     assert last < 10 ** 6 or nan.all()
     _check(s, _run(s, window=40), 40)
     _check(s, _run(s, window=40, sinks=3), 40, 3)
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("first,last", [(0, 1), (70, 75), (20, 40)])
+@pytest.mark.parametrize("way", WAYS)
+def test_values_that_are_no_numbers_at_keys_of_no_weight(way, first, last, bad):
+    """Zero times them is NaN, in the rows that see them, wherever the key is in a step that not all rows see whole."""
+    s = _minus_infinity(way, first, last, F16)
+    page = s["k"].shape[2]
+    for b, length in enumerate(s["seq_lens"]):
+        for p in range(first, min(last, length)):
+            s["v"][s["tables"][b][p // page], :, ::3, p % page] = bad
+    nan = _check(s, _run(s))
+    assert nan[..., ::3].any() or max(s["seq_lens"]) <= first
+    _check(s, _run(s, window=40), 40)
+    _check(s, _run(s, window=40, sinks=3), 40, 3)
