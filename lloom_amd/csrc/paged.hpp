@@ -200,6 +200,10 @@ __device__ __forceinline__ void split8(const float (&x)[8], half8_t& hi, half8_t
     }
 }
 
+// Queries are scaled so that a row's largest is in 2^Q_SHIFT * [1, 2): halves then
+// hold the others exactly to 2^-22 of them or 2^-38 of the largest.
+constexpr int Q_SHIFT = 14;
+
 // Zeroes the infinities and NaN among 8 keys' values; bit j of the result: there
 // was one at key j.  An exponent of all ones and 1 more is the sign's bit.
 __device__ __forceinline__ uint32_t take_odd(uint4& v) {

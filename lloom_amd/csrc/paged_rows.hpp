@@ -70,7 +70,7 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
     float factor = c.scale;
     const int64_t qi = (int64_t)(it.start + tok0 + tok) * c.q_stride + (int64_t)head * D + 8 * g4;
     if constexpr (F32) {
-        // times a power of two of the row's own, so that its largest is in [1, 2)
+        // times a power of two of the row's own, so that its largest is in 2^Q_SHIFT * [1, 2)
         float x[DC][8], top = 0.0f;
 #pragma unroll
         for (int i = 0; i < DC; i++) {
@@ -87,8 +87,8 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
         top = __builtin_fmaxf(top, partner32(top));
         int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
         e = min(max(e, -100), 100);  // a zero, subnormal or infinite row
-        const float down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-        factor *= __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+        const float down = __builtin_bit_cast(float, (uint32_t)(127 + Q_SHIFT - e) << 23);
+        factor *= __builtin_bit_cast(float, (uint32_t)(127 - Q_SHIFT + e) << 23);
 #pragma unroll
         for (int i = 0; i < DC; i++) {
 #pragma unroll

@@ -88,7 +88,7 @@ __device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& c
     float factor = __builtin_fabsf(c.scale);
     const int64_t qi = (int64_t)(it.start + tok0 + tok) * c.q_stride + (int64_t)(h * c.group + row + mine - tok * c.group) * D + 8 * half;
     if constexpr (F32) {
-        // times a power of two of the row's own, so that its largest is in [1, 2)
+        // times a power of two of the row's own, so that its largest is in 2^Q_SHIFT * [1, 2)
         float top = 0.0f;
 #pragma unroll
         for (int i = 0; i < DC; i++) {
@@ -101,8 +101,8 @@ __device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& c
         top = __builtin_fmaxf(top, partner32(top));
         int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
         e = min(max(e, -100), 100);  // a zero, subnormal or infinite row
-        const float down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23) * (c.scale < 0.0f ? -1.0f : 1.0f);
-        factor *= __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+        const float down = __builtin_bit_cast(float, (uint32_t)(127 + Q_SHIFT - e) << 23) * (c.scale < 0.0f ? -1.0f : 1.0f);
+        factor *= __builtin_bit_cast(float, (uint32_t)(127 - Q_SHIFT + e) << 23);
 #pragma unroll
         for (int i = 0; i < DC; i++) {
             const float4 a = *(const float4*)((const float*)c.q + qi + 16 * i);

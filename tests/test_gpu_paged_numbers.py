@@ -94,3 +94,16 @@ def test_values_that_are_no_numbers_at_keys_of_no_weight(way, first, last, bad):
     assert nan[..., ::3].any() or max(s["seq_lens"]) <= first
     _check(s, _run(s, window=40), 40)
     _check(s, _run(s, window=40, sinks=3), 40, 3)
+
+
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("large", [2.0 ** 6, 2.0 ** 12, 2.0 ** 16])
+def test_f32_queries_with_one_large_value(way, large):
+    """The others keep their bits beside it.  (What is left of a value is under 2^-22 of it or, with the row's largest at
+    2^14 or more, half of half's least step, 2^-25, which is 2^-39 of the largest: 2^-23 here, of values of size 2.4.
+    The keys are zero where the large one is, so that the bound is that of the others.)"""
+    s = R.case(*WAYS[way], 64, F32, device=DEV)
+    s["q"] = s["q"] * 1.5
+    s["q"][..., 9] = large
+    s["k"][..., 9].mul_(0.0)
+    _check(s, _run(s))
