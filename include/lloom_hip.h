@@ -309,8 +309,9 @@ int lloom_hip_paged_append(lloom_hip_ctx* ctx, int act_dtype, const void* k_dev,
  * position j <= p with window = 0, j > p - window or j < sinks, and its
  * result is sum_j softmax_j(scale q.k_j) v_j over what it sees: zero where it
  * sees nothing, where no request owns the row, and nothing of a page out of
- * [0, pages).  Values that a token does not see may be anything, and pages that
- * none sees any number (a server's freed ones before a window).  A q_start that
+ * [0, pages).  Values that a token does not see may be anything (an infinite one
+ * of v that it sees makes what it enters infinite or NaN), and pages that none
+ * sees any number (a server's freed ones before a window).  A q_start that
  * falls anywhere or is negative leaves the whole call out: out is zero, EPAGE.  Where
  * it passes `tokens`, the rows that there are keep their positions, EPAGE too.  Sums
  * and the softmax are f32.  With F32 q the products take q and the weights as two halves

@@ -203,6 +203,20 @@ __device__ __forceinline__ void split8(const float (&x)[8], half8_t& hi, half8_t
 // Queries are scaled so that a row's largest is in 2^Q_SHIFT * [1, 2): halves then
 // hold the others exactly to 2^-22 of them or 2^-38 of the largest.
 constexpr int Q_SHIFT = 14;
+// Keys may be infinite: lo has x's sign and is not zero, or the two products would be
+// infinities of both signs, or NaN.  hi is x towards zero for that, and lo half's least
+// number more than the rest, 2^-38 of the row's largest.
+__device__ __forceinline__ void split8_query(const float (&x)[8], half8_t& hi, half8_t& lo) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const auto h = __builtin_amdgcn_cvt_pkrtz(x[i], x[i + 1]);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            hi[i + j] = (_Float16)h[j];
+            lo[i + j] = (_Float16)(x[i + j] - (float)h[j] + __builtin_copysignf(0x1p-24f, x[i + j]));
+        }
+    }
+}
 
 // Zeroes the infinities and NaN among 8 keys' values; bit j of the result: there
 // was one at key j.  An exponent of all ones and 1 more is the sign's bit.

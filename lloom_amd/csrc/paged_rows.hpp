@@ -93,7 +93,7 @@ __device__ __forceinline__ void paged_rows(const PagedCall& c, const PagedCut& c
         for (int i = 0; i < DC; i++) {
 #pragma unroll
             for (int j = 0; j < 8; j++) x[i][j] *= down;
-            split8(x[i], qh[i], ql[i]);
+            split8_query(x[i], qh[i], ql[i]);
         }
     } else {
 #pragma unroll

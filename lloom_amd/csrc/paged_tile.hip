@@ -108,7 +108,7 @@ __device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& c
             const float4 a = *(const float4*)((const float*)c.q + qi + 16 * i);
             const float4 b = *(const float4*)((const float*)c.q + qi + 16 * i + 4);
             const float v[8] = {a.x * down, a.y * down, a.z * down, a.w * down, b.x * down, b.y * down, b.z * down, b.w * down};
-            split8(v, qh[i], ql[i]);
+            split8_query(v, qh[i], ql[i]);
         }
     } else {
         const uint32_t turn = c.scale < 0.0f ? 0x80008000u : 0u;

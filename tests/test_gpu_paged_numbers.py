@@ -107,3 +107,18 @@ def test_f32_queries_with_one_large_value(way, large):
     s["q"][..., 9] = large
     s["k"][..., 9].mul_(0.0)
     _check(s, _run(s))
+
+
+@pytest.mark.parametrize("first,last", SPOILT)
+@pytest.mark.parametrize("way", WAYS)
+def test_infinite_keys_and_f32_queries(way, first, last):
+    """Scores of -inf as from f16 queries, also where a query's value is exact in one half, or is none."""
+    s = _minus_infinity(way, first, last, F32)
+    s["q"][::3, :, 5] = s["q"][::3, :, 5].half().float()
+    s["q"][1::3, ::2, 5] = 0.25
+    nan = _check(s, _run(s))
+    assert last < 10 ** 6 or nan.all()
+    _check(s, _run(s, window=40, sinks=3), 40, 3)
+    s["q"][:, -1, 5] = 0.0  # zero times it is NaN
+    nan = _check(s, _run(s))
+    assert nan[:, -1].any() or max(s["seq_lens"]) <= first
