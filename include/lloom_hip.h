@@ -315,7 +315,8 @@ int lloom_hip_paged_append(lloom_hip_ctx* ctx, int act_dtype, const void* k_dev,
  * falls anywhere or is negative leaves the whole call out: out is zero, EPAGE.  Where
  * it passes `tokens`, the rows that there are keep their positions, EPAGE too.  Sums
  * and the softmax are f32.  With F32 q the products take q and the weights as two halves
- * each (exact to about 2^-22); with F16 the weights are rounded to halves.
+ * each (exact to about 2^-22); with F16 the weights of requests with many rows are
+ * rounded to halves, those of others two halves as well.
  * max_new: no request has more new tokens (0: not known); only speed depends
  * on it. */
 int lloom_hip_paged_attention(lloom_hip_ctx* ctx, int act_dtype, const void* q_dev, int64_t q_stride, int64_t tokens,

@@ -243,7 +243,11 @@ __device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& c
             for (int j = 0; j < 8; j++) l += p[j];
             split8(p, ph, pl);
         } else {
-            // the sum of the weights as rounded, which is what the values are summed with
+            // Rounded to halves, and summed as rounded, which is what the values are summed
+            // with.  Two halves as for f32 cost half the matrix instructions again: 139
+            // against 113 us for a prompt of 4096 tokens (73 and 61 for two chunks of 2048
+            // with a window), for outputs off by 2.06e-4 of 64 bits, what their own
+            // rounding leaves, and not by 2.43e-4.
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 const half2_t two = {(_Float16)p[j], (_Float16)p[j + 1]}, one = {(_Float16)1.0f, (_Float16)1.0f};
