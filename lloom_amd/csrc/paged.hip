@@ -1,6 +1,6 @@
 // paged.hip -- block tables and slot maps from request lengths, and the
 // writes of new k and v rows into the pages of the cache (paged.hpp).
-#include "kernels.hpp"
+#include "paged_launch.hpp"
 #include "kq_common.hpp"
 #include "paged.hpp"
 

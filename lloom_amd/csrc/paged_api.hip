@@ -8,6 +8,7 @@
 #include "api_internal.hpp"
 #include "kq_common.hpp"
 #include "paged.hpp"
+#include "paged_launch.hpp"
 
 using namespace lloom;
 

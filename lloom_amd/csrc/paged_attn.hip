@@ -1,6 +1,6 @@
 // paged_attn.hip -- the paged attention of calls with few rows a request alone
 // (paged_rows.hpp).
-#include "kernels.hpp"
+#include "paged_launch.hpp"
 #include "kq_common.hpp"
 #include "paged_rows.hpp"
 

@@ -26,7 +26,7 @@
 // requests, 62 MB), for 0.1 of 17.8 us less; 0 to 2 % in other calls.
 #pragma once
 
-#include "kernels.hpp"
+#include "paged_launch.hpp"
 #include "kq_common.hpp"
 #include "paged.hpp"
 

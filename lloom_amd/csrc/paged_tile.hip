@@ -18,7 +18,7 @@
 // 370 instructions, and a long tile that is left alone on its CU takes 3900 clocks
 // for it.  Left out by turns, loads are 24 us of the prompt's 111 (without the check
 // of the reference, which is 10), the products with V 13, the weights 13.
-#include "kernels.hpp"
+#include "paged_launch.hpp"
 #include "kq_common.hpp"
 #include "paged_rows.hpp"
 
