@@ -218,21 +218,18 @@ __device__ __forceinline__ void split8_query(const float (&x)[8], half8_t& hi, h
     }
 }
 
-// Zeroes the infinities and NaN among 8 keys' values; bit j of the result: there
-// was one at key j.  An exponent of all ones and 1 more is the sign's bit.
-__device__ __forceinline__ uint32_t take_odd(uint4& v) {
+// Bit j: an infinity or a NaN at key j of 8 keys' values.  An exponent of all ones and
+// 1 more is the sign's bit.
+__device__ __forceinline__ uint32_t odd_keys(uint4 v) {
     uint32_t odd = 0;
-    uint32_t* w = (uint32_t*)&v;
+    const uint32_t* w = (const uint32_t*)&v;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const uint32_t at = ((w[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-        w[j] &= ~(at | (at - (at >> 15)));
         odd |= (at >> 15 & 1) << (2 * j) | (at >> 31) << (2 * j + 1);
     }
     return odd;
 }
-// Bit j: an infinity or a NaN at key j of 8 keys' values.
-__device__ __forceinline__ uint32_t odd_keys(uint4 v) { return take_odd(v); }
 // Zeroes the values of the keys whose bit is not set.
 __device__ __forceinline__ void keep8(uint4& v, uint32_t bits) {
     uint32_t* w = (uint32_t*)&v;

@@ -55,7 +55,7 @@ struct PagedTile {
 
 // Workgroup `wg`; lds: two stages, then bad_group.
 template <int D, bool F32>
-__device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& cut, float* parts, int wg, int wgs, uint8_t* lds,
+__device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& cut, float* parts, int wg, uint8_t* lds,
                                            int (*bad_group)[4]) {
     using C = PagedTile<D, F32>;
     constexpr int DC = D / 16, DT = D / 32, ST = 2;
@@ -498,7 +498,7 @@ __global__ __launch_bounds__((PagedTile<D, F32>::THREADS), D == 256 ? 1 : 2) voi
     };
     __shared__ __align__(16) Lds lds;
     const int wg = blockIdx.x;
-    if (wg < tile_wgs) paged_tile<D, F32>(c, tiles, tile_parts, wg, tile_wgs, lds.t.stages, lds.t.bad_group);
+    if (wg < tile_wgs) paged_tile<D, F32>(c, tiles, tile_parts, wg, lds.t.stages, lds.t.bad_group);
     else paged_rows<D, F32, C::WAVES>(c, rows, row_parts, wg - tile_wgs, gridDim.x - tile_wgs, lds.r.acc, lds.r.stat, c.joins + PAGED_JOINS / 2);
 }
 
