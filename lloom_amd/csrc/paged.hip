@@ -135,7 +135,8 @@ hipError_t launch_paged_plan(const int* cached, const int* fresh, int requests, 
 // whose slots follow each other from a multiple of 8 is stored as one 16-byte
 // piece a dimension, through LDS; the tokens that no run holds (a decode step's,
 // or the ends of a prompt) as single halves.  8192 tokens of 8 x 128 in f16 (67 MB)
-// take 16 us, 4.2 TB/s where a large copy reaches 4.9; 64 tokens 3.4, a launch.
+// take 16 us, 4.2 TB/s where a large copy reaches 4.9, in f32 (101 MB) 22, 4.5 TB/s; 64
+// tokens 3.4, a launch.
 struct AppendArgs {
     const void *k, *v;
     uint16_t *kc, *vc;
@@ -248,7 +249,10 @@ hipError_t launch_paged_append(int act, const void* k, int64_t k_stride, const v
     AppendArgs a{k, v, (uint16_t*)kc, (uint16_t*)vc, slots, flags, k_stride, v_stride, (int64_t)pages << page_shift,
                  tokens, kv_heads, dim, page_shift};
     // heads of 128 in f16, 8 tokens a workgroup against 64: 64 tokens of 8 heads 3.3 and
-    // 6.9 us, 2048 7.5 and 8.8, 4096 12.0 and 10.7, 8192 20.1 and 15.9
+    // 6.9 us, 2048 7.5 and 8.6, 4096 11.9 and 10.7, 8192 21.4 and 16.6; f32 8.7 and 9.9,
+    // 14.6 and 12.9, 26.0 and 21.3.  Heads of 64, 96 and 256 turn between the same two, in
+    // both types (2048 and 4096 tokens of 64 in f16: 5.7 and 6.1, 8.7 and 7.3; of 256 in
+    // f32: 14.4 and 15.2, 27.8 and 22.2).
     const bool few = (int64_t)tokens * kv_heads < 20480;
     if (act == T_F32) few ? append_as<true, 8>(a, s) : append_as<true, 64>(a, s);
     else few ? append_as<false, 8>(a, s) : append_as<false, 64>(a, s);

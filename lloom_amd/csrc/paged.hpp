@@ -65,10 +65,15 @@ struct PagedCut {
 // integers of a cut: chunk, whether the call is refused, then from 16 on items and splits summed
 constexpr int PAGED_INDEX = 16 + 2 * PAGED_MAX_REQUESTS;
 // Whether a request is one of few rows, which are served 16 at a time, each 16
-// reading its keys.  Measured with 16 requests of up to 8191 tokens (heads of 128, 4
+// reading its keys.  Measured with 16 requests of lengths up to 8191 (heads of 128, 4
 // key heads of 4, f16), the kernel of few rows against that of many: 16 rows each
-// 18 and 28 us, 64 22 and 37; two of 30000 tokens, 76 rows 64 and 105, 140 rows 175
-// and 114; eight of 300 tokens, 200 rows 8 and 13, 500 rows 16 and 15.
+// 18 and 28 us, 64 22 and 37; two of 30000 tokens, 64 rows 53 and 86, 128 rows 93 and
+// 173, 192 rows 233 and 125; eight of 900, 96 rows 16 and 30, 256 rows 34 and 36, 400
+// rows 50 and 38; eight of 300, 128 rows 11 and 17, 256 rows 19.5 and 19.0.  In f32
+// and with heads of 64 and 96 the first is ahead by more; with heads of 256 from 192
+// rows on by none (0.8 to 0.9 of it the other).  Sixteen requests that all have 8191
+// tokens are served better by the other from 32 rows on (77 and 62 us; 96 rows 122
+// and 77; heads of 64 37 and 33, of 256 141 and 113): they fill the card with either.
 constexpr int PAGED_FEW = 96, PAGED_FEW_SHORT = 256, PAGED_SHORT = 1024;
 __host__ __device__ inline bool paged_few(int64_t rows, int64_t length) {
     return rows <= PAGED_FEW || (rows <= PAGED_FEW_SHORT && length <= PAGED_SHORT);

@@ -16,8 +16,8 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_paged_rows(PagedCall c, Page
 
 // The sums over a call's requests that paged_find looks an item up in, a workgroup a
 // cut: 4 consecutive requests a thread.  4 us with its launch.  Without it every wave
-// read every request: 241 us against 88 + 4 for 1024 single tokens (188 MB), 57 against
-// 49 + 4 for 256, 208 against 142 + 4 for 224 requests with 24 chunks of 509 tokens; the
+// read every request: 241 us against 90 + 5 for 1024 single tokens (188 MB), 57 against
+// 51 + 4 for 256, 208 against 145 + 5 for 224 requests with 24 chunks of 509 tokens; the
 // search by every wave is 2 us faster up to 128 requests, which is left.
 constexpr int INDEX_WG = 1024, INDEX_EACH = PAGED_MAX_REQUESTS / INDEX_WG;
 

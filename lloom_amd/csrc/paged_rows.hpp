@@ -13,13 +13,15 @@
 // straight from the cache in 16-byte pieces, with no LDS.
 //
 // Bound by reading the cache: one request of 131072 tokens (8 key heads of 128, 537
-// MB) takes 98 us, 5.5 TB/s where a large read reaches 6.4.  With less to read,
+// MB) takes 100 us, 5.4 TB/s where a large read reaches 6.4.  With less to read,
 // latencies in a row are what it takes: of the 10 us of one request of 641 tokens
 // (1.3 MB) the search for the item is 1.2, the page table and a wave's first K and
 // V 2, the second four waves' another 1.7 (a CU's 32 KB of L1 hold what is in
 // flight: 24 B a clock), the waves' sums 0.5, the counter 0.8, the parts' join 1.5,
 // the launch the rest.  Loads a step ahead of the products are there already: eight
 // waves' 16 KB each.
+// Heads of 256 in f32 hold more than the registers: 43 are spilled (31 us for 16 requests
+// of up to 8191 tokens, 66 MB, where f16 takes 21).
 //
 // The weights are two halves (2^-22 of them) for f16 queries too: rounded to one, an
 // output was off by 2.19e-4 of 64 bits and not by the 2.07e-4 of its own rounding (32

@@ -11,9 +11,11 @@
 // Two workgroups a CU: the one's waits and prologue run beside the other's products
 // (one of 8 waves, which share a step's 128 keys: 119 against 116 us for a prompt of
 // 4096 tokens, 16 heads of 128 in f16, and 100 against 64 for two chunks of 2048 with
-// a window of 1024).  The prompt runs at 610 TFLOP/s in 113 us, a large library
+// a window of 1024).  The prompt runs at 640 TFLOP/s in 107 us, a large library
 // product at 1300; with f32 q and p in two halves each, so twice the matrix
-// instructions, four chunks of 509 over 8000 take 131 us (760 TFLOP/s of them).
+// instructions, four chunks of 509 over 8000 take 125 us (795 TFLOP/s of them).  f32
+// spills 5 registers with heads of 128, and 23 with heads of 256 (two chunks of 1500 over
+// 1000: 172 us, 101 in f16).
 // Issue and waits bound it, no unit: a step of a wave is 32 MFMAs (1024 clocks) among
 // 370 instructions, and a long tile that is left alone on its CU takes 3900 clocks
 // for it.  Left out by turns, loads are 24 us of the prompt's 111 (without the check

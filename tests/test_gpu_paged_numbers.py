@@ -128,8 +128,8 @@ def test_infinite_keys_and_f32_queries(way, first, last):
 @pytest.mark.parametrize("weight", [0.5 + 2.0 ** -12 - 2.0 ** -18, 0.5 + 2.0 ** -12 + 2.0 ** -18, 0.75 + 2.0 ** -12 - 2.0 ** -17])
 @pytest.mark.parametrize("cached,new", [(299, 1), (999, 3), (200, 100), (900, 90)])
 def test_values_that_are_all_alike_come_out_as_they_are(cached, new, weight, act):
-    """A key of weight 1 in 32, so that whoever sums a few of them has it, and others of `weight`, which half rounds by nearly half a step: a sum of weights that was not of
-    those that the values are summed with would show that in full.  The result is off by the roundings of both sums, 2 n +
+    """A key of weight 1 in 32, so that whoever sums a few of them has it, and others of `weight`, which half rounds by
+    nearly half a step: a sum of weights that was not of those that the values are summed with would show that in full.  The result is off by the roundings of both sums, 2 n +
     64 of half an f32 step, and f32's weights by twice 2^-22: 1.3e-4 at 1002 keys, under the half step of 2^-12 to the
     number below 1 in f16, so that there it is 1, -1, 0.5 and 2 exactly."""
     s = R.case([cached], [new], 16, 1, 4, 64, act, device=DEV)
