@@ -93,7 +93,7 @@ int lloom_hip_ctx_set_prefill_mma(lloom_hip_ctx* ctx, int mode);
  * id seen by a routed matmul, or an out-of-range embedding id: EEXPERT; a page,
  * slot or length that a paged-cache call could not serve: EPAGE) recorded
  * since the last check, and clear it.  Where both were seen, EEXPERT is
- * reported and EPAGE by the next call. */
+ * reported and EPAGE by the next call.  Other threads may have calls running. */
 int lloom_hip_ctx_sync(lloom_hip_ctx* ctx);
 
 /* ---------------------------------------------------------------- memory --

@@ -102,7 +102,7 @@ __device__ __forceinline__ void paged_tile(const PagedCall& c, const PagedCut& c
         }
         top = __builtin_fmaxf(top, partner32(top));
         int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
-        e = min(max(e, -100), 100);  // a zero, subnormal or infinite row
+        e = min(max(e, Q_SHIFT - 126), 127);  // a zero, subnormal or infinite row; both powers are normal
         const float down = __builtin_bit_cast(float, (uint32_t)(127 + Q_SHIFT - e) << 23) * (c.scale < 0.0f ? -1.0f : 1.0f);
         factor *= __builtin_bit_cast(float, (uint32_t)(127 - Q_SHIFT + e) << 23);
 #pragma unroll

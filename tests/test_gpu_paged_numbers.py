@@ -142,3 +142,14 @@ def test_values_that_are_all_alike_come_out_as_they_are(cached, new, weight, act
     n = cached + new
     tol = 0.0 if act == F16 else ((2 * n + 64) * 2.0 ** -24 + 2 * 2.0 ** -22)
     assert ((got.double() - worth).abs() <= tol * worth.abs()).all()
+
+
+@pytest.mark.parametrize("size", [1e-36, 1e-20, 1e20, 3e37])
+@pytest.mark.parametrize("way", WAYS)
+def test_f32_queries_of_any_size(way, size):
+    """q over f32's range, with a scale that makes of it scores of ordinary size."""
+    s = R.case(*WAYS[way], 64, F32, device=DEV)
+    q = s["q"]
+    s["q"] = q * size
+    s["scale"] = 0.125 / size
+    _check(s, _run(s, scale=s["scale"]))
