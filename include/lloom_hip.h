@@ -287,7 +287,8 @@ int lloom_hip_embedding(lloom_hip_ctx* ctx, int ggml_type, const void* w_dev, in
  * ceil(seq / page_size) - ceil(cached / page_size) pages, from free[0 ..] in the
  * requests' order, which are stored in its table; taken[0] = pages in all.  Rows
  * past the last request's (a padded batch) get position 0 and slot -1; tokens
- * that no page is left for slot -1, and -1 in the table. */
+ * that no page is left for slot -1, and -1 in the table; tokens whose page is
+ * negative, in the table or in the list, slot -1.  Both are reported. */
 int lloom_hip_paged_plan(lloom_hip_ctx* ctx, const uint32_t* cached_dev, const uint32_t* new_dev, int64_t requests,
                          int64_t tokens, void* tables_dev, int64_t table_stride, int64_t max_blocks,
                          const uint32_t* free_dev, int64_t free_count, int64_t page_size, void* q_start_dev,
@@ -317,8 +318,8 @@ int lloom_hip_paged_append(lloom_hip_ctx* ctx, int act_dtype, const void* k_dev,
  * and the softmax are f32.  With F32 q the products take q and the weights as two halves
  * each (exact to about 2^-22); with F16 the weights of requests with many rows are
  * rounded to halves, those of others two halves as well.
- * max_new: no request has more new tokens (0: not known); only speed depends
- * on it. */
+ * max_new: no request has more new tokens (0: not known); only speed and
+ * roundings depend on it. */
 int lloom_hip_paged_attention(lloom_hip_ctx* ctx, int act_dtype, const void* q_dev, int64_t q_stride, int64_t tokens,
                               const void* k_cache_dev, const void* v_cache_dev, int64_t pages, int64_t kv_heads,
                               int64_t group, int64_t head_dim, int64_t page_size, const void* tables_dev,

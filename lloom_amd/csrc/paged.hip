@@ -114,6 +114,7 @@ __global__ __launch_bounds__(PLAN_WG) void k_paged_plan(PlanArgs a) {
             if ((pos & (page - 1)) == 0) *entry = pg;  // -1 where no page is left: attention passes such a page over
         }
     }
+    if (pg < 0) a.flags[0] = 1;
     a.positions[n] = sat31(pos);
     a.slots[n] = pg < 0 ? -1 : ((int64_t)pg << a.page_shift) + (pos & (page - 1));
 }

@@ -134,7 +134,7 @@ def paged_attention(q, k_cache, v_cache, block_tables, q_start, seq_lens, scale=
     head h // (heads // kv_heads).  The token at position p sees position j <= p with window = 0, j > p - window or
     j < sinks.  A q_start that falls anywhere or is negative leaves the call out (out is zero, paged_check() raises);
     one that passes the number of rows leaves out those that are not there (paged_check() raises).  scale: 1 / sqrt(head_dim) by default.  max_new: the most new tokens of any request, where the caller
-    knows it (1 for a decode step): only speed depends on it."""
+    knows it (1 for a decode step): only speed and roundings depend on it."""
     pages, heads, page, dim = _cache_dims(k_cache, v_cache, "paged_attention")
     if q.dim() != 3 or heads == 0 or q.shape[1] == 0 or q.shape[1] % heads:
         raise LloomHipError(3, f"paged_attention: q {tuple(q.shape)} is not [tokens, heads, {dim}] with a multiple of "

@@ -99,3 +99,15 @@ def test_rows_that_are_not_there(way, cut, act):
     plan = L.paged_plan(_ints(cached), _ints(new), s["q"].shape[0], s["t_tables"], _ints([0] * 4096), WAYS[way][2])
     assert plan.q_start.tolist() == s["q_start"] and plan.seq_lens.tolist() == s["seq_lens"]
     _reported()
+
+
+@pytest.mark.parametrize("tables,free", [([[3, -1, 0], [5, 0, 0]], [7, 8]), ([[3, 4, 0], [5, 0, 0]], [7, -2]), ([[3, 4, 0], [-2 ** 31, 0, 0]], [7, 8])])
+def test_a_plan_reports_pages_that_are_none(tables, free):
+    """Tokens whose page is negative, in the table of what a request holds or in the free list."""
+    cached, new = [20, 10], [14, 20]
+    got = L.paged_plan(_ints(cached), _ints(new), 34, _ints(tables), _ints(free), 16)
+    _reported()
+    start, lens, pos, slots, taken, after = R.plan(cached, new, 34, tables, free, 16)
+    assert got.slots.tolist() == slots and -1 in slots and got.positions.tolist() == pos
+    assert got.q_start.tolist() == start and got.seq_lens.tolist() == lens and got.taken.tolist() == [taken]
+    assert got.block_tables.tolist() == after
