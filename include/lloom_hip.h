@@ -51,7 +51,9 @@ enum {
     LLOOM_HIP_Q8_0 = 8,
     LLOOM_HIP_Q4K = 12,
     LLOOM_HIP_Q6K = 14,
-    LLOOM_HIP_Q8K = 15
+    LLOOM_HIP_Q8K = 15,
+    LLOOM_HIP_BF16 = 30,       /* the 8-bit floating-point calls alone      */
+    LLOOM_HIP_E4M3 = 100       /* no GGUF type: 8-bit floating point        */
 };
 
 typedef struct lloom_hip_ctx lloom_hip_ctx;
@@ -330,6 +332,68 @@ int lloom_hip_paged_attention(lloom_hip_ctx* ctx, int act_dtype, const void* q_d
 /* Workspace of an attention call of this shape, to reserve before a capture. */
 int lloom_hip_paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t kv_heads, int64_t group,
                                               int64_t head_dim, int64_t max_new, size_t* bytes);
+
+/* ------------------------------------------------- 8-bit floating point --
+ * Products with e4m3 weights (OCP: 4 bits of exponent, 3 of fraction, no
+ * infinities, at most 448) that have an f32 scale for each block of 128 x 128,
+ * dense and grouped by expert, beside the packed integer ones:
+ *   y[m][n] = sum_b sx[m][b] sw[n / 128][b] sum_{k in b} qx[m][k] qw[n][k]
+ * over blocks b of 128 values of k (the last one may be shorter).  The weight is
+ * [n][k] of bytes with scales [ceil(n / 128)][ceil(k / 128)], as checkpoints
+ * hold them; k is a multiple of 16.  Activations are F32, F16 or BF16, or E4M3
+ * with a scale for each block of a row.  Rows and weights 16-byte aligned.  The
+ * scales of a block are multiplied in f32: products of the two below 2^-126
+ * lose bits.  The calls neither synchronize nor copy; what only the GPU can
+ * see is left out of the result as said below and reported by the next
+ * lloom_hip_ctx_sync as LLOOM_HIP_EEXPERT.
+ *
+ * lloom_hip_fp8_quantize: rows of x [rows][k], x_stride elements apart, into
+ * q [rows][k] and scales [ceil(k / 128)][scales_stride] (a block's rows side by
+ * side).  A block's scale is 2^e with the least e >= -126 for which its largest
+ * finite value is at most 448 * 2^e, 1 for a block of zeros; q is the nearest
+ * e4m3 number of x / scale, ties to even (the division is exact); infinities and
+ * NaN become NaN. */
+int lloom_hip_fp8_quantize(lloom_hip_ctx* ctx, const void* x_dev, int x_dtype, int64_t x_stride, int64_t rows, int64_t k,
+                           void* q_dev, float* scales_dev, int64_t scales_stride, void* stream);
+
+/* The same of silu(gate) * up = gate / (1 + exp(-gate)) * up, formed in f32. */
+int lloom_hip_fp8_silu_mul(lloom_hip_ctx* ctx, const void* gate_dev, int64_t gate_stride, const void* up_dev,
+                           int64_t up_stride, int dtype, int64_t rows, int64_t k, void* q_dev, float* scales_dev,
+                           int64_t scales_stride, void* stream);
+
+/* Weights [experts][n][k] (contiguous) into q of that shape and scales
+ * [experts][ceil(n / 128)][ceil(k / 128)], chosen as above. */
+int lloom_hip_fp8_quantize_weight(lloom_hip_ctx* ctx, const void* w_dev, int w_dtype, int64_t experts, int64_t n,
+                                  int64_t k, void* q_dev, float* scales_dev, void* stream);
+
+/* y[m][n] = x . W^T.  x_dtype E4M3: the scale of row r, block b is
+ * x_scales[r * xs_row + b * xs_block], any f32; else x_scales is not read and
+ * rows are brought into 8 bits as lloom_hip_fp8_quantize does.  y F32, F16 or
+ * BF16 (nearest even), 16-byte aligned, contiguous. */
+int lloom_hip_fp8_matmul(lloom_hip_ctx* ctx, const void* w_dev, const float* w_scales_dev, int64_t n, int64_t k,
+                         const void* x_dev, int x_dtype, int64_t x_stride, const float* x_scales_dev, int64_t xs_row,
+                         int64_t xs_block, int64_t m, void* y_dev, int y_dtype, void* stream);
+
+/* Planes (token * topk + slot) in the order of their experts, planes of one
+ * expert in their own: from ids [tokens][topk] starts[experts + 1] (the first
+ * place of each expert's planes), planes and tokens [tokens * topk] (int32; a
+ * plane's token is plane / topk).  Planes of negative ids (a padded batch) and
+ * of ids past the last expert (reported) come last, from starts[experts] on. */
+int lloom_hip_expert_plan(lloom_hip_ctx* ctx, const uint32_t* ids_dev, int64_t tokens, int64_t topk, int64_t experts,
+                          void* starts_dev, void* planes_dev, void* tokens_dev, void* stream);
+
+/* Products grouped by expert, ragged: W [experts][n][k] with scales
+ * [experts][ceil(n / 128)][ceil(k / 128)]; row i of `rows`, starts[e] <= i <
+ * starts[e + 1], is row gather[i] of x's x_rows (null: i) times weight e, and
+ * is stored at row scatter[i] of y's y_rows (null: i; no two alike).  Rows from
+ * starts[experts] on are zero.  Where starts do not begin with 0, fall, or pass
+ * rows, all of them are; a gather out of range is a row of zeros, a scatter out
+ * of range is not stored; each is reported. */
+int lloom_hip_fp8_grouped_matmul(lloom_hip_ctx* ctx, const void* w_dev, const float* w_scales_dev, int64_t experts,
+                                 int64_t n, int64_t k, const void* x_dev, int x_dtype, int64_t x_stride,
+                                 const float* x_scales_dev, int64_t xs_row, int64_t xs_block, int64_t x_rows,
+                                 const uint32_t* starts_dev, const uint32_t* gather_dev, const uint32_t* scatter_dev,
+                                 int64_t rows, void* y_dev, int y_dtype, int64_t y_rows, void* stream);
 
 /* ------------------------------------------------------- synthetic data --
  * The benchmark/test input generator (not part of the reference): SplitMix64

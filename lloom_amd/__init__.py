@@ -29,3 +29,12 @@ from .paged import (  # noqa: F401
     paged_check,
     paged_plan,
 )
+from .fp8 import (  # noqa: F401
+    ExpertPlan,
+    expert_plan,
+    fp8_grouped_matmul,
+    fp8_matmul,
+    fp8_quantize,
+    fp8_quantize_weight,
+    fp8_silu_mul,
+)

@@ -1,0 +1,232 @@
+// fp8.hpp -- products with e4m3 weights that have a scale for each block of
+// 128 x 128 (fp8_rows.hip, fp8_few.hip, fp8_tile.hip, fp8_api.hip): the calls'
+// launchers and what their kernels share.
+//
+//   y[m][n] = sum_b sx[m][b] sw[n / 128][b] sum_{k in b} qx[m][k] qw[n][k]
+//
+// over blocks b of 128 values of k, q the e4m3 numbers.  A block's inner sum is
+// formed on the matrix cores, the scales meet it in f32.
+#pragma once
+
+#include "kernels.hpp"
+#include "kq_common.hpp"
+
+namespace lloom {
+
+// Type ids beside those of kq_common.hpp: BF16 is GGUF's, E4M3 has none there.
+constexpr int T_BF16 = 30, T_E4M3 = 100;
+constexpr int FP8_BLOCK = 128;
+
+// A product's operands.  Rows of x are x_stride elements apart, its scales
+// (e4m3 x) at [row * xs_row + block * xs_block].  starts (null: one group of
+// all m rows): row i of group e, starts[e] <= i < starts[e + 1], is row
+// gather[i] of x (null: i) and is stored at row scatter[i] of y (null: i).
+struct Fp8Call {
+    const uint8_t* w;
+    const float* ws;
+    const void* x;
+    const float* xs;
+    void* y;
+    const int *starts, *gather, *scatter;
+    int* flags;  // [0]: rows, starts or ids out of range
+    int64_t x_stride, xs_row, xs_block;
+    int n, k, kb, nb, m, x_rows, y_rows, experts;
+};
+
+// fp8_rows.hip: rows of x (F32, F16, BF16; x_stride elements apart) into e4m3 q
+// [rows][k] and scales [block * scales_stride + row]; `up` (or null): of
+// silu(x) * up.
+hipError_t launch_fp8_rows(int type, const void* x, int64_t x_stride, const void* up, int64_t up_stride, int64_t rows,
+                           int64_t k, void* q, float* scales, int64_t scales_stride, hipStream_t s);
+// Weights [planes][n][k] into q and scales [planes][n / 128][k / 128].
+hipError_t launch_fp8_weights(int type, const void* w, int64_t planes, int64_t n, int64_t k, void* q, float* scales,
+                              hipStream_t s);
+// expert_plan.hip
+hipError_t launch_expert_plan(const int* ids, int64_t planes, int topk, int experts, int* starts, int* sorted,
+                              int* tokens, int* flags, hipStream_t s);
+// fp8_few.hip: x of any type; y_type F32, F16 or BF16.
+hipError_t launch_fp8_few(int x_type, int y_type, const Fp8Call& c, hipStream_t s);
+
+#if defined(__HIP_DEVICE_COMPILE__) || defined(__HIPCC__)
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef int fp8_v4i __attribute__((ext_vector_type(4)));
+typedef float fp8_f4 __attribute__((ext_vector_type(4)));
+typedef float fp8_f16v __attribute__((ext_vector_type(16)));
+typedef _Float16 fp8_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 fp8_h8 __attribute__((ext_vector_type(8)));
+
+// ------------------------------------------------------- a block's scale --
+// 2^e with the least e >= -126 for which a block's largest finite size is at
+// most 448 * 2^e (448: the largest e4m3 number, 1.75 * 2^8), 1 for zeros.  The
+// biased e is the size's own exponent less 8, and one more where its fraction
+// passes .75.  The division by it is exact, so each value goes to the e4m3
+// number that is nearest to it, whatever the arithmetic.
+__device__ __forceinline__ uint32_t fp8_size(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
+    return u < 0x7f800000u ? u : 0u;  // what is no number, or infinite, has no say
+}
+__device__ __forceinline__ int fp8_exponent(uint32_t size) {
+    return size ? max((int)((size + 0x1fffffu) >> 23) - 8, 1) : 127;
+}
+__device__ __forceinline__ float fp8_scale(int biased) { return __builtin_bit_cast(float, biased << 23); }
+__device__ __forceinline__ float fp8_inverse(int biased) { return __builtin_bit_cast(float, (254 - biased) << 23); }
+
+// Largest of the 16 lanes of a row, in all of them.
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+    v = max(v, (uint32_t)dppi<DPP_XOR1>((int)v));
+    v = max(v, (uint32_t)dppi<DPP_XOR2>((int)v));
+    v = max(v, (uint32_t)dppi<DPP_HALF_MIRROR>((int)v));
+    return max(v, (uint32_t)dppi<DPP_ROW_MIRROR>((int)v));
+}
+
+// Four values, scaled, to four e4m3 numbers (nearest, ties to even; NaN and
+// infinities to NaN: the values themselves never pass 448).
+__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d) {
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+
+// Eight e4m3 numbers as halves (exact: they are in 2^-9 .. 448).
+__device__ __forceinline__ fp8_h8 fp8_halves(uint32_t lo, uint32_t hi) {
+    const fp8_h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+    const fp8_h2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+    const fp8_h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+    const fp8_h2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+    return fp8_h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// ---------------------------------------------------------------- types --
+template <int TYPE>
+struct Fp8Size {
+    static constexpr int V = TYPE == T_F32 ? 4 : TYPE == T_E4M3 ? 1 : 2;
+};
+
+// Eight values from element i (16-byte aligned) as f32.
+template <int TYPE>
+__device__ __forceinline__ void fp8_load8(const void* p, int64_t i, float (&v)[8]) {
+    if constexpr (TYPE == T_F32) {
+        const float4 a = *(const float4*)((const float*)p + i), b = *(const float4*)((const float*)p + i + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        const uint4 a = *(const uint4*)((const uint16_t*)p + i);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if constexpr (TYPE == T_F16) {
+                v[2 * j] = f16_to_f32(w[j] & 0xffffu);
+                v[2 * j + 1] = f16_to_f32(w[j] >> 16);
+            } else {
+                v[2 * j] = __builtin_bit_cast(float, w[j] << 16);
+                v[2 * j + 1] = __builtin_bit_cast(float, w[j] & 0xffff0000u);
+            }
+        }
+    }
+}
+
+// f32 rounded to y's type (nearest even), its bits.
+template <int TYPE>
+__device__ __forceinline__ uint16_t fp8_half_bits(float v) {
+    if constexpr (TYPE == T_F16) return f32_to_f16(v);
+    return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+// Four neighbours of a row, `count` of which are there; `wide`: the place is
+// aligned for one store of all four.
+template <int TYPE>
+__device__ __forceinline__ void fp8_store4(void* y, int64_t i, const float (&v)[4], int count, bool wide) {
+    if constexpr (TYPE == T_F32) {
+        float* p = (float*)y + i;
+        if (wide && count >= 4) {
+            *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (j < count) p[j] = v[j];
+        }
+    } else {
+        uint16_t* p = (uint16_t*)y + i;
+        uint16_t b[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) b[j] = fp8_half_bits<TYPE>(v[j]);
+        if (wide && count >= 4) {
+            *(uint2*)p = make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (j < count) p[j] = b[j];
+        }
+    }
+}
+
+// ---------------------------------------------------------- tiles of rows --
+// Tile t of a call whose groups are cut into tiles of up to 2^SHIFT rows, in
+// the groups' order, then the rows past the last group (`zero`: no group owns
+// them, y is 0 there).  Every wave looks for itself, 64 groups at a time: a
+// lane has a group, a scan its first tile.  Where starts do not begin with 0,
+// fall, or pass m, no row has a group (and flags[0] is set).
+struct Fp8Tile {
+    int group, first, count;
+    bool zero;
+};
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive
+    const int lane = __lane_id();
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+template <int SHIFT>
+__device__ __forceinline__ Fp8Tile fp8_tile(const Fp8Call& c, int t) {
+    constexpr int ROWS = 1 << SHIFT;
+    if (!c.starts) return {0, t << SHIFT, min(ROWS, c.m - (t << SHIFT)), false};
+    const int lane = __lane_id(), E = c.experts;
+    Fp8Tile r = {0, 0, 0, true};
+    int before = 0;
+    bool bad = c.starts[0] != 0;
+    for (int base = 0; base <= E; base += 64) {
+        const int e = base + lane;
+        const int at = e <= E ? c.starts[e] : 0, next = e < E ? c.starts[e + 1] : c.m;
+        const int count = e <= E ? next - at : 0;
+        bad |= at < 0 || at > c.m || count < 0;
+        const int tiles = (int)(((uint32_t)count + ROWS - 1) >> SHIFT);
+        const int upto = before + wave_scan(tiles);
+        const uint64_t hit = __ballot(t < upto && t >= upto - tiles);
+        if (hit) {
+            const int j = __builtin_ctzll(hit);
+            const int in = (t - (__shfl(upto, j, 64) - __shfl(tiles, j, 64))) << SHIFT;
+            r = {base + j, __shfl(at, j, 64) + in, min(ROWS, __shfl(count, j, 64) - in), base + j == E};
+        }
+        before = __shfl(upto, 63, 64);
+    }
+    if (__ballot(bad)) {
+        r = {0, t << SHIFT, min(ROWS, c.m - (t << SHIFT)), true};
+        if (t == 0) c.flags[0] = 1;
+    }
+    return r;
+}
+// Tiles there can be: one that is not full a group, and one of no group.
+inline int64_t fp8_tiles(const Fp8Call& c, int rows) {
+    if (!c.starts) return ((int64_t)c.m + rows - 1) / rows;
+    return c.m / rows + (c.experts < c.m ? c.experts : c.m) + 1;
+}
+// Row i's row of x and of y, -1 where there is none (flags[0] is set).
+__device__ __forceinline__ int fp8_x_row(const Fp8Call& c, int i) {
+    if (!c.gather) return i;
+    const int r = c.gather[i];
+    if ((uint32_t)r < (uint32_t)c.x_rows) return r;
+    c.flags[0] = 1;
+    return -1;
+}
+__device__ __forceinline__ int fp8_y_row(const Fp8Call& c, int i) {
+    if (!c.scatter) return i;
+    const int r = c.scatter[i];
+    if ((uint32_t)r < (uint32_t)c.y_rows) return r;
+    c.flags[0] = 1;
+    return -1;
+}
+
+#endif
+
+}  // namespace lloom

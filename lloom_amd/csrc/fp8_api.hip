@@ -1,0 +1,196 @@
+// fp8_api.hip -- the C ABI of the 8-bit floating-point products
+// (include/lloom_hip.h): argument checks, routes and launches.
+#include <hip/hip_runtime.h>
+
+#include <mutex>
+
+#include "api_internal.hpp"
+#include "fp8.hpp"
+
+using namespace lloom;
+
+namespace {
+
+constexpr int64_t MAX_ROWS = 1 << 24, MAX_N = 1 << 24, MAX_K = 1 << 22;
+
+bool is_act(int t) { return t == T_F32 || t == T_F16 || t == T_BF16; }
+int64_t type_bytes(int t) { return t == T_F32 ? 4 : t == T_E4M3 ? 1 : 2; }
+
+int check_act(const char* what, int type) {
+    if (is_act(type)) return LLOOM_HIP_OK;
+    return fail(LLOOM_HIP_EDTYPE, "%s: activation dtype %d must be F32, F16 or BF16", what, type);
+}
+
+int check_k(const char* what, int64_t k) {
+    if (k < 1) return fail(LLOOM_HIP_EINVAL, "%s: k %lld", what, (long long)k);
+    if (k % 16 || k > MAX_K)
+        return fail(LLOOM_HIP_ESHAPE, "%s: k %lld is no multiple of 16 up to %lld", what, (long long)k, (long long)MAX_K);
+    return LLOOM_HIP_OK;
+}
+
+// Rows of x: `stride` elements apart, 16-byte aligned.
+int check_rows(const char* what, int type, const void* x, int64_t stride, int64_t rows, int64_t k) {
+    if (rows < 0 || rows > MAX_ROWS)
+        return fail(rows < 0 ? LLOOM_HIP_EINVAL : LLOOM_HIP_ESHAPE, "%s: %lld rows (at most %lld)", what, (long long)rows,
+                    (long long)MAX_ROWS);
+    if (stride < k)
+        return fail(LLOOM_HIP_ESHAPE, "%s: rows of %lld, %lld apart, overlap", what, (long long)k, (long long)stride);
+    if ((uintptr_t)x % 16 || stride * type_bytes(type) % 16)
+        return fail(LLOOM_HIP_EINVAL, "%s: rows must be 16-byte aligned", what);
+    return LLOOM_HIP_OK;
+}
+
+int check_product(const char* what, const void* w, const float* ws, int64_t experts, int64_t n, int64_t k, const void* x,
+                  int x_type, int64_t x_stride, const float* xs, int64_t xs_row, int64_t xs_block, int64_t x_rows,
+                  const void* y, int y_type) {
+    if (!w || !ws || (x_rows && !x)) return fail(LLOOM_HIP_EINVAL, "%s: null argument", what);
+    if (x_type != T_E4M3)
+        if (int rc = check_act(what, x_type)) return rc;
+    if (int rc = check_act(what, y_type)) return rc;
+    if (int rc = check_k(what, k)) return rc;
+    if (n < 1) return fail(LLOOM_HIP_EINVAL, "%s: n %lld", what, (long long)n);
+    if (n > MAX_N) return fail(LLOOM_HIP_ESHAPE, "%s: n %lld is over %lld", what, (long long)n, (long long)MAX_N);
+    if (experts < 1) return fail(LLOOM_HIP_EINVAL, "%s: %lld experts", what, (long long)experts);
+    if (experts > MOE_MAX_EXPERTS)
+        return fail(LLOOM_HIP_ESHAPE, "%s: %lld experts, at most %d", what, (long long)experts, MOE_MAX_EXPERTS);
+    if (int rc = check_rows(what, x_type, x, x_stride, x_rows, k)) return rc;
+    if (x_type == T_E4M3) {
+        if (x_rows && !xs) return fail(LLOOM_HIP_EINVAL, "%s: E4M3 rows without scales", what);
+        if (xs_row < 0 || xs_block < 0)
+            return fail(LLOOM_HIP_EINVAL, "%s: scales %lld and %lld apart", what, (long long)xs_row, (long long)xs_block);
+        if ((uintptr_t)xs % 4) return fail(LLOOM_HIP_EINVAL, "%s: scales must be 4-byte aligned", what);
+    }
+    if ((uintptr_t)w % 16 || (uintptr_t)ws % 4 || (uintptr_t)y % 16)
+        return fail(LLOOM_HIP_EINVAL, "%s: the weight and y must be 16-byte, the scales 4-byte aligned", what);
+    return LLOOM_HIP_OK;
+}
+
+// A grid's workgroups, as a launch of 512 threads counts them.
+int check_grid(const char* what, int64_t rows, int64_t n, int64_t experts) {
+    const int64_t tiles = rows / 16 + (experts < rows ? experts : rows) + 1;
+    if (tiles * ((n + 15) / 16) < ((int64_t)1 << 23)) return LLOOM_HIP_OK;
+    return fail(LLOOM_HIP_ESHAPE, "%s: %lld rows by n %lld", what, (long long)rows, (long long)n);
+}
+
+int run_product(lloom_hip_ctx* ctx, int x_type, int y_type, const Fp8Call& c, hipStream_t s) {
+    HIP_OK(launch_fp8_few(x_type, y_type, c, s));
+    return LLOOM_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int lloom_hip_fp8_quantize(lloom_hip_ctx* ctx, const void* x_dev, int x_dtype, int64_t x_stride, int64_t rows, int64_t k,
+                           void* q_dev, float* scales_dev, int64_t scales_stride, void* stream) {
+    if (!ctx || (rows && (!x_dev || !q_dev || !scales_dev))) return fail(LLOOM_HIP_EINVAL, "fp8_quantize: null argument");
+    if (int rc = check_act("fp8_quantize", x_dtype)) return rc;
+    if (int rc = check_k("fp8_quantize", k)) return rc;
+    if (int rc = check_rows("fp8_quantize", x_dtype, x_dev, x_stride, rows, k)) return rc;
+    if (scales_stride < rows)
+        return fail(LLOOM_HIP_ESHAPE, "fp8_quantize: scales of %lld rows, %lld apart, overlap", (long long)rows,
+                    (long long)scales_stride);
+    if ((uintptr_t)q_dev % 8 || (uintptr_t)scales_dev % 4)
+        return fail(LLOOM_HIP_EINVAL, "fp8_quantize: q must be 8-byte, scales 4-byte aligned");
+    if (rows == 0) return LLOOM_HIP_OK;
+    HIP_OK(hipSetDevice(ctx->device));
+    HIP_OK(launch_fp8_rows(x_dtype, x_dev, x_stride, nullptr, 0, rows, k, q_dev, scales_dev, scales_stride,
+                           (hipStream_t)stream));
+    return LLOOM_HIP_OK;
+}
+
+int lloom_hip_fp8_silu_mul(lloom_hip_ctx* ctx, const void* gate_dev, int64_t gate_stride, const void* up_dev,
+                           int64_t up_stride, int dtype, int64_t rows, int64_t k, void* q_dev, float* scales_dev,
+                           int64_t scales_stride, void* stream) {
+    if (!ctx || (rows && (!gate_dev || !up_dev || !q_dev || !scales_dev)))
+        return fail(LLOOM_HIP_EINVAL, "fp8_silu_mul: null argument");
+    if (int rc = check_act("fp8_silu_mul", dtype)) return rc;
+    if (int rc = check_k("fp8_silu_mul", k)) return rc;
+    if (int rc = check_rows("fp8_silu_mul", dtype, gate_dev, gate_stride, rows, k)) return rc;
+    if (int rc = check_rows("fp8_silu_mul", dtype, up_dev, up_stride, rows, k)) return rc;
+    if (scales_stride < rows)
+        return fail(LLOOM_HIP_ESHAPE, "fp8_silu_mul: scales of %lld rows, %lld apart, overlap", (long long)rows,
+                    (long long)scales_stride);
+    if ((uintptr_t)q_dev % 8 || (uintptr_t)scales_dev % 4)
+        return fail(LLOOM_HIP_EINVAL, "fp8_silu_mul: q must be 8-byte, scales 4-byte aligned");
+    if (rows == 0) return LLOOM_HIP_OK;
+    HIP_OK(hipSetDevice(ctx->device));
+    HIP_OK(launch_fp8_rows(dtype, gate_dev, gate_stride, up_dev, up_stride, rows, k, q_dev, scales_dev, scales_stride,
+                           (hipStream_t)stream));
+    return LLOOM_HIP_OK;
+}
+
+int lloom_hip_fp8_quantize_weight(lloom_hip_ctx* ctx, const void* w_dev, int w_dtype, int64_t experts, int64_t n,
+                                  int64_t k, void* q_dev, float* scales_dev, void* stream) {
+    if (!ctx || !w_dev || !q_dev || !scales_dev) return fail(LLOOM_HIP_EINVAL, "fp8_quantize_weight: null argument");
+    if (int rc = check_act("fp8_quantize_weight", w_dtype)) return rc;
+    if (int rc = check_k("fp8_quantize_weight", k)) return rc;
+    if (experts < 1 || n < 1)
+        return fail(LLOOM_HIP_EINVAL, "fp8_quantize_weight: %lld weights of %lld rows", (long long)experts, (long long)n);
+    if (n > MAX_N || experts > MOE_MAX_EXPERTS || experts * ((n + 127) / 128) * ((k + 127) / 128) >= (1 << 24))
+        return fail(LLOOM_HIP_ESHAPE, "fp8_quantize_weight: %lld weights of [%lld, %lld]", (long long)experts, (long long)n,
+                    (long long)k);
+    if ((uintptr_t)w_dev % 16 || (uintptr_t)q_dev % 8 || (uintptr_t)scales_dev % 4)
+        return fail(LLOOM_HIP_EINVAL, "fp8_quantize_weight: the weight must be 16-byte, q 8-byte, scales 4-byte aligned");
+    HIP_OK(hipSetDevice(ctx->device));
+    HIP_OK(launch_fp8_weights(w_dtype, w_dev, experts, n, k, q_dev, scales_dev, (hipStream_t)stream));
+    return LLOOM_HIP_OK;
+}
+
+int lloom_hip_fp8_matmul(lloom_hip_ctx* ctx, const void* w_dev, const float* w_scales_dev, int64_t n, int64_t k,
+                         const void* x_dev, int x_dtype, int64_t x_stride, const float* x_scales_dev, int64_t xs_row,
+                         int64_t xs_block, int64_t m, void* y_dev, int y_dtype, void* stream) {
+    if (!ctx || (m && !y_dev)) return fail(LLOOM_HIP_EINVAL, "fp8_matmul: null argument");
+    if (int rc = check_product("fp8_matmul", w_dev, w_scales_dev, 1, n, k, x_dev, x_dtype, x_stride, x_scales_dev, xs_row,
+                               xs_block, m, y_dev, y_dtype))
+        return rc;
+    if (int rc = check_grid("fp8_matmul", m, n, 1)) return rc;
+    if (m == 0) return LLOOM_HIP_OK;
+    HIP_OK(hipSetDevice(ctx->device));
+    const Fp8Call c = {(const uint8_t*)w_dev, w_scales_dev, x_dev, x_scales_dev, y_dev, nullptr, nullptr, nullptr,
+                       ctx->flags, x_stride, xs_row, xs_block, (int)n, (int)k, (int)((k + 127) / 128),
+                       (int)((n + 127) / 128), (int)m, (int)m, (int)m, 1};
+    return run_product(ctx, x_dtype, y_dtype, c, (hipStream_t)stream);
+}
+
+int lloom_hip_fp8_grouped_matmul(lloom_hip_ctx* ctx, const void* w_dev, const float* w_scales_dev, int64_t experts,
+                                 int64_t n, int64_t k, const void* x_dev, int x_dtype, int64_t x_stride,
+                                 const float* x_scales_dev, int64_t xs_row, int64_t xs_block, int64_t x_rows,
+                                 const uint32_t* starts_dev, const uint32_t* gather_dev, const uint32_t* scatter_dev,
+                                 int64_t rows, void* y_dev, int y_dtype, int64_t y_rows, void* stream) {
+    if (!ctx || !starts_dev || (rows && !y_dev)) return fail(LLOOM_HIP_EINVAL, "fp8_grouped_matmul: null argument");
+    if (int rc = check_product("fp8_grouped_matmul", w_dev, w_scales_dev, experts, n, k, x_dev, x_dtype, x_stride,
+                               x_scales_dev, xs_row, xs_block, x_rows, y_dev, y_dtype))
+        return rc;
+    if (rows < 0 || y_rows < 0)
+        return fail(LLOOM_HIP_EINVAL, "fp8_grouped_matmul: %lld rows into %lld", (long long)rows, (long long)y_rows);
+    if (rows > MAX_ROWS || y_rows > MAX_ROWS || (!gather_dev && x_rows < rows) || (!scatter_dev && y_rows < rows))
+        return fail(LLOOM_HIP_ESHAPE, "fp8_grouped_matmul: %lld rows (at most %lld) of %lld into %lld", (long long)rows,
+                    (long long)MAX_ROWS, (long long)x_rows, (long long)y_rows);
+    if (int rc = check_grid("fp8_grouped_matmul", rows, n, experts)) return rc;
+    if (rows == 0) return LLOOM_HIP_OK;
+    HIP_OK(hipSetDevice(ctx->device));
+    const Fp8Call c = {(const uint8_t*)w_dev, w_scales_dev, x_dev, x_scales_dev, y_dev, (const int*)starts_dev,
+                       (const int*)gather_dev, (const int*)scatter_dev, ctx->flags, x_stride, xs_row, xs_block, (int)n,
+                       (int)k, (int)((k + 127) / 128), (int)((n + 127) / 128), (int)rows, (int)x_rows, (int)y_rows,
+                       (int)experts};
+    return run_product(ctx, x_dtype, y_dtype, c, (hipStream_t)stream);
+}
+
+int lloom_hip_expert_plan(lloom_hip_ctx* ctx, const uint32_t* ids_dev, int64_t tokens, int64_t topk, int64_t experts,
+                          void* starts_dev, void* planes_dev, void* tokens_dev, void* stream) {
+    if (!ctx || !starts_dev || (tokens && (!ids_dev || !planes_dev || !tokens_dev)))
+        return fail(LLOOM_HIP_EINVAL, "expert_plan: null argument");
+    if (tokens < 0 || topk < 1 || experts < 1)
+        return fail(LLOOM_HIP_EINVAL, "expert_plan: %lld tokens of %lld, %lld experts", (long long)tokens, (long long)topk,
+                    (long long)experts);
+    if (topk > MOE_MAX_EXPERTS || experts > MOE_MAX_EXPERTS || tokens > MAX_ROWS || tokens * topk >= MAX_ROWS)
+        return fail(LLOOM_HIP_ESHAPE, "expert_plan: %lld tokens of %lld (under %lld planes), %lld experts (at most %d)",
+                    (long long)tokens, (long long)topk, (long long)MAX_ROWS, (long long)experts, MOE_MAX_EXPERTS);
+    HIP_OK(hipSetDevice(ctx->device));
+    HIP_OK(launch_expert_plan((const int*)ids_dev, tokens * topk, (int)topk, (int)experts, (int*)starts_dev,
+                              (int*)planes_dev, (int*)tokens_dev, ctx->flags, (hipStream_t)stream));
+    return LLOOM_HIP_OK;
+}
+
+}  // extern "C"

@@ -79,6 +79,13 @@ def lib():
                                                vp, vp, i64, ctypes.c_float, i64, i64, i64, vp, vp], i32),
                 "lloom_hip_paged_attention_workspace_bytes": ([i64, i64, i64, i64, i64, i64,
                                                                ctypes.POINTER(sz)], i32),
+                "lloom_hip_fp8_quantize": ([vp, vp, i32, i64, i64, i64, vp, vp, i64, vp], i32),
+                "lloom_hip_fp8_silu_mul": ([vp, vp, i64, vp, i64, i32, i64, i64, vp, vp, i64, vp], i32),
+                "lloom_hip_fp8_quantize_weight": ([vp, vp, i32, i64, i64, i64, vp, vp, vp], i32),
+                "lloom_hip_fp8_matmul": ([vp, vp, vp, i64, i64, vp, i32, i64, vp, i64, i64, i64, vp, i32, vp], i32),
+                "lloom_hip_expert_plan": ([vp, vp, i64, i64, i64, vp, vp, vp, vp], i32),
+                "lloom_hip_fp8_grouped_matmul": ([vp, vp, vp, i64, i64, i64, vp, i32, i64, vp, i64, i64, i64, vp, vp, vp,
+                                                  i64, vp, i32, i64, vp], i32),
                 "lloom_hip_synth_normal": ([ctypes.c_uint64, ctypes.c_float, ctypes.c_float, vp, i64], i32),
                 "lloom_hip_synth_uniform": ([ctypes.c_uint64, ctypes.c_float, ctypes.c_float, vp, i64], i32),
             }

@@ -41,6 +41,8 @@ pub const LLOOM_HIP_Q8_0: c_int = 8;
 pub const LLOOM_HIP_Q4K: c_int = 12;
 pub const LLOOM_HIP_Q6K: c_int = 14;
 pub const LLOOM_HIP_Q8K: c_int = 15;
+pub const LLOOM_HIP_BF16: c_int = 30;
+pub const LLOOM_HIP_E4M3: c_int = 100;
 
 // Prefill operand mode (lloom_hip_ctx_set_prefill_mma).
 pub const LLOOM_HIP_MMA_F16: c_int = 0;
@@ -339,6 +341,96 @@ extern "C" {
         head_dim: i64,
         max_new: i64,
         bytes: *mut usize,
+    ) -> c_int;
+
+    // Products with 8-bit floating-point weights, dense and grouped by expert.
+    pub fn lloom_hip_fp8_quantize(
+        ctx: *mut lloom_hip_ctx,
+        x_dev: *const c_void,
+        x_dtype: c_int,
+        x_stride: i64,
+        rows: i64,
+        k: i64,
+        q_dev: *mut c_void,
+        scales_dev: *mut f32,
+        scales_stride: i64,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn lloom_hip_fp8_silu_mul(
+        ctx: *mut lloom_hip_ctx,
+        gate_dev: *const c_void,
+        gate_stride: i64,
+        up_dev: *const c_void,
+        up_stride: i64,
+        dtype: c_int,
+        rows: i64,
+        k: i64,
+        q_dev: *mut c_void,
+        scales_dev: *mut f32,
+        scales_stride: i64,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn lloom_hip_fp8_quantize_weight(
+        ctx: *mut lloom_hip_ctx,
+        w_dev: *const c_void,
+        w_dtype: c_int,
+        experts: i64,
+        n: i64,
+        k: i64,
+        q_dev: *mut c_void,
+        scales_dev: *mut f32,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn lloom_hip_fp8_matmul(
+        ctx: *mut lloom_hip_ctx,
+        w_dev: *const c_void,
+        w_scales_dev: *const f32,
+        n: i64,
+        k: i64,
+        x_dev: *const c_void,
+        x_dtype: c_int,
+        x_stride: i64,
+        x_scales_dev: *const f32,
+        xs_row: i64,
+        xs_block: i64,
+        m: i64,
+        y_dev: *mut c_void,
+        y_dtype: c_int,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn lloom_hip_expert_plan(
+        ctx: *mut lloom_hip_ctx,
+        ids_dev: *const u32,
+        tokens: i64,
+        topk: i64,
+        experts: i64,
+        starts_dev: *mut c_void,
+        planes_dev: *mut c_void,
+        tokens_dev: *mut c_void,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn lloom_hip_fp8_grouped_matmul(
+        ctx: *mut lloom_hip_ctx,
+        w_dev: *const c_void,
+        w_scales_dev: *const f32,
+        experts: i64,
+        n: i64,
+        k: i64,
+        x_dev: *const c_void,
+        x_dtype: c_int,
+        x_stride: i64,
+        x_scales_dev: *const f32,
+        xs_row: i64,
+        xs_block: i64,
+        x_rows: i64,
+        starts_dev: *const u32,
+        gather_dev: *const u32,
+        scatter_dev: *const u32,
+        rows: i64,
+        y_dev: *mut c_void,
+        y_dtype: c_int,
+        y_rows: i64,
+        stream: *mut c_void,
     ) -> c_int;
 
     // Host-side synthetic inputs (StdRng-seeded normal / uniform), for benches.
