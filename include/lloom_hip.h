@@ -395,6 +395,11 @@ int lloom_hip_fp8_grouped_matmul(lloom_hip_ctx* ctx, const void* w_dev, const fl
                                  const uint32_t* starts_dev, const uint32_t* gather_dev, const uint32_t* scatter_dev,
                                  int64_t rows, void* y_dev, int y_dtype, int64_t y_rows, void* stream);
 
+/* Workspace of a product with `rows` rows (dense: experts = 1) of x's x_rows, to
+ * reserve before a capture: where there are many rows, x of another type than
+ * E4M3 is brought into 8 bits there, in a launch of its own. */
+int lloom_hip_fp8_workspace_bytes(int x_dtype, int64_t rows, int64_t x_rows, int64_t experts, int64_t k, size_t* bytes);
+
 /* ------------------------------------------------------- synthetic data --
  * The benchmark/test input generator (not part of the reference): SplitMix64
  * seeding xoshiro256**, Box-Muller normals N(mean, std) written as f32 into a

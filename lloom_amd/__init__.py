@@ -37,4 +37,5 @@ from .fp8 import (  # noqa: F401
     fp8_quantize,
     fp8_quantize_weight,
     fp8_silu_mul,
+    fp8_workspace_bytes,
 )

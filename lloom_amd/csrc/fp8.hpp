@@ -44,8 +44,13 @@ hipError_t launch_fp8_weights(int type, const void* w, int64_t planes, int64_t n
 // expert_plan.hip
 hipError_t launch_expert_plan(const int* ids, int64_t planes, int topk, int experts, int* starts, int* sorted,
                               int* tokens, int* flags, hipStream_t s);
+// Whether a call's groups have so few rows that fp8_few.hip serves them.
+inline bool fp8_few_rows(int64_t rows, int64_t experts) { return rows <= 16 * experts; }
 // fp8_few.hip: x of any type; y_type F32, F16 or BF16.
 hipError_t launch_fp8_few(int x_type, int y_type, const Fp8Call& c, hipStream_t s);
+// fp8_tile.hip: x E4M3.  Whether its 32-bit offsets hold the operands.
+bool fp8_tile_fits(const Fp8Call& c);
+hipError_t launch_fp8_tile(int y_type, const Fp8Call& c, hipStream_t s);
 
 #if defined(__HIP_DEVICE_COMPILE__) || defined(__HIPCC__)
 

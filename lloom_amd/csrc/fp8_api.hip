@@ -72,8 +72,31 @@ int check_grid(const char* what, int64_t rows, int64_t n, int64_t experts) {
     return fail(LLOOM_HIP_ESHAPE, "%s: %lld rows by n %lld", what, (long long)rows, (long long)n);
 }
 
-int run_product(lloom_hip_ctx* ctx, int x_type, int y_type, const Fp8Call& c, hipStream_t s) {
-    HIP_OK(launch_fp8_few(x_type, y_type, c, s));
+// x in 8 bits, where a call brings it there in a launch before the product's:
+// q [rows][k], then the scales, block by block.
+struct XCopy {
+    bool needed;
+    size_t scales_at, bytes;
+};
+XCopy x_copy(int x_type, int64_t rows, int64_t x_rows, int64_t experts, int64_t k) {
+    const size_t q = ((size_t)x_rows * k + 255) & ~(size_t)255;
+    return {x_type != T_E4M3 && !fp8_few_rows(rows, experts), q, q + (size_t)x_rows * ((k + 127) / 128) * sizeof(float)};
+}
+
+int run_product(lloom_hip_ctx* ctx, int x_type, int y_type, Fp8Call c, hipStream_t s) {
+    const XCopy copy = x_copy(x_type, c.m, c.x_rows, c.experts, c.k);
+    std::unique_lock<std::mutex> lock(ctx->mu, std::defer_lock);
+    if (copy.needed && c.x_rows) {
+        lock.lock();
+        void* ws = nullptr;
+        if (int rc = ensure_ws(ctx, copy.bytes, s, &ws)) return rc;
+        float* scales = (float*)((uint8_t*)ws + copy.scales_at);
+        HIP_OK(launch_fp8_rows(x_type, c.x, c.x_stride, nullptr, 0, c.x_rows, c.k, ws, scales, c.x_rows, s));
+        c.x = ws, c.x_stride = c.k, c.xs = scales, c.xs_row = 1, c.xs_block = c.x_rows;
+        x_type = T_E4M3;
+    }
+    if (x_type == T_E4M3 && !fp8_few_rows(c.m, c.experts) && fp8_tile_fits(c)) HIP_OK(launch_fp8_tile(y_type, c, s));
+    else HIP_OK(launch_fp8_few(x_type, y_type, c, s));
     return LLOOM_HIP_OK;
 }
 
@@ -190,6 +213,22 @@ int lloom_hip_expert_plan(lloom_hip_ctx* ctx, const uint32_t* ids_dev, int64_t t
     HIP_OK(hipSetDevice(ctx->device));
     HIP_OK(launch_expert_plan((const int*)ids_dev, tokens * topk, (int)topk, (int)experts, (int*)starts_dev,
                               (int*)planes_dev, (int*)tokens_dev, ctx->flags, (hipStream_t)stream));
+    return LLOOM_HIP_OK;
+}
+
+int lloom_hip_fp8_workspace_bytes(int x_dtype, int64_t rows, int64_t x_rows, int64_t experts, int64_t k, size_t* bytes) {
+    if (!bytes) return fail(LLOOM_HIP_EINVAL, "fp8_workspace_bytes: null argument");
+    if (x_dtype != T_E4M3)
+        if (int rc = check_act("fp8_workspace_bytes", x_dtype)) return rc;
+    if (int rc = check_k("fp8_workspace_bytes", k)) return rc;
+    if (rows < 0 || x_rows < 0 || experts < 1)
+        return fail(LLOOM_HIP_EINVAL, "fp8_workspace_bytes: %lld rows of %lld, %lld experts", (long long)rows,
+                    (long long)x_rows, (long long)experts);
+    if (rows > MAX_ROWS || x_rows > MAX_ROWS || experts > MOE_MAX_EXPERTS)
+        return fail(LLOOM_HIP_ESHAPE, "fp8_workspace_bytes: %lld rows of %lld (at most %lld), %lld experts (at most %d)",
+                    (long long)rows, (long long)x_rows, (long long)MAX_ROWS, (long long)experts, MOE_MAX_EXPERTS);
+    const XCopy copy = x_copy(x_dtype, rows, x_rows, experts, k);
+    *bytes = copy.needed ? copy.bytes : 0;
     return LLOOM_HIP_OK;
 }
 

@@ -1,0 +1,288 @@
+// fp8_tile.hip -- products with e4m3 weights for many rows of x: tiles through
+// LDS.  Built with the MFMA results in VGPRs (-amdgpu-mfma-vgpr-form): a block's
+// sum is read by the VALU right away.
+#include "fp8.hpp"
+#include "kq_gemm.hpp"
+
+namespace lloom {
+
+#pragma clang fp contract(off)
+
+// A workgroup has BM rows of x and BN of the weight, WM x WN waves with MF x NF
+// tiles of 32 x 32 each; k moves a block (128) a step through S LDS stages,
+//   W [BN][128] e4m3, piece p (16 bytes) of row r at p ^ swizzle(r)
+//   X [BM][128] likewise
+//   scales [BM] f32 of the block's rows
+// every byte by buffer_load .. lds: what is out of the operands (rows past a
+// tile's, a last block's bytes past k) has an offset out of the buffer's range
+// and arrives as zeros.  Lane (h, c) of a wave takes pieces 2 i + h, i < 4, of row
+// c of both operands: which bytes meet in which instruction does not matter.
+// The weight is the matrix instructions' A: a lane's 16 sums are of one row of x,
+// so one factor (its scale times the weight block's) serves them all.
+template <int WM_, int WN_, int MF_, int NF_, int S_>
+struct Fp8Cfg {
+    static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_, S = S_;
+    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+    static constexpr int BM = 32 * WM * MF, BN = 32 * WN * NF;
+    static constexpr int SHIFT = BM == 32 ? 5 : BM == 64 ? 6 : BM == 128 ? 7 : 8;
+    static constexpr int W = BN * 128, X = BM * 128, XS = BM * 4 < 256 ? 256 : BM * 4, STAGE = W + X + XS;
+    static constexpr int W_LOADS = BN / 8 / WAVES, X_LOADS = BM / 8 / WAVES;
+    static constexpr int XS_LOADS = (BM / 64 + WAVES - 1) / WAVES < 1 ? 1 : (BM / 64 + WAVES - 1) / WAVES;
+    static constexpr int DMA = W_LOADS + X_LOADS + XS_LOADS;
+    static constexpr int PITCH = 32 * NF * 4 + 16;  // a row of a wave's part of y on its way out, f32 at most
+    static constexpr int OUT = WAVES * 32 * PITCH, RING = S * STAGE, LDS = RING > OUT ? RING : OUT;
+    static_assert(BM == 1 << SHIFT && W_LOADS * WAVES * 8 == BN && X_LOADS * WAVES * 8 == BM, "whole loads");
+    static_assert(128 % (32 * NF) == 0, "a wave's weight rows share their scales");
+    static_assert((S - 1) * DMA <= 63 && LDS <= 160 * 1024, "counts and LDS");
+};
+
+constexpr uint32_t FP8_OUT = 0x80000000u;  // an offset that no buffer holds
+
+__device__ __forceinline__ fp8_v4i fp8_buffer(const void* p) {
+    const uint64_t a = (uint64_t)p;
+    return fp8_v4i{(int)__builtin_amdgcn_readfirstlane((int)a),
+                   (int)__builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff), (int)FP8_OUT, 0x00020000};
+}
+__device__ __forceinline__ void fp8_dma16(fp8_v4i b, uint32_t voff, uint32_t soff, uint32_t lds) {
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(b), "s"(soff), "{m0}"(lds) : "memory");
+}
+__device__ __forceinline__ void fp8_dma4(fp8_v4i b, uint32_t voff, uint32_t soff, uint32_t lds) {
+    asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(voff), "s"(b), "s"(soff), "{m0}"(lds) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void fp8_wait() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ int fp8_swizzle(int row) { return row & 7; }
+
+// A lane's 64 bytes of a row of a stage.
+struct Fp8Row {
+    uint4 p[4];
+};
+__device__ __forceinline__ Fp8Row fp8_read(const uint8_t* rows, int row, int h) {
+    Fp8Row r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r.p[i] = *(const uint4*)(rows + row * 128 + 16 * ((2 * i + h) ^ fp8_swizzle(row)));
+    return r;
+}
+__device__ __forceinline__ v8i fp8_operand(const Fp8Row& r, int j) {
+    const uint4 a = r.p[2 * j], b = r.p[2 * j + 1];
+    return v8i{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+}
+
+template <class C, bool EXACT, int YT>
+__global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nbn) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c32 = lane & 31;
+    const int wv = __builtin_amdgcn_readfirstlane(wave), wm = wv / C::WN, wn = wv % C::WN;
+    int t, bn;
+    Fp8Tile tile;
+    if (c.starts) {
+        t = blockIdx.x / nbn, bn = blockIdx.x - t * nbn;
+        tile = fp8_tile<C::SHIFT>(c, t);
+        if (tile.count <= 0) return;
+    } else {
+        tile_of((c.m + C::BM - 1) / C::BM, nbn, t, bn);
+        tile = fp8_tile<C::SHIFT>(c, t);
+    }
+    const int n0 = bn * C::BN, steps = tile.zero ? 0 : c.kb;
+
+    // this wave's share of a stage: per-lane byte offsets, fixed for all steps
+    const uint8_t* wbase = c.w + ((int64_t)tile.group * c.n + n0) * c.k;
+    const fp8_v4i wbuf = fp8_buffer(wbase);
+    const int64_t x0 = c.gather ? 0 : tile.first;
+    const fp8_v4i xbuf = fp8_buffer((const uint8_t*)c.x + x0 * c.x_stride);
+    const fp8_v4i sbuf = fp8_buffer(c.xs + x0 * c.xs_row);
+    uint32_t woff[C::W_LOADS], xoff[C::X_LOADS], soff[C::XS_LOADS];
+    const int piece = (lane & 7) ^ fp8_swizzle(lane >> 3);  // the lane's, of every row that it loads
+#pragma unroll
+    for (int i = 0; i < C::W_LOADS; i++) {
+        const int row = 8 * (wv * C::W_LOADS + i) + (lane >> 3);
+        woff[i] = n0 + row < c.n ? (uint32_t)row * (uint32_t)c.k + 16u * piece : FP8_OUT;
+    }
+#pragma unroll
+    for (int i = 0; i < C::X_LOADS; i++) {
+        const int row = 8 * (wv * C::X_LOADS + i) + (lane >> 3);
+        const int from = row < tile.count && steps ? fp8_x_row(c, tile.first + row) : -1;
+        xoff[i] = from >= 0 ? (uint32_t)(from - (int)x0) * (uint32_t)c.x_stride + 16u * piece : FP8_OUT;
+    }
+#pragma unroll
+    for (int i = 0; i < C::XS_LOADS; i++) {
+        const int row = (64 * (wv + C::WAVES * i) + lane) % (C::BM < 64 ? 64 : C::BM);
+        const int from = row < tile.count && steps ? fp8_x_row(c, tile.first + row) : -1;
+        soff[i] = from >= 0 ? (uint32_t)(from - (int)x0) * (uint32_t)c.xs_row * 4u : FP8_OUT;
+    }
+    const uint32_t lds0 = lds_addr(smem);
+    auto issue = [&](int s, int slot) {
+        const uint32_t st = lds0 + slot * C::STAGE, at = 128u * s;
+        const bool cut = 128 * s + 16 * piece >= c.k;  // past the end of the rows
+#pragma unroll
+        for (int i = 0; i < C::W_LOADS; i++)
+            fp8_dma16(wbuf, cut ? FP8_OUT : woff[i], at, st + 1024 * (wv * C::W_LOADS + i));
+#pragma unroll
+        for (int i = 0; i < C::X_LOADS; i++)
+            fp8_dma16(xbuf, cut ? FP8_OUT : xoff[i], at, st + C::W + 1024 * (wv * C::X_LOADS + i));
+#pragma unroll
+        for (int i = 0; i < C::XS_LOADS; i++)
+            fp8_dma4(sbuf, soff[i], (uint32_t)s * (uint32_t)c.xs_block * 4u,
+                     st + C::W + C::X + 256 * ((wv + C::WAVES * i) % (C::BM < 64 ? 1 : C::BM / 64)));
+    };
+
+    fp8_f16v acc[C::NF][C::MF];
+#pragma unroll
+    for (int b = 0; b < C::NF; b++)
+#pragma unroll
+        for (int a = 0; a < C::MF; a++) acc[b][a] = fp8_f16v{};
+
+    const float* ws = c.ws + ((int64_t)tile.group * c.nb + min((n0 + wn * 32 * C::NF) >> 7, c.nb - 1)) * c.kb;
+    float wscale = 0.0f;  // lane l: of block 64 i + l
+    if (steps) {
+#pragma unroll
+        for (int i = 0; i < C::S - 1; i++) issue(min(i, steps - 1), i);
+        __builtin_amdgcn_sched_barrier(0);
+        fp8_wait<(C::S - 2) * C::DMA>();
+        __builtin_amdgcn_s_barrier();
+    }
+    for (int s = 0; s < steps; s++) {
+        if ((s & 63) == 0) wscale = ws[min(s + lane, c.kb - 1)];
+        issue(min(s + C::S - 1, steps - 1), (s + C::S - 1) % C::S);
+        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t* W = smem + (s % C::S) * C::STAGE;
+        const uint8_t* X = W + C::W;
+        const float* XS = (const float*)(X + C::X);
+        const float sw = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wscale), s & 63));
+        float f[C::MF];
+        Fp8Row x[C::MF];
+#pragma unroll
+        for (int a = 0; a < C::MF; a++) {
+            const int row = (wm * C::MF + a) * 32 + c32;
+            f[a] = XS[row] * sw;
+            x[a] = fp8_read(X, row, h);
+        }
+        if constexpr (EXACT) {
+            fp8_h8 xh[C::MF][8];
+#pragma unroll
+            for (int a = 0; a < C::MF; a++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    xh[a][2 * i] = fp8_halves(x[a].p[i].x, x[a].p[i].y);
+                    xh[a][2 * i + 1] = fp8_halves(x[a].p[i].z, x[a].p[i].w);
+                }
+#pragma unroll
+            for (int b = 0; b < C::NF; b++) {
+                const Fp8Row w = fp8_read(W, (wn * C::NF + b) * 32 + c32, h);
+                fp8_f16v d[C::MF];
+#pragma unroll
+                for (int a = 0; a < C::MF; a++) d[a] = fp8_f16v{};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const fp8_h8 w0 = fp8_halves(w.p[i].x, w.p[i].y), w1 = fp8_halves(w.p[i].z, w.p[i].w);
+#pragma unroll
+                    for (int a = 0; a < C::MF; a++) {
+                        d[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w0, xh[a][2 * i], d[a], 0, 0, 0);
+                        d[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w1, xh[a][2 * i + 1], d[a], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int a = 0; a < C::MF; a++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[b][a][r] = __builtin_fmaf(d[a][r], f[a], acc[b][a][r]);
+            }
+        } else {
+#pragma unroll
+            for (int b = 0; b < C::NF; b++) {
+                const Fp8Row w = fp8_read(W, (wn * C::NF + b) * 32 + c32, h);
+#pragma unroll
+                for (int a = 0; a < C::MF; a++) {
+                    fp8_f16v d = {};
+                    d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp8_operand(w, 0), fp8_operand(x[a], 0), d, 0, 0, 0, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp8_operand(w, 1), fp8_operand(x[a], 1), d, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[b][a][r] = __builtin_fmaf(d[r], f[a], acc[b][a][r]);
+                }
+            }
+        }
+        // step s + 1 has landed and every wave is done reading step s
+        __builtin_amdgcn_sched_barrier(0);
+        fp8_wait<(C::S - 2) * C::DMA>();
+        __builtin_amdgcn_s_barrier();
+    }
+    // what is still in flight lands in the ring before y passes through it
+    fp8_wait<0>();
+    __builtin_amdgcn_s_barrier();
+
+    // y: a wave's 32 rows at a time through LDS, so that stores run along n
+    constexpr int SIZE = YT == T_F32 ? 4 : 2, PER = 16 / SIZE, LANES = 32 * C::NF / PER, ROWS = 64 / LANES;
+    uint8_t* part = smem + wv * 32 * C::PITCH;
+    const int col0 = n0 + wn * 32 * C::NF, cl = lane % LANES * PER;
+    const bool wide = c.n % PER == 0;
+#pragma unroll
+    for (int a = 0; a < C::MF; a++) {
+#pragma unroll
+        for (int b = 0; b < C::NF; b++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                uint8_t* p = part + c32 * C::PITCH + SIZE * (32 * b + 2 * r + 4 * h);
+                if constexpr (YT == T_F32) {
+                    *(float4*)p = make_float4(acc[b][a][r], acc[b][a][r + 1], acc[b][a][r + 2], acc[b][a][r + 3]);
+                } else {
+                    *(uint2*)p = make_uint2(
+                        fp8_half_bits<YT>(acc[b][a][r]) | (uint32_t)fp8_half_bits<YT>(acc[b][a][r + 1]) << 16,
+                        fp8_half_bits<YT>(acc[b][a][r + 2]) | (uint32_t)fp8_half_bits<YT>(acc[b][a][r + 3]) << 16);
+                }
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 32; i += ROWS) {
+            const int lr = i + lane / LANES, row = (wm * C::MF + a) * 32 + lr, col = col0 + cl;
+            const uint4 v = *(const uint4*)(part + lr * C::PITCH + SIZE * cl);
+            if (row >= tile.count || col >= c.n) continue;
+            const int yr = fp8_y_row(c, tile.first + row);
+            if (yr < 0) continue;
+            uint8_t* y = (uint8_t*)c.y + ((int64_t)yr * c.n + col) * SIZE;
+            if (wide) {
+                *(uint4*)y = v;
+            } else {
+                const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < PER; j++) {
+                    if (col + j >= c.n) break;
+                    if constexpr (YT == T_F32) ((uint32_t*)y)[j] = e[j];
+                    else ((uint16_t*)y)[j] = (uint16_t)(e[j >> 1] >> (16 * (j & 1)));
+                }
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
+template <class C, bool EXACT, int YT>
+static hipError_t tile_of_type(const Fp8Call& c, hipStream_t s) {
+    const int nbn = (c.n + C::BN - 1) / C::BN;
+    const hipError_t e = set_lds_limit((const void*)k_fp8_tile<C, EXACT, YT>, C::LDS);
+    if (e != hipSuccess) return e;
+    k_fp8_tile<C, EXACT, YT><<<dim3((uint32_t)(fp8_tiles(c, C::BM) * nbn)), C::THREADS, C::LDS, s>>>(c, nbn);
+    return hipGetLastError();
+}
+
+using Cfg256 = Fp8Cfg<4, 2, 2, 4, 2>;  // 256 rows of x, 256 of the weight
+using Cfg128 = Fp8Cfg<2, 2, 2, 2, 2>;  // 128, 128
+
+template <class C>
+static hipError_t tile_with(int y_type, const Fp8Call& c, hipStream_t s) {
+    return y_type == T_F16 ? tile_of_type<C, false, T_F16>(c, s) : tile_of_type<C, false, T_BF16>(c, s);
+}
+
+bool fp8_tile_fits(const Fp8Call& c) {
+    // 32-bit offsets: of a tile's weight rows, of x's rows (all of them where they are gathered) and of their scales
+    const int64_t rows = c.gather ? c.x_rows : 256, most = FP8_OUT;
+    return (int64_t)257 * c.k < most && rows * c.x_stride + c.k < most &&
+           (rows * c.xs_row + c.kb * c.xs_block) * 4 < most;
+}
+
+hipError_t launch_fp8_tile(int y_type, const Fp8Call& c, hipStream_t s) {
+    if (y_type == T_F32) return tile_of_type<Cfg128, true, T_F32>(c, s);
+    return c.m >= 2048 ? tile_with<Cfg256>(y_type, c, s) : tile_with<Cfg128>(y_type, c, s);
+}
+
+}  // namespace lloom

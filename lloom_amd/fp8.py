@@ -16,6 +16,7 @@ with y [tokens * topk, n] in the order of ids, as QTensor.indexed_moe_forward ha
 only the GPU can see (an id, a start or a row out of range) is left out of the result and raised by the next paged_check()
 as EEXPERT.
 """
+import ctypes
 from typing import NamedTuple
 
 import torch
@@ -225,3 +226,14 @@ def fp8_grouped_matmul(x, weight, weight_scales, starts, x_scales=None, gather=N
                                              r.data_ptr(), _IDS[r.dtype], _stride(r), xs, s0, s1, r.shape[0], st, g, c, rows,
                                              out.data_ptr(), _IDS[dtype], shape[0], _stream_of(i)))
     return out
+
+
+def fp8_workspace_bytes(dtype, rows, k, x_rows=None, experts=1):
+    """The workspace a product of `rows` rows takes (reserve_workspace it before a capture): x of dtype [x_rows, k], as many
+    as rows by default."""
+    if dtype not in _IDS:
+        raise LloomHipError(2, f"fp8_workspace_bytes: {dtype} is not f32, f16, bf16 or e4m3")
+    out = ctypes.c_size_t()
+    check(lib().lloom_hip_fp8_workspace_bytes(_IDS[dtype], rows, rows if x_rows is None else x_rows, experts, k,
+                                              ctypes.byref(out)))
+    return out.value

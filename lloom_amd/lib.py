@@ -86,6 +86,7 @@ def lib():
                 "lloom_hip_expert_plan": ([vp, vp, i64, i64, i64, vp, vp, vp, vp], i32),
                 "lloom_hip_fp8_grouped_matmul": ([vp, vp, vp, i64, i64, i64, vp, i32, i64, vp, i64, i64, i64, vp, vp, vp,
                                                   i64, vp, i32, i64, vp], i32),
+                "lloom_hip_fp8_workspace_bytes": ([i32, i64, i64, i64, i64, ctypes.POINTER(sz)], i32),
                 "lloom_hip_synth_normal": ([ctypes.c_uint64, ctypes.c_float, ctypes.c_float, vp, i64], i32),
                 "lloom_hip_synth_uniform": ([ctypes.c_uint64, ctypes.c_float, ctypes.c_float, vp, i64], i32),
             }

@@ -432,6 +432,14 @@ extern "C" {
         y_rows: i64,
         stream: *mut c_void,
     ) -> c_int;
+    pub fn lloom_hip_fp8_workspace_bytes(
+        x_dtype: c_int,
+        rows: i64,
+        x_rows: i64,
+        experts: i64,
+        k: i64,
+        bytes: *mut usize,
+    ) -> c_int;
 
     // Host-side synthetic inputs (StdRng-seeded normal / uniform), for benches.
     pub fn lloom_hip_synth_normal(seed: u64, mean: f32, std: f32, out: *mut f32, count: i64) -> c_int;
