@@ -53,7 +53,16 @@ template <int N>
 __device__ __forceinline__ void fp8_wait() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ int fp8_swizzle(int row) { return row & 7; }
+// A load and its wait in one: left to the compiler, the loop would wait for
+// it, and so for the whole next stage, in every step.
+__device__ __forceinline__ float fp8_load_now(const float* p) {
+    float v;
+    asm volatile("global_load_dword %0, %1, off\n\ts_waitcnt vmcnt(0)" : "=&v"(v) : "v"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ int fp8_swizzle(int row) { return (row >> 1) & 7; }
+// The piece of `row` that a lane brings to its place in the row.
+__device__ __forceinline__ int fp8_piece(int row, int lane) { return (lane & 7) ^ fp8_swizzle(row); }
 
 // A lane's 64 bytes of a row of a stage.
 struct Fp8Row {
@@ -94,15 +103,14 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
     const fp8_v4i xbuf = fp8_buffer((const uint8_t*)c.x + x0 * c.x_stride);
     const fp8_v4i sbuf = fp8_buffer(c.xs + x0 * c.xs_row);
     uint32_t woff[C::W_LOADS], xoff[C::X_LOADS], soff[C::XS_LOADS];
-    const int piece = (lane & 7) ^ fp8_swizzle(lane >> 3);  // the lane's, of every row that it loads
 #pragma unroll
     for (int i = 0; i < C::W_LOADS; i++) {
-        const int row = 8 * (wv * C::W_LOADS + i) + (lane >> 3);
+        const int row = 8 * (wv * C::W_LOADS + i) + (lane >> 3), piece = fp8_piece(row, lane);
         woff[i] = n0 + row < c.n ? (uint32_t)row * (uint32_t)c.k + 16u * piece : FP8_OUT;
     }
 #pragma unroll
     for (int i = 0; i < C::X_LOADS; i++) {
-        const int row = 8 * (wv * C::X_LOADS + i) + (lane >> 3);
+        const int row = 8 * (wv * C::X_LOADS + i) + (lane >> 3), piece = fp8_piece(row, lane);
         const int from = row < tile.count && steps ? fp8_x_row(c, tile.first + row) : -1;
         xoff[i] = from >= 0 ? (uint32_t)(from - (int)x0) * (uint32_t)c.x_stride + 16u * piece : FP8_OUT;
     }
@@ -115,13 +123,14 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
     const uint32_t lds0 = lds_addr(smem);
     auto issue = [&](int s, int slot) {
         const uint32_t st = lds0 + slot * C::STAGE, at = 128u * s;
-        const bool cut = 128 * s + 16 * piece >= c.k;  // past the end of the rows
+        const bool cut = c.k - 128 * s < 128;  // some pieces are past the end of the rows
+        auto past = [&](int row) { return cut && 128 * s + 16 * fp8_piece(row, lane) >= c.k; };
 #pragma unroll
         for (int i = 0; i < C::W_LOADS; i++)
-            fp8_dma16(wbuf, cut ? FP8_OUT : woff[i], at, st + 1024 * (wv * C::W_LOADS + i));
+            fp8_dma16(wbuf, past(8 * (wv * C::W_LOADS + i) + (lane >> 3)) ? FP8_OUT : woff[i], at, st + 1024 * (wv * C::W_LOADS + i));
 #pragma unroll
         for (int i = 0; i < C::X_LOADS; i++)
-            fp8_dma16(xbuf, cut ? FP8_OUT : xoff[i], at, st + C::W + 1024 * (wv * C::X_LOADS + i));
+            fp8_dma16(xbuf, past(8 * (wv * C::X_LOADS + i) + (lane >> 3)) ? FP8_OUT : xoff[i], at, st + C::W + 1024 * (wv * C::X_LOADS + i));
 #pragma unroll
         for (int i = 0; i < C::XS_LOADS; i++)
             fp8_dma4(sbuf, soff[i], (uint32_t)s * (uint32_t)c.xs_block * 4u,
@@ -144,7 +153,7 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
         __builtin_amdgcn_s_barrier();
     }
     for (int s = 0; s < steps; s++) {
-        if ((s & 63) == 0) wscale = ws[min(s + lane, c.kb - 1)];
+        if ((s & 63) == 0) wscale = fp8_load_now(ws + min(s + lane, c.kb - 1));
         issue(min(s + C::S - 1, steps - 1), (s + C::S - 1) % C::S);
         __builtin_amdgcn_sched_barrier(0);
         const uint8_t* W = smem + (s % C::S) * C::STAGE;
