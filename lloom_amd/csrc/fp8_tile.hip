@@ -9,7 +9,7 @@ namespace lloom {
 #pragma clang fp contract(off)
 
 // A workgroup has BM rows of x and BN of the weight, WM x WN waves with MF x NF
-// tiles of 32 x 32 each; k moves a block (128) a step through S LDS stages,
+// tiles of 32 x 32 each; k moves a block (128) a step through two LDS stages,
 //   W [BN][128] e4m3, piece p (16 bytes) of row r at p ^ swizzle(r)
 //   X [BM][128] likewise
 //   scales [BM] f32 of the block's rows
@@ -19,21 +19,21 @@ namespace lloom {
 // c of both operands: which bytes meet in which instruction does not matter.
 // The weight is the matrix instructions' A: a lane's 16 sums are of one row of x,
 // so one factor (its scale times the weight block's) serves them all.
-template <int WM_, int WN_, int MF_, int NF_, int S_>
+template <int WM_, int WN_, int MF_, int NF_>
 struct Fp8Cfg {
-    static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_, S = S_;
+    static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_;
     static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int BM = 32 * WM * MF, BN = 32 * WN * NF;
     static constexpr int SHIFT = BM == 32 ? 5 : BM == 64 ? 6 : BM == 128 ? 7 : 8;
     static constexpr int W = BN * 128, X = BM * 128, XS = BM * 4 < 256 ? 256 : BM * 4, STAGE = W + X + XS;
     static constexpr int W_LOADS = BN / 8 / WAVES, X_LOADS = BM / 8 / WAVES;
     static constexpr int XS_LOADS = (BM / 64 + WAVES - 1) / WAVES < 1 ? 1 : (BM / 64 + WAVES - 1) / WAVES;
-    static constexpr int DMA = W_LOADS + X_LOADS + XS_LOADS;
     static constexpr int PITCH = 32 * NF * 4 + 16;  // a row of a wave's part of y on its way out, f32 at most
-    static constexpr int OUT = WAVES * 32 * PITCH, RING = S * STAGE, LDS = RING > OUT ? RING : OUT;
+    static constexpr int OUT = WAVES * 32 * PITCH, RING = 2 * STAGE;
+    static constexpr int LDS = RING + BM * 4 > OUT ? RING + BM * 4 : OUT;
     static_assert(BM == 1 << SHIFT && W_LOADS * WAVES * 8 == BN && X_LOADS * WAVES * 8 == BM, "whole loads");
     static_assert(128 % (32 * NF) == 0, "a wave's weight rows share their scales");
-    static_assert((S - 1) * DMA <= 63 && LDS <= 160 * 1024, "counts and LDS");
+    static_assert(LDS <= 160 * 1024, "LDS");
 };
 
 constexpr uint32_t FP8_OUT = 0x80000000u;  // an offset that no buffer holds
@@ -49,10 +49,6 @@ __device__ __forceinline__ void fp8_dma16(fp8_v4i b, uint32_t voff, uint32_t sof
 __device__ __forceinline__ void fp8_dma4(fp8_v4i b, uint32_t voff, uint32_t soff, uint32_t lds) {
     asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(voff), "s"(b), "s"(soff), "{m0}"(lds) : "memory");
 }
-template <int N>
-__device__ __forceinline__ void fp8_wait() {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
 // A load and its wait in one: left to the compiler, the loop would wait for
 // it, and so for the whole next stage, in every step.
 __device__ __forceinline__ float fp8_load_now(const float* p) {
@@ -61,8 +57,9 @@ __device__ __forceinline__ float fp8_load_now(const float* p) {
     return v;
 }
 __device__ __forceinline__ int fp8_swizzle(int row) { return (row >> 1) & 7; }
-// The piece of `row` that a lane brings to its place in the row.
-__device__ __forceinline__ int fp8_piece(int row, int lane) { return (lane & 7) ^ fp8_swizzle(row); }
+// Keeps a tile's sums in the place of the program where they are written: the
+// compiler would gather a step's at its end, and spill.
+__device__ __forceinline__ void fp8_here(fp8_f16v& v) { asm volatile("" : "+v"(v)); }
 
 // A lane's 64 bytes of a row of a stage.
 struct Fp8Row {
@@ -70,8 +67,9 @@ struct Fp8Row {
 };
 __device__ __forceinline__ Fp8Row fp8_read(const uint8_t* rows, int row, int h) {
     Fp8Row r;
+    const int at = row * 128 + 16 * (h ^ fp8_swizzle(row));
 #pragma unroll
-    for (int i = 0; i < 4; i++) r.p[i] = *(const uint4*)(rows + row * 128 + 16 * ((2 * i + h) ^ fp8_swizzle(row)));
+    for (int i = 0; i < 4; i++) r.p[i] = *(const uint4*)(rows + (at ^ 32 * i));
     return r;
 }
 __device__ __forceinline__ v8i fp8_operand(const Fp8Row& r, int j) {
@@ -96,45 +94,51 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
     }
     const int n0 = bn * C::BN, steps = tile.zero ? 0 : c.kb;
 
-    // this wave's share of a stage: per-lane byte offsets, fixed for all steps
     const uint8_t* wbase = c.w + ((int64_t)tile.group * c.n + n0) * c.k;
     const fp8_v4i wbuf = fp8_buffer(wbase);
     const int64_t x0 = c.gather ? 0 : tile.first;
     const fp8_v4i xbuf = fp8_buffer((const uint8_t*)c.x + x0 * c.x_stride);
     const fp8_v4i sbuf = fp8_buffer(c.xs + x0 * c.xs_row);
-    uint32_t woff[C::W_LOADS], xoff[C::X_LOADS], soff[C::XS_LOADS];
-#pragma unroll
-    for (int i = 0; i < C::W_LOADS; i++) {
-        const int row = 8 * (wv * C::W_LOADS + i) + (lane >> 3), piece = fp8_piece(row, lane);
-        woff[i] = n0 + row < c.n ? (uint32_t)row * (uint32_t)c.k + 16u * piece : FP8_OUT;
-    }
-#pragma unroll
-    for (int i = 0; i < C::X_LOADS; i++) {
-        const int row = 8 * (wv * C::X_LOADS + i) + (lane >> 3), piece = fp8_piece(row, lane);
-        const int from = row < tile.count && steps ? fp8_x_row(c, tile.first + row) : -1;
-        xoff[i] = from >= 0 ? (uint32_t)(from - (int)x0) * (uint32_t)c.x_stride + 16u * piece : FP8_OUT;
-    }
-#pragma unroll
-    for (int i = 0; i < C::XS_LOADS; i++) {
-        const int row = (64 * (wv + C::WAVES * i) + lane) % (C::BM < 64 ? 64 : C::BM);
-        const int from = row < tile.count && steps ? fp8_x_row(c, tile.first + row) : -1;
-        soff[i] = from >= 0 ? (uint32_t)(from - (int)x0) * (uint32_t)c.xs_row * 4u : FP8_OUT;
-    }
+    // A wave's loads of an operand are WAVES * 8 rows apart, so its lanes' pieces
+    // are alike in all of them.  Rows of x are looked up in LDS, where they wait
+    // for their step (-1: none): held in registers their offsets would spill.
+    int* s_from = (int*)(smem + C::RING);
+    for (int row = threadIdx.x; row < C::BM; row += C::THREADS)
+        s_from[row] = row < tile.count && steps ? fp8_x_row(c, tile.first + row) - (int)x0 : -1;
+    __syncthreads();
+    const int row0 = 8 * wv + (lane >> 3), byte = 16 * ((lane & 7) ^ fp8_swizzle(row0));
+    const uint32_t wlast = (uint32_t)min(C::BN, c.n - n0) - 1;
     const uint32_t lds0 = lds_addr(smem);
-    auto issue = [&](int s, int slot) {
+    constexpr int XS_PARTS = C::BM < 64 ? 1 : C::BM / 64;
+    struct From {
+        int x[C::X_LOADS], s[C::XS_LOADS];
+    };
+    auto look = [&](From& from) {
+#pragma unroll
+        for (int i = 0; i < C::X_LOADS; i++) from.x[i] = s_from[row0 + 8 * C::WAVES * i];
+#pragma unroll
+        for (int i = 0; i < C::XS_LOADS; i++) from.s[i] = s_from[(64 * ((wv + C::WAVES * i) % XS_PARTS) + lane) % C::BM];
+    };
+    auto issue = [&](int s, int slot, const From& from) {
         const uint32_t st = lds0 + slot * C::STAGE, at = 128u * s;
-        const bool cut = c.k - 128 * s < 128;  // some pieces are past the end of the rows
-        auto past = [&](int row) { return cut && 128 * s + 16 * fp8_piece(row, lane) >= c.k; };
+        const bool past = (int)at + byte >= c.k;  // the last block's pieces past the end of the rows
 #pragma unroll
-        for (int i = 0; i < C::W_LOADS; i++)
-            fp8_dma16(wbuf, past(8 * (wv * C::W_LOADS + i) + (lane >> 3)) ? FP8_OUT : woff[i], at, st + 1024 * (wv * C::W_LOADS + i));
+        for (int i = 0; i < C::W_LOADS; i++) {
+            const uint32_t off = min((uint32_t)(row0 + 8 * C::WAVES * i), wlast) * (uint32_t)c.k + byte;
+            fp8_dma16(wbuf, past ? FP8_OUT : off, at, st + 1024 * (wv + C::WAVES * i));
+        }
 #pragma unroll
-        for (int i = 0; i < C::X_LOADS; i++)
-            fp8_dma16(xbuf, past(8 * (wv * C::X_LOADS + i) + (lane >> 3)) ? FP8_OUT : xoff[i], at, st + C::W + 1024 * (wv * C::X_LOADS + i));
+        for (int i = 0; i < C::X_LOADS; i++) {
+            const int r = from.x[i];
+            fp8_dma16(xbuf, past || r < 0 ? FP8_OUT : (uint32_t)r * (uint32_t)c.x_stride + byte, at,
+                      st + C::W + 1024 * (wv + C::WAVES * i));
+        }
 #pragma unroll
-        for (int i = 0; i < C::XS_LOADS; i++)
-            fp8_dma4(sbuf, soff[i], (uint32_t)s * (uint32_t)c.xs_block * 4u,
-                     st + C::W + C::X + 256 * ((wv + C::WAVES * i) % (C::BM < 64 ? 1 : C::BM / 64)));
+        for (int i = 0; i < C::XS_LOADS; i++) {
+            const int r = from.s[i];
+            fp8_dma4(sbuf, r < 0 ? FP8_OUT : (uint32_t)r * (uint32_t)c.xs_row * 4u,
+                     (uint32_t)s * (uint32_t)c.xs_block * 4u, st + C::W + C::X + 256 * ((wv + C::WAVES * i) % XS_PARTS));
+        }
     };
 
     fp8_f16v acc[C::NF][C::MF];
@@ -145,79 +149,111 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
 
     const float* ws = c.ws + ((int64_t)tile.group * c.nb + min((n0 + wn * 32 * C::NF) >> 7, c.nb - 1)) * c.kb;
     float wscale = 0.0f;  // lane l: of block 64 i + l
-    if (steps) {
-#pragma unroll
-        for (int i = 0; i < C::S - 1; i++) issue(min(i, steps - 1), i);
-        __builtin_amdgcn_sched_barrier(0);
-        fp8_wait<(C::S - 2) * C::DMA>();
-        __builtin_amdgcn_s_barrier();
-    }
-    for (int s = 0; s < steps; s++) {
+    auto weight_scale = [&](int s) {
         if ((s & 63) == 0) wscale = fp8_load_now(ws + min(s + lane, c.kb - 1));
-        issue(min(s + C::S - 1, steps - 1), (s + C::S - 1) % C::S);
+        return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wscale), s & 63));
+    };
+    auto read_w = [&](int slot, int b) { return fp8_read(smem + slot * C::STAGE, (wn * C::NF + b) * 32 + c32, h); };
+    auto read_x = [&](int slot, int a) { return fp8_read(smem + slot * C::STAGE + C::W, (wm * C::MF + a) * 32 + c32, h); };
+    auto read_s = [&](int slot, int a) {
+        return *(const float*)(smem + slot * C::STAGE + C::W + C::X + 4 * ((wm * C::MF + a) * 32 + c32));
+    };
+    // Everything of a step's stage is read before its last weight rows are
+    // multiplied: there the next stage has had a step's time to land, a barrier
+    // frees the slot for the one after, and the next step's first operands are
+    // read under the products that are left.
+    auto turn = [&](int s) {
+        From from;
+        look(from);
         __builtin_amdgcn_sched_barrier(0);
-        const uint8_t* W = smem + (s % C::S) * C::STAGE;
-        const uint8_t* X = W + C::W;
-        const float* XS = (const float*)(X + C::X);
-        const float sw = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wscale), s & 63));
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        if (s + 2 < steps) issue(s + 2, s & 1, from);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (steps) {
+        From from;
+        look(from);
+        issue(0, 0, from);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        if (steps > 1) issue(1, 1, from);
+        __builtin_amdgcn_sched_barrier(0);
+        Fp8Row x[C::MF], w = read_w(0, 0);
         float f[C::MF];
-        Fp8Row x[C::MF];
 #pragma unroll
-        for (int a = 0; a < C::MF; a++) {
-            const int row = (wm * C::MF + a) * 32 + c32;
-            f[a] = XS[row] * sw;
-            x[a] = fp8_read(X, row, h);
-        }
-        if constexpr (EXACT) {
-            fp8_h8 xh[C::MF][8];
+        for (int a = 0; a < C::MF; a++) x[a] = read_x(0, a), f[a] = read_s(0, a);
+        for (int s = 0; s < steps; s++) {
+            const float sw = weight_scale(s);
 #pragma unroll
-            for (int a = 0; a < C::MF; a++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    xh[a][2 * i] = fp8_halves(x[a].p[i].x, x[a].p[i].y);
-                    xh[a][2 * i + 1] = fp8_halves(x[a].p[i].z, x[a].p[i].w);
-                }
-#pragma unroll
-            for (int b = 0; b < C::NF; b++) {
-                const Fp8Row w = fp8_read(W, (wn * C::NF + b) * 32 + c32, h);
-                fp8_f16v d[C::MF];
-#pragma unroll
-                for (int a = 0; a < C::MF; a++) d[a] = fp8_f16v{};
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const fp8_h8 w0 = fp8_halves(w.p[i].x, w.p[i].y), w1 = fp8_halves(w.p[i].z, w.p[i].w);
-#pragma unroll
-                    for (int a = 0; a < C::MF; a++) {
-                        d[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w0, xh[a][2 * i], d[a], 0, 0, 0);
-                        d[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w1, xh[a][2 * i + 1], d[a], 0, 0, 0);
-                    }
-                }
+            for (int a = 0; a < C::MF; a++) f[a] *= sw;
+            float next[C::MF];
+            if constexpr (EXACT) {
+                fp8_h8 xh[C::MF][8];
 #pragma unroll
                 for (int a = 0; a < C::MF; a++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) acc[b][a][r] = __builtin_fmaf(d[a][r], f[a], acc[b][a][r]);
-            }
-        } else {
+                    for (int i = 0; i < 4; i++) {
+                        xh[a][2 * i] = fp8_halves(x[a].p[i].x, x[a].p[i].y);
+                        xh[a][2 * i + 1] = fp8_halves(x[a].p[i].z, x[a].p[i].w);
+                    }
 #pragma unroll
-            for (int b = 0; b < C::NF; b++) {
-                const Fp8Row w = fp8_read(W, (wn * C::NF + b) * 32 + c32, h);
+                for (int b = 0; b < C::NF; b++) {
+                    Fp8Row ahead;
+                    if (b == C::NF - 1) {
+                        turn(s);
+                        ahead = read_w((s + 1) & 1, 0);
 #pragma unroll
-                for (int a = 0; a < C::MF; a++) {
-                    fp8_f16v d = {};
-                    d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp8_operand(w, 0), fp8_operand(x[a], 0), d, 0, 0, 0, 0, 0, 0);
-                    d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp8_operand(w, 1), fp8_operand(x[a], 1), d, 0, 0, 0, 0, 0, 0);
+                        for (int a = 0; a < C::MF; a++) x[a] = read_x((s + 1) & 1, a), next[a] = read_s((s + 1) & 1, a);
+                    } else {
+                        ahead = read_w(s & 1, b + 1);
+                    }
+                    fp8_f16v d[C::MF];
 #pragma unroll
-                    for (int r = 0; r < 16; r++) acc[b][a][r] = __builtin_fmaf(d[r], f[a], acc[b][a][r]);
+                    for (int a = 0; a < C::MF; a++) d[a] = fp8_f16v{};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const fp8_h8 w0 = fp8_halves(w.p[i].x, w.p[i].y), w1 = fp8_halves(w.p[i].z, w.p[i].w);
+#pragma unroll
+                        for (int a = 0; a < C::MF; a++) {
+                            d[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w0, xh[a][2 * i], d[a], 0, 0, 0);
+                            d[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w1, xh[a][2 * i + 1], d[a], 0, 0, 0);
+                        }
+                    }
+#pragma unroll
+                    for (int a = 0; a < C::MF; a++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) acc[b][a][r] = __builtin_fmaf(d[a][r], f[a], acc[b][a][r]);
+                    w = ahead;
+                }
+            } else {
+#pragma unroll
+                for (int b = 0; b < C::NF; b++) {
+                    const Fp8Row ahead = b < C::NF - 1 ? read_w(s & 1, b + 1) : read_w((s + 1) & 1, 0);
+#pragma unroll
+                    for (int a = 0; a < C::MF; a++) {
+                        fp8_f16v d = {};
+                        d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp8_operand(w, 0), fp8_operand(x[a], 0), d, 0, 0, 0, 0, 0, 0);
+                        d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp8_operand(w, 1), fp8_operand(x[a], 1), d, 0, 0, 0, 0, 0, 0);
+                        if (b == C::NF - 2 && a == 0) {
+                            fp8_here(d);
+                            turn(s);
+                        }
+                        if (b == C::NF - 1) x[a] = read_x((s + 1) & 1, a), next[a] = read_s((s + 1) & 1, a);
+#pragma unroll
+                        for (int r = 0; r < 16; r++) acc[b][a][r] = __builtin_fmaf(d[r], f[a], acc[b][a][r]);
+                        fp8_here(acc[b][a]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    w = ahead;
                 }
             }
+#pragma unroll
+            for (int a = 0; a < C::MF; a++) f[a] = next[a];
         }
-        // step s + 1 has landed and every wave is done reading step s
-        __builtin_amdgcn_sched_barrier(0);
-        fp8_wait<(C::S - 2) * C::DMA>();
-        __builtin_amdgcn_s_barrier();
     }
-    // what is still in flight lands in the ring before y passes through it
-    fp8_wait<0>();
+    // every wave has read its last operands before y passes through the ring
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
 
     // y: a wave's 32 rows at a time through LDS, so that stores run along n
@@ -274,8 +310,8 @@ static hipError_t tile_of_type(const Fp8Call& c, hipStream_t s) {
     return hipGetLastError();
 }
 
-using Cfg256 = Fp8Cfg<4, 2, 2, 4, 2>;  // 256 rows of x, 256 of the weight
-using Cfg128 = Fp8Cfg<2, 2, 2, 2, 2>;  // 128, 128
+using Cfg256 = Fp8Cfg<4, 2, 2, 4>;  // 256 rows of x, 256 of the weight
+using Cfg128 = Fp8Cfg<2, 2, 2, 2>;  // 128, 128
 
 template <class C>
 static hipError_t tile_with(int y_type, const Fp8Call& c, hipStream_t s) {
