@@ -395,9 +395,9 @@ int lloom_hip_fp8_grouped_matmul(lloom_hip_ctx* ctx, const void* w_dev, const fl
                                  const uint32_t* starts_dev, const uint32_t* gather_dev, const uint32_t* scatter_dev,
                                  int64_t rows, void* y_dev, int y_dtype, int64_t y_rows, void* stream);
 
-/* Workspace of a product with `rows` rows (dense: experts = 1) of x's x_rows, to
- * reserve before a capture: where there are many rows, x of another type than
- * E4M3 is brought into 8 bits there, in a launch of its own. */
+/* Workspace of a product with `rows` rows of x's x_rows (experts 0: not grouped),
+ * to reserve before a capture: where a workgroup does not do that for itself, x
+ * of another type than E4M3 is brought into 8 bits there in a launch before. */
 int lloom_hip_fp8_workspace_bytes(int x_dtype, int64_t rows, int64_t x_rows, int64_t experts, int64_t k, size_t* bytes);
 
 /* ------------------------------------------------------- synthetic data --

@@ -30,7 +30,7 @@ struct Fp8Call {
     const int *starts, *gather, *scatter;
     int* flags;  // [0]: rows, starts or ids out of range
     int64_t x_stride, xs_row, xs_block;
-    int n, k, kb, nb, m, x_rows, y_rows, experts;
+    int n, k, kb, nb, m, x_rows, y_rows, experts, y_type;
 };
 
 // fp8_rows.hip: rows of x (F32, F16, BF16; x_stride elements apart) into e4m3 q
@@ -46,11 +46,12 @@ hipError_t launch_expert_plan(const int* ids, int64_t planes, int topk, int expe
                               int* tokens, int* flags, hipStream_t s);
 // Whether a call's groups have so few rows that fp8_few.hip serves them.
 inline bool fp8_few_rows(int64_t rows, int64_t experts) { return rows <= 16 * experts; }
-// fp8_few.hip: x of any type; y_type F32, F16 or BF16.
-hipError_t launch_fp8_few(int x_type, int y_type, const Fp8Call& c, hipStream_t s);
-// fp8_tile.hip: x E4M3.  Whether its 32-bit offsets hold the operands.
-bool fp8_tile_fits(const Fp8Call& c);
-hipError_t launch_fp8_tile(int y_type, const Fp8Call& c, hipStream_t s);
+// fp8_few.hip: x E4M3, or any type where fp8_few_fuses (it is brought into 8 bits
+// by each workgroup).
+bool fp8_few_fuses(int x_type, int64_t rows, int64_t k, bool grouped);
+hipError_t launch_fp8_few(int x_type, const Fp8Call& c, hipStream_t s);
+// fp8_tile.hip: x E4M3.
+hipError_t launch_fp8_tile(const Fp8Call& c, hipStream_t s);
 
 #if defined(__HIP_DEVICE_COMPILE__) || defined(__HIPCC__)
 
@@ -67,9 +68,24 @@ typedef _Float16 fp8_h8 __attribute__((ext_vector_type(8)));
 // biased e is the size's own exponent less 8, and one more where its fraction
 // passes .75.  The division by it is exact, so each value goes to the e4m3
 // number that is nearest to it, whatever the arithmetic.
+__device__ __forceinline__ uint32_t fp8_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 __device__ __forceinline__ uint32_t fp8_size(float v) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
+    const uint32_t u = fp8_bits(v);
     return u < 0x7f800000u ? u : 0u;  // what is no number, or infinite, has no say
+}
+// Largest size of N values: as bits, and value by value only where some are no
+// numbers (theirs are the largest bits).
+template <int N>
+__device__ __forceinline__ uint32_t fp8_largest(const float (&v)[N]) {
+    uint32_t u = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) u = max(u, fp8_bits(v[i]));
+    if (__builtin_expect(u >= 0x7f800000u, 0)) {
+        u = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) u = max(u, fp8_size(v[i]));
+    }
+    return u;
 }
 __device__ __forceinline__ int fp8_exponent(uint32_t size) {
     return size ? max((int)((size + 0x1fffffu) >> 23) - 8, 1) : 127;
@@ -77,6 +93,11 @@ __device__ __forceinline__ int fp8_exponent(uint32_t size) {
 __device__ __forceinline__ float fp8_scale(int biased) { return __builtin_bit_cast(float, biased << 23); }
 __device__ __forceinline__ float fp8_inverse(int biased) { return __builtin_bit_cast(float, (254 - biased) << 23); }
 
+// Largest of the lanes that are 16 apart, in all of them.
+__device__ __forceinline__ uint32_t column_max(uint32_t v) {
+    v = max(v, __builtin_bit_cast(uint32_t, partner16(__builtin_bit_cast(float, v))));
+    return max(v, __builtin_bit_cast(uint32_t, partner32(__builtin_bit_cast(float, v))));
+}
 // Largest of the 16 lanes of a row, in all of them.
 __device__ __forceinline__ uint32_t row16_max(uint32_t v) {
     v = max(v, (uint32_t)dppi<DPP_XOR1>((int)v));
@@ -163,6 +184,17 @@ __device__ __forceinline__ void fp8_store4(void* y, int64_t i, const float (&v)[
     }
 }
 
+// --------------------------------------------------------------- buffers --
+// Operands are read through buffers of 2^31 bytes from a tile's own first: what is
+// not there (rows past the operand's or a tile's, bytes past k) gets an offset
+// that no buffer holds, which reads zeros and nothing of memory.
+constexpr uint32_t FP8_OUT = 0x80000000u;
+__device__ __forceinline__ fp8_v4i fp8_buffer(const void* p) {
+    const uint64_t a = (uint64_t)p;
+    return fp8_v4i{(int)__builtin_amdgcn_readfirstlane((int)a),
+                   (int)__builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff), (int)FP8_OUT, 0x00020000};
+}
+
 // ---------------------------------------------------------- tiles of rows --
 // Tile t of a call whose groups are cut into tiles of up to 2^SHIFT rows, in
 // the groups' order, then the rows past the last group (`zero`: no group owns
@@ -173,15 +205,18 @@ struct Fp8Tile {
     int group, first, count;
     bool zero;
 };
-__device__ __forceinline__ int wave_scan(int v) {  // inclusive
-    const int lane = __lane_id();
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o, 64);
-        if (lane >= o) v += u;
-    }
-    return v;
+// Inclusive sums over the lanes, by DPP alone: within rows of 16 (row_shr), then
+// the last lane of a row to the next (row_bcast15) and of the first half to the
+// second (row_bcast31).
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
 }
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 template <int SHIFT>
 __device__ __forceinline__ Fp8Tile fp8_tile(const Fp8Call& c, int t) {
     constexpr int ROWS = 1 << SHIFT;
@@ -190,20 +225,29 @@ __device__ __forceinline__ Fp8Tile fp8_tile(const Fp8Call& c, int t) {
     Fp8Tile r = {0, 0, 0, true};
     int before = 0;
     bool bad = c.starts[0] != 0;
-    for (int base = 0; base <= E; base += 64) {
-        const int e = base + lane;
-        const int at = e <= E ? c.starts[e] : 0, next = e < E ? c.starts[e + 1] : c.m;
-        const int count = e <= E ? next - at : 0;
-        bad |= at < 0 || at > c.m || count < 0;
-        const int tiles = (int)(((uint32_t)count + ROWS - 1) >> SHIFT);
-        const int upto = before + wave_scan(tiles);
-        const uint64_t hit = __ballot(t < upto && t >= upto - tiles);
-        if (hit) {
-            const int j = __builtin_ctzll(hit);
-            const int in = (t - (__shfl(upto, j, 64) - __shfl(tiles, j, 64))) << SHIFT;
-            r = {base + j, __shfl(at, j, 64) + in, min(ROWS, __shfl(count, j, 64) - in), base + j == E};
+    for (int base = 0; base <= E; base += 256) {
+        int at[4], next[4];  // loads of 256 groups together
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int e = base + 64 * i + lane;
+            at[i] = e <= E ? c.starts[e] : c.m;
+            next[i] = e < E ? c.starts[e + 1] : c.m;
         }
-        before = __shfl(upto, 63, 64);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (base + 64 * i > E) break;
+            const int count = next[i] - at[i];
+            bad |= at[i] < 0 || at[i] > c.m || count < 0;
+            const int tiles = (int)(((uint32_t)count + ROWS - 1) >> SHIFT);
+            const int upto = before + wave_scan(tiles);
+            const uint64_t hit = __ballot(t < upto && t >= upto - tiles);
+            if (hit) {
+                const int j = __builtin_ctzll(hit), g = base + 64 * i + j;
+                const int in = (t - (lane_value(upto, j) - lane_value(tiles, j))) << SHIFT;
+                r = {g, lane_value(at[i], j) + in, min(ROWS, lane_value(count, j) - in), g == E};
+            }
+            before = lane_value(upto, 63);
+        }
     }
     if (__ballot(bad)) {
         r = {0, t << SHIFT, min(ROWS, c.m - (t << SHIFT)), true};

@@ -78,13 +78,24 @@ struct XCopy {
     bool needed;
     size_t scales_at, bytes;
 };
-XCopy x_copy(int x_type, int64_t rows, int64_t x_rows, int64_t experts, int64_t k) {
+XCopy x_copy(int x_type, int64_t rows, int64_t x_rows, int64_t k, bool grouped) {
     const size_t q = ((size_t)x_rows * k + 255) & ~(size_t)255;
-    return {x_type != T_E4M3 && !fp8_few_rows(rows, experts), q, q + (size_t)x_rows * ((k + 127) / 128) * sizeof(float)};
+    return {x_type != T_E4M3 && !fp8_few_fuses(x_type, rows, k, grouped), q,
+            q + (size_t)x_rows * ((k + 127) / 128) * sizeof(float)};
 }
 
-int run_product(lloom_hip_ctx* ctx, int x_type, int y_type, Fp8Call c, hipStream_t s) {
-    const XCopy copy = x_copy(x_type, c.m, c.x_rows, c.experts, c.k);
+// The kernels' 32-bit offsets: of a tile's rows of x, or of all rows that may be
+// gathered, and of their scales.
+int check_offsets(const char* what, int64_t rows, int64_t row_bytes, int64_t xs_row, int64_t xs_block, int64_t k) {
+    const int64_t most = (int64_t)1 << 31;
+    if (rows * row_bytes + k < most && (rows * xs_row + (k + 127) / 128 * xs_block) * 4 < most) return LLOOM_HIP_OK;
+    return fail(LLOOM_HIP_ESHAPE, "%s: %lld rows of x, %lld bytes apart, are past 2^31 bytes (or their scales are)", what,
+                (long long)rows, (long long)row_bytes);
+}
+
+int run_product(lloom_hip_ctx* ctx, int x_type, Fp8Call c, hipStream_t s) {
+    const bool grouped = c.starts != nullptr;
+    const XCopy copy = x_copy(x_type, c.m, c.x_rows, c.k, grouped);
     std::unique_lock<std::mutex> lock(ctx->mu, std::defer_lock);
     if (copy.needed && c.x_rows) {
         lock.lock();
@@ -95,8 +106,11 @@ int run_product(lloom_hip_ctx* ctx, int x_type, int y_type, Fp8Call c, hipStream
         c.x = ws, c.x_stride = c.k, c.xs = scales, c.xs_row = 1, c.xs_block = c.x_rows;
         x_type = T_E4M3;
     }
-    if (x_type == T_E4M3 && !fp8_few_rows(c.m, c.experts) && fp8_tile_fits(c)) HIP_OK(launch_fp8_tile(y_type, c, s));
-    else HIP_OK(launch_fp8_few(x_type, y_type, c, s));
+    if (int rc = check_offsets(grouped ? "fp8_grouped_matmul" : "fp8_matmul", c.gather ? c.x_rows : 256,
+                               c.x_stride * type_bytes(x_type), c.xs_row, c.xs_block, c.k))
+        return rc;
+    if (fp8_few_rows(c.m, c.experts)) HIP_OK(launch_fp8_few(x_type, c, s));
+    else HIP_OK(launch_fp8_tile(c, s));
     return LLOOM_HIP_OK;
 }
 
@@ -172,8 +186,8 @@ int lloom_hip_fp8_matmul(lloom_hip_ctx* ctx, const void* w_dev, const float* w_s
     HIP_OK(hipSetDevice(ctx->device));
     const Fp8Call c = {(const uint8_t*)w_dev, w_scales_dev, x_dev, x_scales_dev, y_dev, nullptr, nullptr, nullptr,
                        ctx->flags, x_stride, xs_row, xs_block, (int)n, (int)k, (int)((k + 127) / 128),
-                       (int)((n + 127) / 128), (int)m, (int)m, (int)m, 1};
-    return run_product(ctx, x_dtype, y_dtype, c, (hipStream_t)stream);
+                       (int)((n + 127) / 128), (int)m, (int)m, (int)m, 1, y_dtype};
+    return run_product(ctx, x_dtype, c, (hipStream_t)stream);
 }
 
 int lloom_hip_fp8_grouped_matmul(lloom_hip_ctx* ctx, const void* w_dev, const float* w_scales_dev, int64_t experts,
@@ -196,8 +210,8 @@ int lloom_hip_fp8_grouped_matmul(lloom_hip_ctx* ctx, const void* w_dev, const fl
     const Fp8Call c = {(const uint8_t*)w_dev, w_scales_dev, x_dev, x_scales_dev, y_dev, (const int*)starts_dev,
                        (const int*)gather_dev, (const int*)scatter_dev, ctx->flags, x_stride, xs_row, xs_block, (int)n,
                        (int)k, (int)((k + 127) / 128), (int)((n + 127) / 128), (int)rows, (int)x_rows, (int)y_rows,
-                       (int)experts};
-    return run_product(ctx, x_dtype, y_dtype, c, (hipStream_t)stream);
+                       (int)experts, y_dtype};
+    return run_product(ctx, x_dtype, c, (hipStream_t)stream);
 }
 
 int lloom_hip_expert_plan(lloom_hip_ctx* ctx, const uint32_t* ids_dev, int64_t tokens, int64_t topk, int64_t experts,
@@ -221,13 +235,13 @@ int lloom_hip_fp8_workspace_bytes(int x_dtype, int64_t rows, int64_t x_rows, int
     if (x_dtype != T_E4M3)
         if (int rc = check_act("fp8_workspace_bytes", x_dtype)) return rc;
     if (int rc = check_k("fp8_workspace_bytes", k)) return rc;
-    if (rows < 0 || x_rows < 0 || experts < 1)
+    if (rows < 0 || x_rows < 0 || experts < 0)
         return fail(LLOOM_HIP_EINVAL, "fp8_workspace_bytes: %lld rows of %lld, %lld experts", (long long)rows,
                     (long long)x_rows, (long long)experts);
     if (rows > MAX_ROWS || x_rows > MAX_ROWS || experts > MOE_MAX_EXPERTS)
         return fail(LLOOM_HIP_ESHAPE, "fp8_workspace_bytes: %lld rows of %lld (at most %lld), %lld experts (at most %d)",
                     (long long)rows, (long long)x_rows, (long long)MAX_ROWS, (long long)experts, MOE_MAX_EXPERTS);
-    const XCopy copy = x_copy(x_dtype, rows, x_rows, experts, k);
+    const XCopy copy = x_copy(x_dtype, rows, x_rows, k, experts > 0);
     *bytes = copy.needed ? copy.bytes : 0;
     return LLOOM_HIP_OK;
 }

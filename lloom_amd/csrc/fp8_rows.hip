@@ -37,10 +37,7 @@ __global__ __launch_bounds__(256) void k_fp8_rows(const void* __restrict__ x, in
     }
 #pragma unroll
     for (int i = 0; i < R; i++) {
-        uint32_t size = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) size = max(size, fp8_size(v[i][j]));
-        const int e = fp8_exponent(row16_max(size));
+        const int e = fp8_exponent(row16_max(fp8_largest(v[i])));
         const float f = fp8_inverse(e);
         if (in && r0 + i < rows)
             *(uint2*)(q + (int64_t)(r0 + i) * k + col) =
@@ -99,13 +96,10 @@ __global__ __launch_bounds__(256) void k_fp8_weights(const void* __restrict__ w,
         const int row = row0 + 16 * i;
         if (row < n && col < k) {
             fp8_load8<TYPE>(w, (plane * n + row) * k + col, v[i]);
-#pragma unroll
-            for (int j = 0; j < 8; j++) size = max(size, fp8_size(v[i][j]));
+            size = max(size, fp8_largest(v[i]));
         }
     }
-    size = row16_max(size);
-    size = max(size, (uint32_t)__shfl_xor((int)size, 16, 64));
-    size = max(size, (uint32_t)__shfl_xor((int)size, 32, 64));
+    size = column_max(row16_max(size));
     if ((threadIdx.x & 63) == 0) s_size[threadIdx.x >> 6] = size;
     __syncthreads();
     const int e = fp8_exponent(max(max(s_size[0], s_size[1]), max(s_size[2], s_size[3])));

@@ -36,13 +36,6 @@ struct Fp8Cfg {
     static_assert(LDS <= 160 * 1024, "LDS");
 };
 
-constexpr uint32_t FP8_OUT = 0x80000000u;  // an offset that no buffer holds
-
-__device__ __forceinline__ fp8_v4i fp8_buffer(const void* p) {
-    const uint64_t a = (uint64_t)p;
-    return fp8_v4i{(int)__builtin_amdgcn_readfirstlane((int)a),
-                   (int)__builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff), (int)FP8_OUT, 0x00020000};
-}
 __device__ __forceinline__ void fp8_dma16(fp8_v4i b, uint32_t voff, uint32_t soff, uint32_t lds) {
     asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(b), "s"(soff), "{m0}"(lds) : "memory");
 }
@@ -314,20 +307,13 @@ using Cfg256 = Fp8Cfg<4, 2, 2, 4>;  // 256 rows of x, 256 of the weight
 using Cfg128 = Fp8Cfg<2, 2, 2, 2>;  // 128, 128
 
 template <class C>
-static hipError_t tile_with(int y_type, const Fp8Call& c, hipStream_t s) {
-    return y_type == T_F16 ? tile_of_type<C, false, T_F16>(c, s) : tile_of_type<C, false, T_BF16>(c, s);
+static hipError_t tile_with(const Fp8Call& c, hipStream_t s) {
+    return c.y_type == T_F16 ? tile_of_type<C, false, T_F16>(c, s) : tile_of_type<C, false, T_BF16>(c, s);
 }
 
-bool fp8_tile_fits(const Fp8Call& c) {
-    // 32-bit offsets: of a tile's weight rows, of x's rows (all of them where they are gathered) and of their scales
-    const int64_t rows = c.gather ? c.x_rows : 256, most = FP8_OUT;
-    return (int64_t)257 * c.k < most && rows * c.x_stride + c.k < most &&
-           (rows * c.xs_row + c.kb * c.xs_block) * 4 < most;
-}
-
-hipError_t launch_fp8_tile(int y_type, const Fp8Call& c, hipStream_t s) {
-    if (y_type == T_F32) return tile_of_type<Cfg128, true, T_F32>(c, s);
-    return c.m >= 2048 ? tile_with<Cfg256>(y_type, c, s) : tile_with<Cfg128>(y_type, c, s);
+hipError_t launch_fp8_tile(const Fp8Call& c, hipStream_t s) {
+    if (c.y_type == T_F32) return tile_of_type<Cfg128, true, T_F32>(c, s);
+    return c.m >= 2048 ? tile_with<Cfg256>(c, s) : tile_with<Cfg128>(c, s);
 }
 
 }  // namespace lloom

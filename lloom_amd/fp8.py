@@ -228,9 +228,9 @@ def fp8_grouped_matmul(x, weight, weight_scales, starts, x_scales=None, gather=N
     return out
 
 
-def fp8_workspace_bytes(dtype, rows, k, x_rows=None, experts=1):
+def fp8_workspace_bytes(dtype, rows, k, x_rows=None, experts=0):
     """The workspace a product of `rows` rows takes (reserve_workspace it before a capture): x of dtype [x_rows, k], as many
-    as rows by default."""
+    as rows by default; experts: 0 for fp8_matmul."""
     if dtype not in _IDS:
         raise LloomHipError(2, f"fp8_workspace_bytes: {dtype} is not f32, f16, bf16 or e4m3")
     out = ctypes.c_size_t()

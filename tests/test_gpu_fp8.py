@@ -179,7 +179,7 @@ def check_product(y, x, xs, w, ws):
     assert np.all(np.abs(got - want) <= off), np.max(np.abs(got - want) / off)
 
 
-SIZES = [(1, 16, 16), (1, 64, 128), (2, 24, 144), (5, 130, 272), (16, 128, 2048), (17, 257, 1040), (33, 96, 96), (64, 384, 640),
+SIZES = [(1, 16, 16), (1, 6152, 912), (1, 80, 8208), (4, 16400, 272), (12, 4104, 2064), (1, 64, 128), (2, 24, 144), (5, 130, 272), (16, 128, 2048), (17, 257, 1040), (33, 96, 96), (64, 384, 640),
          (65, 200, 1376), (129, 127, 512), (255, 264, 768), (300, 520, 256), (1030, 1000, 400),
          (2100, 264, 144), (2049, 300, 912)]
 
@@ -217,7 +217,7 @@ def ragged(counts, extra, seed):
 
 GROUPS = [([3], 0), ([0, 1, 16, 17, 0, 5], 0), ([15, 16, 17, 31, 32, 33, 0, 64, 65, 1], 3), ([127, 128, 129, 0, 255, 257], 1),
           ([0, 0, 0], 5), ([1] * 70, 0), ([0] * 130 + [9] + [0] * 60, 2), ([600, 1], 0),
-          ([1000, 0, 3, 1200, 257], 9)]
+          ([1000, 0, 3, 1200, 257], 9), ([1, 0, 2, 1, 0, 4], 2), ([3] * 600, 7)]
 
 
 @pytest.mark.parametrize("out", ACTS)
