@@ -109,7 +109,7 @@ int run_product(lloom_hip_ctx* ctx, int x_type, Fp8Call c, hipStream_t s) {
     if (int rc = check_offsets(grouped ? "fp8_grouped_matmul" : "fp8_matmul", c.gather ? c.x_rows : 256,
                                c.x_stride * type_bytes(x_type), c.xs_row, c.xs_block, c.k))
         return rc;
-    if (fp8_few_rows(c.m, c.experts)) HIP_OK(launch_fp8_few(x_type, c, s));
+    if (fp8_few_rows(c)) HIP_OK(launch_fp8_few(x_type, c, s));
     else HIP_OK(launch_fp8_tile(c, s));
     return LLOOM_HIP_OK;
 }

@@ -19,9 +19,9 @@ namespace lloom {
 // c of both operands: which bytes meet in which instruction does not matter.
 // The weight is the matrix instructions' A: a lane's 16 sums are of one row of x,
 // so one factor (its scale times the weight block's) serves them all.
-template <int WM_, int WN_, int MF_, int NF_>
+template <int WM_, int WN_, int MF_, int NF_, int S_>
 struct Fp8Cfg {
-    static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_;
+    static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_, S = S_;
     static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int BM = 32 * WM * MF, BN = 32 * WN * NF;
     static constexpr int SHIFT = BM == 32 ? 5 : BM == 64 ? 6 : BM == 128 ? 7 : 8;
@@ -29,11 +29,12 @@ struct Fp8Cfg {
     static constexpr int W_LOADS = BN / 8 / WAVES, X_LOADS = BM / 8 / WAVES;
     static constexpr int XS_LOADS = (BM / 64 + WAVES - 1) / WAVES < 1 ? 1 : (BM / 64 + WAVES - 1) / WAVES;
     static constexpr int PITCH = 32 * NF * 4 + 16;  // a row of a wave's part of y on its way out, f32 at most
-    static constexpr int OUT = WAVES * 32 * PITCH, RING = 2 * STAGE;
+    static constexpr int OUT = WAVES * 32 * PITCH, RING = S * STAGE;
     static constexpr int LDS = RING + BM * 4 > OUT ? RING + BM * 4 : OUT;
     static_assert(BM == 1 << SHIFT && W_LOADS * WAVES * 8 == BN && X_LOADS * WAVES * 8 == BM, "whole loads");
     static_assert(128 % (32 * NF) == 0, "a wave's weight rows share their scales");
-    static_assert(LDS <= 160 * 1024, "LDS");
+    static constexpr int DMA = W_LOADS + X_LOADS + XS_LOADS;  // a wave's loads of a stage
+    static_assert((S - 1) * DMA <= 63 && LDS <= 160 * 1024, "counts and LDS");
 };
 
 __device__ __forceinline__ void fp8_dma16(fp8_v4i b, uint32_t voff, uint32_t soff, uint32_t lds) {
@@ -50,6 +51,11 @@ __device__ __forceinline__ float fp8_load_now(const float* p) {
     return v;
 }
 __device__ __forceinline__ int fp8_swizzle(int row) { return (row >> 1) & 7; }
+// This wave's reads of LDS are done, and all its loads but the last N.
+template <int N>
+__device__ __forceinline__ void fp8_landed() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
 // Keeps a tile's sums in the place of the program where they are written: the
 // compiler would gather a step's at its end, and spill.
 __device__ __forceinline__ void fp8_here(fp8_f16v& v) { asm volatile("" : "+v"(v)); }
@@ -152,37 +158,42 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
         return *(const float*)(smem + slot * C::STAGE + C::W + C::X + 4 * ((wm * C::MF + a) * 32 + c32));
     };
     // Everything of a step's stage is read before its last weight rows are
-    // multiplied: there the next stage has had a step's time to land, a barrier
-    // frees the slot for the one after, and the next step's first operands are
-    // read under the products that are left.
-    auto turn = [&](int s) {
+    // multiplied: there the next stage has had S - 1 steps' time to land, a barrier
+    // frees the slot for the one S steps on, and the next step's first operands
+    // are read under the products that are left.
+    auto turn = [&](int s, int slot) {
         From from;
         look(from);
         __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (C::S > 2 && s + C::S - 1 < steps) fp8_landed<(C::S - 2) * C::DMA>();
+        else fp8_landed<0>();
         __builtin_amdgcn_s_barrier();
-        if (s + 2 < steps) issue(s + 2, s & 1, from);
+        if (s + C::S < steps) issue(s + C::S, slot, from);
         __builtin_amdgcn_sched_barrier(0);
     };
     if (steps) {
         From from;
         look(from);
-        issue(0, 0, from);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < C::S; i++)
+            if (i < steps) issue(i, i, from);
+        if (steps >= C::S) fp8_landed<(C::S - 1) * C::DMA>();
+        else fp8_landed<0>();
         __builtin_amdgcn_s_barrier();
-        if (steps > 1) issue(1, 1, from);
         __builtin_amdgcn_sched_barrier(0);
         Fp8Row x[C::MF], w = read_w(0, 0);
         float f[C::MF];
 #pragma unroll
         for (int a = 0; a < C::MF; a++) x[a] = read_x(0, a), f[a] = read_s(0, a);
+        int slot = 0;
         for (int s = 0; s < steps; s++) {
+            const int after = slot + 1 < C::S ? slot + 1 : 0;
             const float sw = weight_scale(s);
 #pragma unroll
             for (int a = 0; a < C::MF; a++) f[a] *= sw;
             float next[C::MF];
+            fp8_h8 xh[EXACT ? C::MF : 1][8];
             if constexpr (EXACT) {
-                fp8_h8 xh[C::MF][8];
 #pragma unroll
                 for (int a = 0; a < C::MF; a++)
 #pragma unroll
@@ -190,17 +201,11 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
                         xh[a][2 * i] = fp8_halves(x[a].p[i].x, x[a].p[i].y);
                         xh[a][2 * i + 1] = fp8_halves(x[a].p[i].z, x[a].p[i].w);
                     }
+            }
 #pragma unroll
-                for (int b = 0; b < C::NF; b++) {
-                    Fp8Row ahead;
-                    if (b == C::NF - 1) {
-                        turn(s);
-                        ahead = read_w((s + 1) & 1, 0);
-#pragma unroll
-                        for (int a = 0; a < C::MF; a++) x[a] = read_x((s + 1) & 1, a), next[a] = read_s((s + 1) & 1, a);
-                    } else {
-                        ahead = read_w(s & 1, b + 1);
-                    }
+            for (int b = 0; b < C::NF; b++) {
+                const Fp8Row ahead = b < C::NF - 1 ? read_w(slot, b + 1) : read_w(after, 0);
+                if constexpr (EXACT) {
                     fp8_f16v d[C::MF];
 #pragma unroll
                     for (int a = 0; a < C::MF; a++) d[a] = fp8_f16v{};
@@ -213,16 +218,19 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
                             d[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w1, xh[a][2 * i + 1], d[a], 0, 0, 0);
                         }
                     }
+                    if (b == C::NF - 2) {
+                        fp8_here(d[C::MF - 1]);
+                        turn(s, slot);
+                    }
 #pragma unroll
-                    for (int a = 0; a < C::MF; a++)
+                    for (int a = 0; a < C::MF; a++) {
+                        if (b == C::NF - 1) x[a] = read_x(after, a), next[a] = read_s(after, a);
 #pragma unroll
                         for (int r = 0; r < 16; r++) acc[b][a][r] = __builtin_fmaf(d[a][r], f[a], acc[b][a][r]);
-                    w = ahead;
-                }
-            } else {
-#pragma unroll
-                for (int b = 0; b < C::NF; b++) {
-                    const Fp8Row ahead = b < C::NF - 1 ? read_w(s & 1, b + 1) : read_w((s + 1) & 1, 0);
+                        fp8_here(acc[b][a]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                } else {
 #pragma unroll
                     for (int a = 0; a < C::MF; a++) {
                         fp8_f16v d = {};
@@ -230,19 +238,20 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
                         d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp8_operand(w, 1), fp8_operand(x[a], 1), d, 0, 0, 0, 0, 0, 0);
                         if (b == C::NF - 2 && a == 0) {
                             fp8_here(d);
-                            turn(s);
+                            turn(s, slot);
                         }
-                        if (b == C::NF - 1) x[a] = read_x((s + 1) & 1, a), next[a] = read_s((s + 1) & 1, a);
+                        if (b == C::NF - 1) x[a] = read_x(after, a), next[a] = read_s(after, a);
 #pragma unroll
                         for (int r = 0; r < 16; r++) acc[b][a][r] = __builtin_fmaf(d[r], f[a], acc[b][a][r]);
                         fp8_here(acc[b][a]);
                         __builtin_amdgcn_sched_barrier(0);
                     }
-                    w = ahead;
                 }
+                w = ahead;
             }
 #pragma unroll
             for (int a = 0; a < C::MF; a++) f[a] = next[a];
+            slot = after;
         }
     }
     // every wave has read its last operands before y passes through the ring
@@ -303,17 +312,34 @@ static hipError_t tile_of_type(const Fp8Call& c, hipStream_t s) {
     return hipGetLastError();
 }
 
-using Cfg256 = Fp8Cfg<4, 2, 2, 4>;  // 256 rows of x, 256 of the weight
-using Cfg128 = Fp8Cfg<2, 2, 2, 2>;  // 128, 128
-
 template <class C>
 static hipError_t tile_with(const Fp8Call& c, hipStream_t s) {
-    return c.y_type == T_F16 ? tile_of_type<C, false, T_F16>(c, s) : tile_of_type<C, false, T_BF16>(c, s);
+    switch (c.y_type) {
+        case T_F32: return tile_of_type<C, true, T_F32>(c, s);
+        case T_F16: return tile_of_type<C, false, T_F16>(c, s);
+        default: return tile_of_type<C, false, T_BF16>(c, s);
+    }
 }
 
+// The largest tile that is mostly full and leaves workgroups for all CUs; us by
+// (rows of x, of the weight) a tile:
+//   (32, 128) / (64, 128) / (128, 128): 256 rows of [4096, 4096] 19 / 21 / 27, 192 of
+//     [8192, 2048] 13.8 / 12.9 / 16.6, 128 of [8192, 8192] 36 / 55 / 61 (with two
+//     stages; three in the first)
+//   (64, 128) / (128, 128) / (256, 256): 509 rows of [8192, 2048] 15.8 / 17.8 / -, into
+//     f32 24.7 / 25.8; 2048 rows 59 / 48 / 41; 4096 of [4096, 4096] into f32 152 / 136
+//   grouped, top 8 of 128 experts [1536, 2048], 8, 12 and 32 rows an expert on
+//     average: 71 / 73 / 82, 77 / 75 / 81, 92 / 85 / 94; of 64 [2048, 2048], 256 and
+//     1024: - / 141 / 128 and (256, 256) 134, - / 451 / 402 / 368
 hipError_t launch_fp8_tile(const Fp8Call& c, hipStream_t s) {
-    if (c.y_type == T_F32) return tile_of_type<Cfg128, true, T_F32>(c, s);
-    return c.m >= 2048 ? tile_with<Cfg256>(c, s) : tile_with<Cfg128>(c, s);
+    auto count = [&](int rows, int cols) { return (int64_t)((c.m + rows - 1) / rows) * ((c.n + cols - 1) / cols); };
+    const int64_t each = c.m / c.experts;
+    if (c.y_type != T_F32 && (c.starts ? each >= 512 : count(256, 256) >= 200))
+        return c.y_type == T_F16 ? tile_of_type<Fp8Cfg<4, 2, 2, 4, 2>, false, T_F16>(c, s)
+                                 : tile_of_type<Fp8Cfg<4, 2, 2, 4, 2>, false, T_BF16>(c, s);
+    if (c.starts ? each >= 96 : count(128, 128) >= 300) return tile_with<Fp8Cfg<2, 2, 2, 2, 2>>(c, s);
+    if (c.starts ? each >= 10 : count(64, 128) >= 180) return tile_with<Fp8Cfg<2, 2, 1, 2, 2>>(c, s);
+    return tile_with<Fp8Cfg<1, 2, 1, 2, 3>>(c, s);
 }
 
 }  // namespace lloom
