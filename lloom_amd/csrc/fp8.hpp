@@ -204,7 +204,7 @@ __device__ __forceinline__ fp8_v4i fp8_buffer(const void* p) {
 // ---------------------------------------------------------- tiles of rows --
 // Tile t of a call whose groups are cut into tiles of up to 2^SHIFT rows, in
 // the groups' order, then the rows past the last group (`zero`: no group owns
-// them, y is 0 there).  Every wave looks for itself, 64 groups at a time: a
+// them, y is 0 there).  Every wave looks for itself: a
 // lane has a group, a scan its first tile.  Where starts do not begin with 0,
 // fall, or pass m, no row has a group (and flags[0] is set).
 struct Fp8Tile {
@@ -223,41 +223,66 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
 }
 __device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+// 256 groups from `base` on, four a lane: their first rows, rows, and tiles up to
+// and with each, `before` tiles being ahead of them.
 template <int SHIFT>
-__device__ __forceinline__ Fp8Tile fp8_tile(const Fp8Call& c, int t) {
-    constexpr int ROWS = 1 << SHIFT;
-    if (!c.starts) return {0, t << SHIFT, min(ROWS, c.m - (t << SHIFT)), false};
-    const int lane = __lane_id(), E = c.experts;
-    Fp8Tile r = {0, 0, 0, true};
-    int before = 0;
-    bool bad = c.starts[0] != 0;
-    for (int base = 0; base <= E; base += 256) {
-        int at[4], next[4];  // loads of 256 groups together
+struct Fp8Groups {
+    int at[4], count[4], upto[4];
+    // returns the tiles up to the last of them
+    __device__ __forceinline__ int read(const Fp8Call& c, int base, int before, bool& bad) {
+        int next[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int e = base + 64 * i + lane;
-            at[i] = e <= E ? c.starts[e] : c.m;
-            next[i] = e < E ? c.starts[e + 1] : c.m;
+            const int e = base + 64 * i + (int)__lane_id();
+            at[i] = e <= c.experts ? c.starts[e] : c.m;
+            next[i] = e < c.experts ? c.starts[e + 1] : c.m;
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            if (base + 64 * i > E) break;
-            const int count = next[i] - at[i];
-            bad |= at[i] < 0 || at[i] > c.m || count < 0;
-            const int tiles = (int)(((uint32_t)count + ROWS - 1) >> SHIFT);
-            const int upto = before + wave_scan(tiles);
-            const uint64_t hit = __ballot(t < upto && t >= upto - tiles);
-            if (hit) {
-                const int j = __builtin_ctzll(hit), g = base + 64 * i + j;
-                const int in = (t - (lane_value(upto, j) - lane_value(tiles, j))) << SHIFT;
-                r = {g, lane_value(at[i], j) + in, min(ROWS, lane_value(count, j) - in), g == E};
-            }
-            before = lane_value(upto, 63);
+            count[i] = next[i] - at[i];
+            upto[i] = before;
+            if (base + 64 * i > c.experts) continue;
+            bad |= at[i] < 0 || at[i] > c.m || count[i] < 0;
+            upto[i] += wave_scan(tiles(i));
+            before = lane_value(upto[i], 63);
         }
+        return before;
     }
+    __device__ __forceinline__ int tiles(int i) const { return (int)(((uint32_t)count[i] + (1 << SHIFT) - 1) >> SHIFT); }
+};
+// The tile of a workgroup: place(tiles that there are) says which one, -1: none.
+template <int SHIFT, class Place>
+__device__ __forceinline__ Fp8Tile fp8_tile(const Fp8Call& c, Place place) {
+    constexpr int ROWS = 1 << SHIFT;
+    const int E = c.experts, cut = (int)(((uint32_t)c.m + ROWS - 1) >> SHIFT);  // tiles of rows that no group cuts
+    if (!c.starts) {
+        const int t = place(cut);
+        return {0, t << SHIFT, t < 0 ? 0 : min(ROWS, c.m - (t << SHIFT)), false};
+    }
+    Fp8Groups<SHIFT> g;
+    int tiles = 0;
+    bool bad = c.starts[0] != 0;
+    for (int base = 0; base <= E; base += 256) tiles = g.read(c, base, tiles, bad);
     if (__ballot(bad)) {
-        r = {0, t << SHIFT, min(ROWS, c.m - (t << SHIFT)), true};
+        const int t = place(cut);
         if (t == 0) c.flags[0] = 1;
+        return {0, t << SHIFT, t < 0 ? 0 : min(ROWS, c.m - (t << SHIFT)), true};
+    }
+    const int t = place(tiles);
+    Fp8Tile r = {0, 0, 0, true};
+    if (t < 0 || t >= tiles) return r;
+    int before = 0;
+    for (int base = 0; base <= E; base += 256) {
+        if (E >= 256) before = g.read(c, base, before, bad);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint64_t hit = __ballot(t < g.upto[i] && t >= g.upto[i] - g.tiles(i));
+            if (hit) {  // the lanes past the last group have no tiles
+                const int j = __builtin_ctzll(hit), e = base + 64 * i + j;
+                const int in = (t - (lane_value(g.upto[i], j) - lane_value(g.tiles(i), j))) << SHIFT;
+                r = {e, lane_value(g.at[i], j) + in, min(ROWS, lane_value(g.count[i], j) - in), e == E};
+            }
+        }
     }
     return r;
 }

@@ -29,7 +29,7 @@ __global__ __launch_bounds__(64 * W) void k_fp8_few(const Fp8Call c, int nblocks
     extern __shared__ __align__(16) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r16 = lane & 15;
     const int t = blockIdx.x / nblocks, n0 = 16 * NT * (blockIdx.x - t * nblocks);
-    const Fp8Tile tile = fp8_tile<MT == 1 ? 4 : MT == 2 ? 5 : 6>(c, t);
+    const Fp8Tile tile = fp8_tile<MT == 1 ? 4 : MT == 2 ? 5 : 6>(c, [&](int) { return t; });
     if (tile.count <= 0) return;  // the same in all waves
     fp8_f4 acc[NT][MT];
 #pragma unroll

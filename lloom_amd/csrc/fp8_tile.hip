@@ -76,21 +76,35 @@ __device__ __forceinline__ v8i fp8_operand(const Fp8Row& r, int j) {
     return v8i{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
 }
 
+// Place of a workgroup among a grouped call's tiles: a run of them an XCD, walked
+// in groups of four, as tile_of walks another call's: what an XCD's workgroups
+// have in flight then shares rows of x and of the weight in its L2 (8192 tokens top
+// 8 of 64 experts, [2048, 2048]: 389 us in launch order, 377 so; smaller tiles have
+// fewer rows of one expert to share, (128, 128) 129 and 140).  t is -1 where none is
+// left.
+__device__ __forceinline__ void fp8_grouped_place(int tiles, int nbn, int& t, int& bn) {
+    const int all = tiles * nbn, each = all >> 3, more = all & 7;
+    const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
+    const int pid = xcd * each + min(xcd, more) + i;
+    const int per = 4 * nbn, group = pid / per, in = pid - group * per, size = min(tiles - 4 * group, 4);
+    const bool none = i >= each + (xcd < more ? 1 : 0);
+    t = none ? -1 : 4 * group + in % size;
+    bn = none ? 0 : in / size;
+}
+
 template <class C, bool EXACT, int YT>
 __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nbn) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c32 = lane & 31;
     const int wv = __builtin_amdgcn_readfirstlane(wave), wm = wv / C::WN, wn = wv % C::WN;
     int t, bn;
-    Fp8Tile tile;
-    if (c.starts) {
-        t = blockIdx.x / nbn, bn = blockIdx.x - t * nbn;
-        tile = fp8_tile<C::SHIFT>(c, t);
-        if (tile.count <= 0) return;
-    } else {
-        tile_of((c.m + C::BM - 1) / C::BM, nbn, t, bn);
-        tile = fp8_tile<C::SHIFT>(c, t);
-    }
+    const Fp8Tile tile = fp8_tile<C::SHIFT>(c, [&](int tiles) {
+        if (!c.starts) tile_of(tiles, nbn, t, bn);
+        else if (C::BM >= 256) fp8_grouped_place(tiles, nbn, t, bn);
+        else t = blockIdx.x / nbn, bn = blockIdx.x - t * nbn;
+        return t;
+    });
+    if (tile.count <= 0) return;
     const int n0 = bn * C::BN, steps = tile.zero ? 0 : c.kb;
 
     const uint8_t* wbase = c.w + ((int64_t)tile.group * c.n + n0) * c.k;
@@ -118,25 +132,26 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
 #pragma unroll
         for (int i = 0; i < C::XS_LOADS; i++) from.s[i] = s_from[(64 * ((wv + C::WAVES * i) % XS_PARTS) + lane) % C::BM];
     };
-    auto issue = [&](int s, int slot, const From& from) {
+    // loads lo .. hi - 1 of the wave's share of a stage
+    auto issue = [&](int s, int slot, const From& from, int lo, int hi) {
         const uint32_t st = lds0 + slot * C::STAGE, at = 128u * s;
         const bool past = (int)at + byte >= c.k;  // the last block's pieces past the end of the rows
 #pragma unroll
-        for (int i = 0; i < C::W_LOADS; i++) {
-            const uint32_t off = min((uint32_t)(row0 + 8 * C::WAVES * i), wlast) * (uint32_t)c.k + byte;
-            fp8_dma16(wbuf, past ? FP8_OUT : off, at, st + 1024 * (wv + C::WAVES * i));
-        }
-#pragma unroll
-        for (int i = 0; i < C::X_LOADS; i++) {
-            const int r = from.x[i];
-            fp8_dma16(xbuf, past || r < 0 ? FP8_OUT : (uint32_t)r * (uint32_t)c.x_stride + byte, at,
-                      st + C::W + 1024 * (wv + C::WAVES * i));
-        }
-#pragma unroll
-        for (int i = 0; i < C::XS_LOADS; i++) {
-            const int r = from.s[i];
-            fp8_dma4(sbuf, r < 0 ? FP8_OUT : (uint32_t)r * (uint32_t)c.xs_row * 4u,
-                     (uint32_t)s * (uint32_t)c.xs_block * 4u, st + C::W + C::X + 256 * ((wv + C::WAVES * i) % XS_PARTS));
+        for (int j = 0; j < C::DMA; j++) {
+            if (j < lo || j >= hi) continue;
+            if (j < C::X_LOADS) {
+                const int i = j, r = from.x[i];
+                fp8_dma16(xbuf, past || r < 0 ? FP8_OUT : (uint32_t)r * (uint32_t)c.x_stride + byte, at,
+                          st + C::W + 1024 * (wv + C::WAVES * i));
+            } else if (j < C::X_LOADS + C::XS_LOADS) {
+                const int i = j - C::X_LOADS, r = from.s[i];
+                fp8_dma4(sbuf, r < 0 ? FP8_OUT : (uint32_t)r * (uint32_t)c.xs_row * 4u,
+                         (uint32_t)s * (uint32_t)c.xs_block * 4u, st + C::W + C::X + 256 * ((wv + C::WAVES * i) % XS_PARTS));
+            } else {
+                const int i = j - C::X_LOADS - C::XS_LOADS;
+                const uint32_t off = min((uint32_t)(row0 + 8 * C::WAVES * i), wlast) * (uint32_t)c.k + byte;
+                fp8_dma16(wbuf, past ? FP8_OUT : off, at, st + 1024 * (wv + C::WAVES * i));
+            }
         }
     };
 
@@ -160,23 +175,29 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
     // Everything of a step's stage is read before its last weight rows are
     // multiplied: there the next stage has had S - 1 steps' time to land, a barrier
     // frees the slot for the one S steps on, and the next step's first operands
-    // are read under the products that are left.
+    // are read under the products that are left.  That one's loads are issued in
+    // parts between those products where a CU has one workgroup: a wave waits at
+    // each for its place in the queue (8192^3: all at once 550 us, 536 so; 2048
+    // tokens top 8 of 64 experts on (128, 128) tiles 136 and 143).
+    From from;
+    constexpr int PARTS = C::BM >= 256 ? 2 * C::MF : 1, PART = (C::DMA + PARTS - 1) / PARTS;
+    auto bring = [&](int s, int slot, int part) {
+        if (s + C::S < steps) issue(s + C::S, slot, from, part * PART, (part + 1) * PART);
+    };
     auto turn = [&](int s, int slot) {
-        From from;
         look(from);
         __builtin_amdgcn_sched_barrier(0);
         if (C::S > 2 && s + C::S - 1 < steps) fp8_landed<(C::S - 2) * C::DMA>();
         else fp8_landed<0>();
         __builtin_amdgcn_s_barrier();
-        if (s + C::S < steps) issue(s + C::S, slot, from);
+        bring(s, slot, 0);
         __builtin_amdgcn_sched_barrier(0);
     };
     if (steps) {
-        From from;
         look(from);
 #pragma unroll
         for (int i = 0; i < C::S; i++)
-            if (i < steps) issue(i, i, from);
+            if (i < steps) issue(i, i, from, 0, C::DMA);
         if (steps >= C::S) fp8_landed<(C::S - 1) * C::DMA>();
         else fp8_landed<0>();
         __builtin_amdgcn_s_barrier();
@@ -239,6 +260,9 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
                         if (b == C::NF - 2 && a == 0) {
                             fp8_here(d);
                             turn(s, slot);
+                        } else if (b >= C::NF - 2) {
+                            fp8_here(d);
+                            bring(s, slot, (b - C::NF + 2) * C::MF + a);
                         }
                         if (b == C::NF - 1) x[a] = read_x(after, a), next[a] = read_s(after, a);
 #pragma unroll
