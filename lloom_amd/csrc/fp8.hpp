@@ -49,8 +49,8 @@ hipError_t launch_expert_plan(const int* ids, int64_t planes, int topk, int expe
 // 4096] 14.8 against 18.9 us, of [8192, 8192] 34.9 / 35.6, 192 of [8192, 2048] 22 /
 // 12.5.  Grouped, us with 4, 8 and 12 rows an expert on average: [128, 1536, 2048]
 // 67, 79, 88 against 67, 72, 75, [128, 2048, 768] 41, 50, 55 / 41, 46, 49.
-inline bool fp8_few_rows(const Fp8Call& c) {
-    return c.starts ? c.m <= 4 * (int64_t)c.experts : (int64_t)c.m * c.n <= 96 * 8192 || c.m <= 16;
+inline bool fp8_few_rows(int64_t rows, int64_t n, int64_t experts, bool grouped) {
+    return grouped ? rows <= 4 * experts : rows * n <= 96 * 8192 || rows <= 16;
 }
 // fp8_few.hip: x E4M3, or any type where fp8_few_fuses (it is brought into 8 bits
 // by each workgroup).

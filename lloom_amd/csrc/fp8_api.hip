@@ -65,10 +65,14 @@ int check_product(const char* what, const void* w, const float* ws, int64_t expe
     return LLOOM_HIP_OK;
 }
 
-// A grid's workgroups, as a launch of 512 threads counts them.
-int check_grid(const char* what, int64_t rows, int64_t n, int64_t experts) {
-    const int64_t tiles = rows / 16 + (experts < rows ? experts : rows) + 1;
-    if (tiles * ((n + 15) / 16) < ((int64_t)1 << 23)) return LLOOM_HIP_OK;
+// A launch has fewer than 2^32 threads: fp8_few.hip's at most 512 for 16 rows of x
+// and of the weight, fp8_tile.hip's 128 for 32 rows of x and 128 of the weight.
+int check_grid(const char* what, int64_t rows, int64_t n, int64_t experts, bool grouped) {
+    const int64_t more = experts < rows ? experts : rows;
+    const bool fits = fp8_few_rows(rows, n, experts, grouped)
+                          ? (rows / 16 + more + 1) * ((n + 15) / 16) < ((int64_t)1 << 23)
+                          : (rows / 32 + more + 1) * ((n + 127) / 128) < ((int64_t)1 << 25);
+    if (fits) return LLOOM_HIP_OK;
     return fail(LLOOM_HIP_ESHAPE, "%s: %lld rows by n %lld", what, (long long)rows, (long long)n);
 }
 
@@ -84,18 +88,24 @@ XCopy x_copy(int x_type, int64_t rows, int64_t x_rows, int64_t k, bool grouped) 
             q + (size_t)x_rows * ((k + 127) / 128) * sizeof(float)};
 }
 
-// The kernels' 32-bit offsets: of a tile's rows of x, or of all rows that may be
-// gathered, and of their scales.
-int check_offsets(const char* what, int64_t rows, int64_t row_bytes, int64_t xs_row, int64_t xs_block, int64_t k) {
-    const int64_t most = (int64_t)1 << 31;
-    if (rows * row_bytes + k < most && (rows * xs_row + (k + 127) / 128 * xs_block) * 4 < most) return LLOOM_HIP_OK;
-    return fail(LLOOM_HIP_ESHAPE, "%s: %lld rows of x, %lld bytes apart, are past 2^31 bytes (or their scales are)", what,
-                (long long)rows, (long long)row_bytes);
+// The kernels' 32-bit offsets: of a tile's rows of e4m3 x, or of all rows that may
+// be gathered, and of their scales.
+int check_offsets(const char* what, int x_type, int64_t rows, int64_t x_rows, int64_t stride, int64_t xs_row,
+                  int64_t xs_block, int64_t k, bool grouped, bool gathered) {
+    if (x_type != T_E4M3) {
+        if (!x_copy(x_type, rows, x_rows, k, grouped).needed) return LLOOM_HIP_OK;
+        stride = k, xs_row = 1, xs_block = x_rows;
+    }
+    const int64_t most = (int64_t)1 << 31, reach = gathered ? x_rows : 256;
+    if (stride < most && xs_row < most && xs_block < most && reach * stride + k < most &&
+        (reach * xs_row + (k + 127) / 128 * xs_block) * 4 < most)
+        return LLOOM_HIP_OK;
+    return fail(LLOOM_HIP_ESHAPE, "%s: %lld rows of x, %lld bytes apart, or their scales, are past 2^31 bytes", what,
+                (long long)reach, (long long)stride);
 }
 
 int run_product(lloom_hip_ctx* ctx, int x_type, Fp8Call c, hipStream_t s) {
-    const bool grouped = c.starts != nullptr;
-    const XCopy copy = x_copy(x_type, c.m, c.x_rows, c.k, grouped);
+    const XCopy copy = x_copy(x_type, c.m, c.x_rows, c.k, c.starts != nullptr);
     std::unique_lock<std::mutex> lock(ctx->mu, std::defer_lock);
     if (copy.needed && c.x_rows) {
         lock.lock();
@@ -104,12 +114,9 @@ int run_product(lloom_hip_ctx* ctx, int x_type, Fp8Call c, hipStream_t s) {
         float* scales = (float*)((uint8_t*)ws + copy.scales_at);
         HIP_OK(launch_fp8_rows(x_type, c.x, c.x_stride, nullptr, 0, c.x_rows, c.k, ws, scales, c.x_rows, s));
         c.x = ws, c.x_stride = c.k, c.xs = scales, c.xs_row = 1, c.xs_block = c.x_rows;
-        x_type = T_E4M3;
     }
-    if (int rc = check_offsets(grouped ? "fp8_grouped_matmul" : "fp8_matmul", c.gather ? c.x_rows : 256,
-                               c.x_stride * type_bytes(x_type), c.xs_row, c.xs_block, c.k))
-        return rc;
-    if (fp8_few_rows(c)) HIP_OK(launch_fp8_few(x_type, c, s));
+    if (copy.needed) x_type = T_E4M3;
+    if (fp8_few_rows(c.m, c.n, c.experts, c.starts != nullptr)) HIP_OK(launch_fp8_few(x_type, c, s));
     else HIP_OK(launch_fp8_tile(c, s));
     return LLOOM_HIP_OK;
 }
@@ -181,7 +188,8 @@ int lloom_hip_fp8_matmul(lloom_hip_ctx* ctx, const void* w_dev, const float* w_s
     if (int rc = check_product("fp8_matmul", w_dev, w_scales_dev, 1, n, k, x_dev, x_dtype, x_stride, x_scales_dev, xs_row,
                                xs_block, m, y_dev, y_dtype))
         return rc;
-    if (int rc = check_grid("fp8_matmul", m, n, 1)) return rc;
+    if (int rc = check_offsets("fp8_matmul", x_dtype, m, m, x_stride, xs_row, xs_block, k, false, false)) return rc;
+    if (int rc = check_grid("fp8_matmul", m, n, 1, false)) return rc;
     if (m == 0) return LLOOM_HIP_OK;
     HIP_OK(hipSetDevice(ctx->device));
     const Fp8Call c = {(const uint8_t*)w_dev, w_scales_dev, x_dev, x_scales_dev, y_dev, nullptr, nullptr, nullptr,
@@ -204,7 +212,10 @@ int lloom_hip_fp8_grouped_matmul(lloom_hip_ctx* ctx, const void* w_dev, const fl
     if (rows > MAX_ROWS || y_rows > MAX_ROWS || (!gather_dev && x_rows < rows) || (!scatter_dev && y_rows < rows))
         return fail(LLOOM_HIP_ESHAPE, "fp8_grouped_matmul: %lld rows (at most %lld) of %lld into %lld", (long long)rows,
                     (long long)MAX_ROWS, (long long)x_rows, (long long)y_rows);
-    if (int rc = check_grid("fp8_grouped_matmul", rows, n, experts)) return rc;
+    if (int rc = check_offsets("fp8_grouped_matmul", x_dtype, rows, x_rows, x_stride, xs_row, xs_block, k, true,
+                               gather_dev != nullptr))
+        return rc;
+    if (int rc = check_grid("fp8_grouped_matmul", rows, n, experts, true)) return rc;
     if (rows == 0) return LLOOM_HIP_OK;
     HIP_OK(hipSetDevice(ctx->device));
     const Fp8Call c = {(const uint8_t*)w_dev, w_scales_dev, x_dev, x_scales_dev, y_dev, (const int*)starts_dev,
