@@ -167,6 +167,10 @@ def _out_dtype(x, x_scales, out_dtype, out, what):
     return d
 
 
+def _new(like, dtype, rows, n):
+    return like.new_empty((rows, n)) if like.dtype is dtype else torch.empty((rows, n), dtype=dtype, device=like.device)
+
+
 def _check_out(out, shape, dtype, i, what):
     if out.dtype is not dtype or out.shape != shape or not out.is_contiguous() or out.get_device() != i:
         raise LloomHipError(3, f"{what}: out {tuple(out.shape)} {out.dtype} on {out.device} does not fit the contiguous "
@@ -183,7 +187,9 @@ def fp8_matmul(x, weight, weight_scales, x_scales=None, out_dtype=None, out=None
     r, rows, stride, xs, s0, s1 = _x(x, x_scales, i, k, "fp8_matmul")
     d = _out_dtype(x, x_scales, out_dtype, out, "fp8_matmul")
     if out is None:
-        out = torch.empty((rows, n) if r is x else x.shape[:-1] + (n,), dtype=d, device=weight.device)
+        out = _new(r, d, rows, n)
+        if len(x.shape) != 2:
+            out = out.view(x.shape[:-1] + (n,))
     else:
         _check_out(out, x.shape[:-1] + (n,), d, i, "fp8_matmul")
     rc = lib().lloom_hip_fp8_matmul(ctx, weight.data_ptr(), weight_scales.data_ptr(), n, k, r.data_ptr(), _IDS[r.dtype],
@@ -243,7 +249,7 @@ def fp8_grouped_matmul(x, weight, weight_scales, starts, x_scales=None, gather=N
     d = _out_dtype(x, x_scales, out_dtype, out, what)
     y_rows = rows
     if out is None:
-        out = torch.empty((rows, n), dtype=d, device=weight.device)
+        out = _new(r, d, rows, n)
     else:
         if scatter is not None and out.dim() == 2:
             y_rows = max(rows, out.shape[0])
