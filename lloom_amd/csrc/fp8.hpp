@@ -45,12 +45,12 @@ hipError_t launch_fp8_weights(int type, const void* w, int64_t planes, int64_t n
 hipError_t launch_expert_plan(const int* ids, int64_t planes, int topk, int experts, int* starts, int* sorted,
                               int* tokens, int* flags, hipStream_t s);
 // Whether fp8_few.hip serves a call (else fp8_tile.hip).  Its workgroups' tiles
-// meet no other's, so it keeps all CUs busy with small outputs: 96 rows of [4096,
-// 4096] 14.8 against 18.9 us, of [8192, 8192] 34.9 / 35.6, 192 of [8192, 2048] 22 /
-// 12.5.  Grouped, us with 4, 8 and 12 rows an expert on average: [128, 1536, 2048]
+// meet no other's, so it keeps all CUs busy with small outputs: 128 rows of [4096,
+// 4096] 15.1 against 19.0 us, 192 26 / 19, 64 rows of [8192, 2048] 9.7 / 11.1, 96 12.7
+// / 11.6, 192 22 / 12.5.  Grouped, us with 4, 8 and 12 rows an expert on average: [128, 1536, 2048]
 // 67, 79, 88 against 67, 72, 75, [128, 2048, 768] 41, 50, 55 / 41, 46, 49.
 inline bool fp8_few_rows(int64_t rows, int64_t n, int64_t experts, bool grouped) {
-    return grouped ? rows <= 4 * experts : rows * n <= 96 * 8192 || rows <= 16;
+    return grouped ? rows <= 4 * experts : rows * n <= 128 * 4096 || rows <= 16;
 }
 // fp8_few.hip: x E4M3, or any type where fp8_few_fuses (it is brought into 8 bits
 // by each workgroup).

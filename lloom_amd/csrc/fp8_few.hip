@@ -29,7 +29,7 @@ __global__ __launch_bounds__(64 * W) void k_fp8_few(const Fp8Call c, int nblocks
     extern __shared__ __align__(16) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r16 = lane & 15;
     const int t = blockIdx.x / nblocks, n0 = 16 * NT * (blockIdx.x - t * nblocks);
-    const Fp8Tile tile = fp8_tile<MT == 1 ? 4 : MT == 2 ? 5 : 6>(c, [&](int) { return t; });
+    const Fp8Tile tile = fp8_tile<MT == 1 ? 4 : 5>(c, [&](int) { return t; });
     if (tile.count <= 0) return;  // the same in all waves
     fp8_f4 acc[NT][MT];
 #pragma unroll
@@ -211,7 +211,6 @@ static hipError_t few_with(const Fp8Call& c, hipStream_t s) {
     if constexpr (XT == T_E4M3) {
         if (!c.starts && c.m > 16) {
             auto enough = [&](int rows, int cols) { return (int64_t)((c.m + rows - 1) / rows) * ((c.n + cols - 1) / cols) >= 200; };
-            if (c.m > 32 && enough(64, 64)) return few_of<XT, 4, 4, 4, 1>(c, s);
             if (enough(32, 64)) return few_of<XT, 4, 2, 4, 1>(c, s);
             if (enough(32, 32)) return few_of<XT, 4, 2, 2, 1>(c, s);
             return few_of<XT, 4, 1, 2, 2>(c, s);

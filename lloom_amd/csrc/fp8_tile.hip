@@ -8,17 +8,31 @@ namespace lloom {
 
 #pragma clang fp contract(off)
 
-// A workgroup has BM rows of x and BN of the weight, WM x WN waves with MF x NF
-// tiles of 32 x 32 each; k moves a block (128) a step through two LDS stages,
+// A workgroup has BM rows of x and BN of the weight, WM x WN waves with 32 MF x 32
+// NF of them each; k moves a block (128) a step through S LDS stages,
 //   W [BN][128] e4m3, piece p (16 bytes) of row r at p ^ swizzle(r)
 //   X [BM][128] likewise
 //   scales [BM] f32 of the block's rows
 // every byte by buffer_load .. lds: what is out of the operands (rows past a
 // tile's, a last block's bytes past k) has an offset out of the buffer's range
-// and arrives as zeros.  Lane (h, c) of a wave takes pieces 2 i + h, i < 4, of row
-// c of both operands: which bytes meet in which instruction does not matter.
-// The weight is the matrix instructions' A: a lane's 16 sums are of one row of x,
-// so one factor (its scale times the weight block's) serves them all.
+// and arrives as zeros.  Lane (g, c) of a wave takes the same pieces of row c of
+// both operands; which bytes meet in which instruction does not matter.  The
+// weight is the matrix instructions' A: a lane's sums are of one row of x, so one
+// factor (its scale times the weight block's) serves them all.
+//
+// Into F16 and BF16 a block of a 16 x 16 tile is one v_mfma_f32_16x16x128_f8f6f4.
+// It adds groups of eight products with 14 bits from the group's largest on (what
+// is under 2^-13 of that is cut), the groups and the blocks in f32: 1.5e-5 of the
+// result in the 2-norm for normal values, where F16's own rounding is 2.1e-4 and
+// BF16's 1.7e-3.  Into F32 (EXACT) the numbers go as halves to v_mfma_f32_32x32x16_
+// f16, whose products are exact and whose sums are f32, at half the rate (8192^3:
+// 527 us and 1030).  Tiles of 32 x 32 for the former: 543, their sums waiting for
+// two chained instructions.
+//
+// 8192^3 into BF16 is 2090 TFLOP/s; without the loads 424 us, without LDS and
+// barriers too 382, with zeros for data 493, 354 and 301: the clock falls with the
+// data's bits, and the loads cost a fifth, nearly all of it though every tile come
+// from one place of the L2 (490).
 template <int WM_, int WN_, int MF_, int NF_, int S_>
 struct Fp8Cfg {
     static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_, S = S_;
@@ -58,7 +72,10 @@ __device__ __forceinline__ void fp8_landed() {
 }
 // Keeps a tile's sums in the place of the program where they are written: the
 // compiler would gather a step's at its end, and spill.
-__device__ __forceinline__ void fp8_here(fp8_f16v& v) { asm volatile("" : "+v"(v)); }
+template <class V>
+__device__ __forceinline__ void fp8_here(V& v) {
+    asm volatile("" : "+v"(v));
+}
 
 // A lane's 64 bytes of a row of a stage.
 struct Fp8Row {
@@ -71,8 +88,10 @@ __device__ __forceinline__ Fp8Row fp8_read(const uint8_t* rows, int row, int h) 
     for (int i = 0; i < 4; i++) r.p[i] = *(const uint4*)(rows + (at ^ 32 * i));
     return r;
 }
-__device__ __forceinline__ v8i fp8_operand(const Fp8Row& r, int j) {
-    const uint4 a = r.p[2 * j], b = r.p[2 * j + 1];
+// The same for tiles of 16 x 16: lane (g, c) takes pieces g and g + 4.
+__device__ __forceinline__ v8i fp8_read16(const uint8_t* rows, int row, int g) {
+    const int at = row * 128 + 16 * (g ^ fp8_swizzle(row));
+    const uint4 a = *(const uint4*)(rows + at), b = *(const uint4*)(rows + (at ^ 64));
     return v8i{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
 }
 
@@ -92,10 +111,19 @@ __device__ __forceinline__ void fp8_grouped_place(int tiles, int nbn, int& t, in
     bn = none ? 0 : in / size;
 }
 
+template <bool EXACT>
+struct Fp8Sums {
+    typedef fp8_f16v V;
+};
+template <>
+struct Fp8Sums<false> {
+    typedef fp8_f4 V;
+};
+
 template <class C, bool EXACT, int YT>
 __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nbn) {
     extern __shared__ __align__(16) uint8_t smem[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c32 = lane & 31;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wv = __builtin_amdgcn_readfirstlane(wave), wm = wv / C::WN, wn = wv % C::WN;
     int t, bn;
     const Fp8Tile tile = fp8_tile<C::SHIFT>(c, [&](int tiles) {
@@ -155,11 +183,15 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
         }
     };
 
-    fp8_f16v acc[C::NF][C::MF];
+    // tiles of 32 x 32 (EXACT) or 16 x 16
+    constexpr int T = EXACT ? 32 : 16, MT = C::MF * 32 / T, NT = C::NF * 32 / T;
+    typedef typename Fp8Sums<EXACT>::V Sums;
+    const int ct = lane % T, ht = lane / T;
+    Sums acc[NT][MT];
 #pragma unroll
-    for (int b = 0; b < C::NF; b++)
+    for (int b = 0; b < NT; b++)
 #pragma unroll
-        for (int a = 0; a < C::MF; a++) acc[b][a] = fp8_f16v{};
+        for (int a = 0; a < MT; a++) acc[b][a] = Sums{};
 
     const float* ws = c.ws + ((int64_t)tile.group * c.nb + min((n0 + wn * 32 * C::NF) >> 7, c.nb - 1)) * c.kb;
     float wscale = 0.0f;  // lane l: of block 64 i + l
@@ -167,10 +199,8 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
         if ((s & 63) == 0) wscale = fp8_load_now(ws + min(s + lane, c.kb - 1));
         return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wscale), s & 63));
     };
-    auto read_w = [&](int slot, int b) { return fp8_read(smem + slot * C::STAGE, (wn * C::NF + b) * 32 + c32, h); };
-    auto read_x = [&](int slot, int a) { return fp8_read(smem + slot * C::STAGE + C::W, (wm * C::MF + a) * 32 + c32, h); };
     auto read_s = [&](int slot, int a) {
-        return *(const float*)(smem + slot * C::STAGE + C::W + C::X + 4 * ((wm * C::MF + a) * 32 + c32));
+        return *(const float*)(smem + slot * C::STAGE + C::W + C::X + 4 * ((wm * MT + a) * T + ct));
     };
     // Everything of a step's stage is read before its last weight rows are
     // multiplied: there the next stage has had S - 1 steps' time to land, a barrier
@@ -180,7 +210,7 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
     // each for its place in the queue (8192^3: all at once 550 us, 536 so; 2048
     // tokens top 8 of 64 experts on (128, 128) tiles 136 and 143).
     From from;
-    constexpr int PARTS = C::BM >= 256 ? 2 * C::MF : 1, PART = (C::DMA + PARTS - 1) / PARTS;
+    constexpr int PARTS = C::BM >= 256 ? C::DMA : 1, PART = (C::DMA + PARTS - 1) / PARTS;
     auto bring = [&](int s, int slot, int part) {
         if (s + C::S < steps) issue(s + C::S, slot, from, part * PART, (part + 1) * PART);
     };
@@ -202,80 +232,105 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
         else fp8_landed<0>();
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        Fp8Row x[C::MF], w = read_w(0, 0);
-        float f[C::MF];
+        float f[MT], next[MT];
 #pragma unroll
-        for (int a = 0; a < C::MF; a++) x[a] = read_x(0, a), f[a] = read_s(0, a);
+        for (int a = 0; a < MT; a++) f[a] = read_s(0, a);
         int slot = 0;
-        for (int s = 0; s < steps; s++) {
-            const int after = slot + 1 < C::S ? slot + 1 : 0;
-            const float sw = weight_scale(s);
+        if constexpr (EXACT) {
+            auto read_w = [&](int slot, int b) { return fp8_read(smem + slot * C::STAGE, (wn * NT + b) * 32 + ct, ht); };
+            auto read_x = [&](int slot, int a) { return fp8_read(smem + slot * C::STAGE + C::W, (wm * MT + a) * 32 + ct, ht); };
+            Fp8Row x[MT], w = read_w(0, 0);
 #pragma unroll
-            for (int a = 0; a < C::MF; a++) f[a] *= sw;
-            float next[C::MF];
-            fp8_h8 xh[EXACT ? C::MF : 1][8];
-            if constexpr (EXACT) {
+            for (int a = 0; a < MT; a++) x[a] = read_x(0, a);
+            for (int s = 0; s < steps; s++) {
+                const int after = slot + 1 < C::S ? slot + 1 : 0;
+                const float sw = weight_scale(s);
+                fp8_h8 xh[MT][8];
 #pragma unroll
-                for (int a = 0; a < C::MF; a++)
+                for (int a = 0; a < MT; a++) {
+                    f[a] *= sw;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         xh[a][2 * i] = fp8_halves(x[a].p[i].x, x[a].p[i].y);
                         xh[a][2 * i + 1] = fp8_halves(x[a].p[i].z, x[a].p[i].w);
                     }
-            }
+                }
 #pragma unroll
-            for (int b = 0; b < C::NF; b++) {
-                const Fp8Row ahead = b < C::NF - 1 ? read_w(slot, b + 1) : read_w(after, 0);
-                if constexpr (EXACT) {
-                    fp8_f16v d[C::MF];
+                for (int b = 0; b < NT; b++) {
+                    const Fp8Row ahead = b < NT - 1 ? read_w(slot, b + 1) : read_w(after, 0);
+                    fp8_f16v d[MT];
 #pragma unroll
-                    for (int a = 0; a < C::MF; a++) d[a] = fp8_f16v{};
+                    for (int a = 0; a < MT; a++) d[a] = fp8_f16v{};
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const fp8_h8 w0 = fp8_halves(w.p[i].x, w.p[i].y), w1 = fp8_halves(w.p[i].z, w.p[i].w);
 #pragma unroll
-                        for (int a = 0; a < C::MF; a++) {
+                        for (int a = 0; a < MT; a++) {
                             d[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w0, xh[a][2 * i], d[a], 0, 0, 0);
                             d[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w1, xh[a][2 * i + 1], d[a], 0, 0, 0);
                         }
                     }
-                    if (b == C::NF - 2) {
-                        fp8_here(d[C::MF - 1]);
+                    if (b == NT - 2) {
+                        fp8_here(d[MT - 1]);
                         turn(s, slot);
                     }
 #pragma unroll
-                    for (int a = 0; a < C::MF; a++) {
-                        if (b == C::NF - 1) x[a] = read_x(after, a), next[a] = read_s(after, a);
+                    for (int a = 0; a < MT; a++) {
+                        if (b == NT - 1) x[a] = read_x(after, a), next[a] = read_s(after, a);
 #pragma unroll
                         for (int r = 0; r < 16; r++) acc[b][a][r] = __builtin_fmaf(d[a][r], f[a], acc[b][a][r]);
                         fp8_here(acc[b][a]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
-                } else {
-#pragma unroll
-                    for (int a = 0; a < C::MF; a++) {
-                        fp8_f16v d = {};
-                        d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp8_operand(w, 0), fp8_operand(x[a], 0), d, 0, 0, 0, 0, 0, 0);
-                        d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp8_operand(w, 1), fp8_operand(x[a], 1), d, 0, 0, 0, 0, 0, 0);
-                        if (b == C::NF - 2 && a == 0) {
-                            fp8_here(d);
-                            turn(s, slot);
-                        } else if (b >= C::NF - 2) {
-                            fp8_here(d);
-                            bring(s, slot, (b - C::NF + 2) * C::MF + a);
-                        }
-                        if (b == C::NF - 1) x[a] = read_x(after, a), next[a] = read_s(after, a);
-#pragma unroll
-                        for (int r = 0; r < 16; r++) acc[b][a][r] = __builtin_fmaf(d[r], f[a], acc[b][a][r]);
-                        fp8_here(acc[b][a]);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
+                    w = ahead;
                 }
-                w = ahead;
-            }
 #pragma unroll
-            for (int a = 0; a < C::MF; a++) f[a] = next[a];
-            slot = after;
+                for (int a = 0; a < MT; a++) f[a] = next[a];
+                slot = after;
+            }
+        } else {
+            // a wave's tiles in turn, the sums of the one LAG before brought home
+            // under a tile's products; weight rows are read two tiles' rows ahead
+            constexpr int LAG = 2, TILES = NT * MT, TURN = (NT - 3) * MT;
+            auto read_w = [&](int slot, int b) { return fp8_read16(smem + slot * C::STAGE, (wn * NT + b) * 16 + ct, ht); };
+            auto read_x = [&](int slot, int a) { return fp8_read16(smem + slot * C::STAGE + C::W, (wm * MT + a) * 16 + ct, ht); };
+            v8i x[MT], w[3] = {read_w(0, 0), read_w(0, 1), v8i{}};
+#pragma unroll
+            for (int a = 0; a < MT; a++) x[a] = read_x(0, a);
+            for (int s = 0; s < steps; s++) {
+                const int after = slot + 1 < C::S ? slot + 1 : 0;
+                const float sw = weight_scale(s);
+#pragma unroll
+                for (int a = 0; a < MT; a++) f[a] *= sw;
+                fp8_f4 d[LAG + 1];
+#pragma unroll
+                for (int t = 0; t < TILES + LAG; t++) {
+                    const int b = t / MT, a = t % MT;
+                    if (t < TILES) {
+                        if (a == 0) w[2] = b + 2 < NT ? read_w(slot, b + 2) : read_w(after, b + 2 - NT);
+                        d[t % (LAG + 1)] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[0], x[a], fp8_f4{}, 0, 0, 0, 0, 0, 0);
+                        if (t == TURN) {
+                            fp8_here(d[t % (LAG + 1)]);
+                            turn(s, slot);
+                        } else if (C::BM >= 256 && t > TURN && t - TURN < PARTS) {
+                            bring(s, slot, t - TURN);
+                        }
+                        if (b == NT - 1) x[a] = read_x(after, a), next[a] = read_s(after, a);
+                        if (a == MT - 1) w[0] = w[1], w[1] = w[2];
+                    }
+                    if (t >= LAG) {
+                        const int u = t - LAG;
+                        fp8_f4& v = acc[u / MT][u % MT];
+#pragma unroll
+                        for (int r = 0; r < 4; r++) v[r] = __builtin_fmaf(d[u % (LAG + 1)][r], f[u % MT], v[r]);
+                        fp8_here(v);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int a = 0; a < MT; a++) f[a] = next[a];
+                slot = after;
+            }
         }
     }
     // every wave has read its last operands before y passes through the ring
@@ -290,18 +345,21 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
 #pragma unroll
     for (int a = 0; a < C::MF; a++) {
 #pragma unroll
-        for (int b = 0; b < C::NF; b++)
+        for (int b = 0; b < NT; b++)
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                uint8_t* p = part + c32 * C::PITCH + SIZE * (32 * b + 2 * r + 4 * h);
-                if constexpr (YT == T_F32) {
-                    *(float4*)p = make_float4(acc[b][a][r], acc[b][a][r + 1], acc[b][a][r + 2], acc[b][a][r + 3]);
-                } else {
-                    *(uint2*)p = make_uint2(
-                        fp8_half_bits<YT>(acc[b][a][r]) | (uint32_t)fp8_half_bits<YT>(acc[b][a][r + 1]) << 16,
-                        fp8_half_bits<YT>(acc[b][a][r + 2]) | (uint32_t)fp8_half_bits<YT>(acc[b][a][r + 3]) << 16);
+            for (int q = 0; q < MT / C::MF; q++)
+#pragma unroll
+                for (int r = 0; r < T * T / 64; r += 4) {
+                    const Sums& v = acc[b][a * (MT / C::MF) + q];
+                    uint8_t* p = part + (T * q + ct) * C::PITCH + SIZE * (T * b + 2 * r + 4 * ht);
+                    if constexpr (YT == T_F32) {
+                        *(float4*)p = make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
+                    } else {
+                        *(uint2*)p =
+                            make_uint2(fp8_half_bits<YT>(v[r]) | (uint32_t)fp8_half_bits<YT>(v[r + 1]) << 16,
+                                       fp8_half_bits<YT>(v[r + 2]) | (uint32_t)fp8_half_bits<YT>(v[r + 3]) << 16);
+                    }
                 }
-            }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
         for (int i = 0; i < 32; i += ROWS) {
