@@ -50,10 +50,10 @@ hipError_t launch_expert_plan(const int* ids, int64_t planes, int topk, int expe
 // / 11.6, 192 22 / 12.5.  Grouped, us with 4, 8 and 12 rows an expert on average: [128, 1536, 2048]
 // 67, 79, 88 against 67, 72, 75, [128, 2048, 768] 41, 50, 55 / 41, 46, 49.
 inline bool fp8_few_rows(int64_t rows, int64_t n, int64_t experts, bool grouped) {
-    return grouped ? rows <= 4 * experts : rows * n <= 128 * 4096 || rows <= 16;
+    return rows <= 16 || (grouped ? rows <= 4 * experts : rows * n <= 128 * 4096);
 }
 // fp8_few.hip: x E4M3, or any type where fp8_few_fuses (it is brought into 8 bits
-// by each workgroup).
+// by each workgroup; only calls of up to 16 rows, which are all few).
 bool fp8_few_fuses(int x_type, int64_t rows, int64_t k, bool grouped);
 hipError_t launch_fp8_few(int x_type, const Fp8Call& c, hipStream_t s);
 // fp8_tile.hip: x E4M3.

@@ -33,6 +33,8 @@ int check_rows(const char* what, int type, const void* x, int64_t stride, int64_
     if (rows < 0 || rows > MAX_ROWS)
         return fail(rows < 0 ? LLOOM_HIP_EINVAL : LLOOM_HIP_ESHAPE, "%s: %lld rows (at most %lld)", what, (long long)rows,
                     (long long)MAX_ROWS);
+    if (rows * k > ((int64_t)1 << 36))  // a launch's threads, 8 values each
+        return fail(LLOOM_HIP_ESHAPE, "%s: %lld rows of %lld", what, (long long)rows, (long long)k);
     if (stride < k)
         return fail(LLOOM_HIP_ESHAPE, "%s: rows of %lld, %lld apart, overlap", what, (long long)k, (long long)stride);
     if ((uintptr_t)x % 16 || stride * type_bytes(type) % 16)

@@ -414,6 +414,7 @@ static hipError_t tile_with(const Fp8Call& c, hipStream_t s) {
 //     average: 71 / 73 / 82, 77 / 75 / 81, 92 / 85 / 94; of 64 [2048, 2048], 256 and
 //     1024: - / 141 / 128 and (256, 256) 134, - / 451 / 402 / 368
 hipError_t launch_fp8_tile(const Fp8Call& c, hipStream_t s) {
+    if (!c.xs && c.x_rows) return hipErrorInvalidValue;  // rows that are not in 8 bits
     auto count = [&](int rows, int cols) { return (int64_t)((c.m + rows - 1) / rows) * ((c.n + cols - 1) / cols); };
     const int64_t each = c.m / c.experts;
     if (c.y_type != T_F32 && (c.starts ? each >= 512 : count(256, 256) >= 200))

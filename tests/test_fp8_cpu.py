@@ -61,7 +61,7 @@ def refused(call, kw, code, name):
 ROWS = [(dict(ctx=None), EINVAL), (dict(q=None), EINVAL), (dict(s=None), EINVAL), (dict(dtype=12), EDTYPE),
         (dict(dtype=100), EDTYPE), (dict(k=0), EINVAL), (dict(k=-16), EINVAL), (dict(k=24), ESHAPE), (dict(k=1 << 23), ESHAPE),
         (dict(rows=-1), EINVAL), (dict(rows=(1 << 24) + 1, ss=1 << 25), ESHAPE), (dict(ss=3), ESHAPE), (dict(q=PTR + 4), EINVAL),
-        (dict(s=PTR + 2), EINVAL)]
+        (dict(s=PTR + 2), EINVAL), (dict(rows=1 << 24, ss=1 << 24, k=8192), ESHAPE)]
 
 
 @pytest.mark.parametrize("kw,code", ROWS + [(dict(x=None), EINVAL), (dict(stride=255), ESHAPE), (dict(stride=258), EINVAL),

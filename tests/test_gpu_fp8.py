@@ -244,6 +244,20 @@ def test_grouped(L, counts, extra, out):
     assert not y[order[i]].any() and not y2[i.cuda()].any()
 
 
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("counts", [[16], [13], [9, 7], [5, 0, 10], [17], [30, 3], [40, 1, 0]])
+def test_few_experts_of_few_rows(L, counts, act):
+    """Rows of every type around the 16 that workgroups bring into 8 bits themselves, for fewer experts than that counts."""
+    starts, rows, order = ragged(counts, 0, 3)
+    w, ws = weights(rows, len(counts), 80, 400)
+    x = normal(rows, rows, 400, dtype=act)
+    y = L.fp8_grouped_matmul(x.cuda(), w.cuda(), ws.cuda(), starts.cuda(), gather=order.int().cuda())
+    for e, c in enumerate(counts):
+        i = slice(int(starts[e]), int(starts[e]) + c)
+        if c:
+            check_product(y[i], x[order[i]], None, w[e], ws[e])
+
+
 # -------------------------------------------------------------------- plan --
 
 def plan_of(ids, experts):
