@@ -53,8 +53,8 @@ inline bool fp8_few_rows(int64_t rows, int64_t n, int64_t experts, bool grouped)
     return rows <= 16 || (grouped ? rows <= 4 * experts : rows * n <= 128 * 4096);
 }
 // fp8_few.hip: x E4M3, or any type where fp8_few_fuses (it is brought into 8 bits
-// by each workgroup; only calls of up to 16 rows, which are all few).
-bool fp8_few_fuses(int x_type, int64_t rows, int64_t k, bool grouped);
+// by each workgroup; only calls that fp8_few_rows gives to it).
+bool fp8_few_fuses(int x_type, int64_t rows, int64_t k, int64_t experts, bool grouped);
 hipError_t launch_fp8_few(int x_type, const Fp8Call& c, hipStream_t s);
 // fp8_tile.hip: x E4M3.
 hipError_t launch_fp8_tile(const Fp8Call& c, hipStream_t s);

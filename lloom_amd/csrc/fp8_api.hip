@@ -84,18 +84,18 @@ struct XCopy {
     bool needed;
     size_t scales_at, bytes;
 };
-XCopy x_copy(int x_type, int64_t rows, int64_t x_rows, int64_t k, bool grouped) {
+XCopy x_copy(int x_type, int64_t rows, int64_t x_rows, int64_t k, int64_t experts, bool grouped) {
     const size_t q = ((size_t)x_rows * k + 255) & ~(size_t)255;
-    return {x_type != T_E4M3 && !fp8_few_fuses(x_type, rows, k, grouped), q,
+    return {x_type != T_E4M3 && !fp8_few_fuses(x_type, rows, k, experts, grouped), q,
             q + (size_t)x_rows * ((k + 127) / 128) * sizeof(float)};
 }
 
 // The kernels' 32-bit offsets: of a tile's rows of e4m3 x, or of all rows that may
 // be gathered, and of their scales.
 int check_offsets(const char* what, int x_type, int64_t rows, int64_t x_rows, int64_t stride, int64_t xs_row,
-                  int64_t xs_block, int64_t k, bool grouped, bool gathered) {
+                  int64_t xs_block, int64_t k, int64_t experts, bool grouped, bool gathered) {
     if (x_type != T_E4M3) {
-        if (!x_copy(x_type, rows, x_rows, k, grouped).needed) return LLOOM_HIP_OK;
+        if (!x_copy(x_type, rows, x_rows, k, experts, grouped).needed) return LLOOM_HIP_OK;
         stride = k, xs_row = 1, xs_block = x_rows;
     }
     const int64_t most = (int64_t)1 << 31, reach = gathered ? x_rows : 256;
@@ -107,7 +107,7 @@ int check_offsets(const char* what, int x_type, int64_t rows, int64_t x_rows, in
 }
 
 int run_product(lloom_hip_ctx* ctx, int x_type, Fp8Call c, hipStream_t s) {
-    const XCopy copy = x_copy(x_type, c.m, c.x_rows, c.k, c.starts != nullptr);
+    const XCopy copy = x_copy(x_type, c.m, c.x_rows, c.k, c.experts, c.starts != nullptr);
     std::unique_lock<std::mutex> lock(ctx->mu, std::defer_lock);
     if (copy.needed && c.x_rows) {
         lock.lock();
@@ -190,7 +190,7 @@ int lloom_hip_fp8_matmul(lloom_hip_ctx* ctx, const void* w_dev, const float* w_s
     if (int rc = check_product("fp8_matmul", w_dev, w_scales_dev, 1, n, k, x_dev, x_dtype, x_stride, x_scales_dev, xs_row,
                                xs_block, m, y_dev, y_dtype))
         return rc;
-    if (int rc = check_offsets("fp8_matmul", x_dtype, m, m, x_stride, xs_row, xs_block, k, false, false)) return rc;
+    if (int rc = check_offsets("fp8_matmul", x_dtype, m, m, x_stride, xs_row, xs_block, k, 1, false, false)) return rc;
     if (int rc = check_grid("fp8_matmul", m, n, 1, false)) return rc;
     if (m == 0) return LLOOM_HIP_OK;
     HIP_OK(hipSetDevice(ctx->device));
@@ -214,7 +214,7 @@ int lloom_hip_fp8_grouped_matmul(lloom_hip_ctx* ctx, const void* w_dev, const fl
     if (rows > MAX_ROWS || y_rows > MAX_ROWS || (!gather_dev && x_rows < rows) || (!scatter_dev && y_rows < rows))
         return fail(LLOOM_HIP_ESHAPE, "fp8_grouped_matmul: %lld rows (at most %lld) of %lld into %lld", (long long)rows,
                     (long long)MAX_ROWS, (long long)x_rows, (long long)y_rows);
-    if (int rc = check_offsets("fp8_grouped_matmul", x_dtype, rows, x_rows, x_stride, xs_row, xs_block, k, true,
+    if (int rc = check_offsets("fp8_grouped_matmul", x_dtype, rows, x_rows, x_stride, xs_row, xs_block, k, experts, true,
                                gather_dev != nullptr))
         return rc;
     if (int rc = check_grid("fp8_grouped_matmul", rows, n, experts, true)) return rc;
@@ -254,7 +254,7 @@ int lloom_hip_fp8_workspace_bytes(int x_dtype, int64_t rows, int64_t x_rows, int
     if (rows > MAX_ROWS || x_rows > MAX_ROWS || experts > MOE_MAX_EXPERTS)
         return fail(LLOOM_HIP_ESHAPE, "fp8_workspace_bytes: %lld rows of %lld (at most %lld), %lld experts (at most %d)",
                     (long long)rows, (long long)x_rows, (long long)MAX_ROWS, (long long)experts, MOE_MAX_EXPERTS);
-    const XCopy copy = x_copy(x_dtype, rows, x_rows, k, experts > 0);
+    const XCopy copy = x_copy(x_dtype, rows, x_rows, k, experts, experts > 0);
     *bytes = copy.needed ? copy.bytes : 0;
     return LLOOM_HIP_OK;
 }

@@ -175,13 +175,15 @@ static int64_t few_lds(int64_t rows, int64_t k) {
     return (rows < 16 ? rows : 16) * (kb * 128 + 16 + kb * 4);
 }
 
-// One row of few blocks, and the few rows of a grouped call, each of which meets
-// few of them in a tile, are cheaper brought into 8 bits by every workgroup than
-// in a launch before (2.3 us): m = 1 on [6144, 2048] 5.9 against 8.0 us, 16 rows
-// 8.7 against 8.5, 32 tokens of 128 experts (16 rows at once in LDS) 84 against 58.
-bool fp8_few_fuses(int x_type, int64_t rows, int64_t k, bool grouped) {
-    if (x_type == T_E4M3 || rows > 16) return false;
-    return few_lds(rows, k) <= 65536 && (grouped || rows * ((k + 127) / 128) <= 64);
+// One row of few blocks, and a grouped call's rows where an expert has no more than
+// one on average, are cheaper brought into 8 bits by every workgroup than in a
+// launch before (2.3 us): one row of [6144, 2048] 5.9 against 8.0 us, 16 rows 8.7
+// against 8.5; top 8 of 128 experts, [1536, 2048], 4 tokens 19.8 / 21.0, 16 47.2 / 46.7,
+// 32 60 / 57, 64 77 / 68; 32 tokens top 2 of 64, [1024, 1024], 12.0 / 14.6.
+bool fp8_few_fuses(int x_type, int64_t rows, int64_t k, int64_t experts, bool grouped) {
+    if (x_type == T_E4M3) return false;
+    if (grouped) return (rows <= 16 || rows <= experts) && few_lds(rows, k) <= 40960;
+    return rows <= 16 && rows * ((k + 127) / 128) <= 64 && few_lds(rows, k) <= 65536;
 }
 
 template <int XT, int W, int MT, int NT, int D>
