@@ -4,18 +4,19 @@
 
 namespace lloom {
 
-// A workgroup an expert (the last one: planes of none), and each for itself: a
-// wave has a run of planes, counts in it those of smaller experts and those of
-// its own, and with the counts of all waves knows where its own go; a ballot
-// ranks a row of 64.  No atomics, so the order is the planes' own, and nothing
-// passes between workgroups; what it costs is that each reads all ids.  ROWS rows
-// of 64 are loaded at a time, the next ones under those in work, and what they hold
-// goes to a list in LDS first, so that stores have full waves.  ONCE: a run is no
-// longer than that and is kept for the second time.  128 experts, 256 planes 2.7 us,
-// 16384 4.8, 65536 12.7 (22.5 with a load at a time and stores of what each row
-// holds): the ids pass 256 KB a workgroup twice, and five VALU operations each.  Two
-// workgroups an expert, half of the second part each: 12.6, of 256 experts 18.6
-// against 13.0.
+// A workgroup an expert (the last one's also has the planes of none, which follow
+// its own: one workgroup more than CUs is 15 us for 10), and each for itself: a
+// wave has a run of planes, counts in it those of smaller experts, and lists its
+// own in LDS, a ballot ranking a row of 64; with the counts of all waves it knows
+// where its own go.  No atomics, so the order is the planes' own, and nothing passes
+// between workgroups; what it costs is that each reads all ids.  ROWS rows of 64
+// are loaded at a time, the next ones under those in work.  A wave whose list is
+// too short (over PLAN_LIST planes of one expert in its run) goes through its run
+// again, a list at a time.  128 experts, 256 planes 2.9 us (a launch), 16384 5.4,
+// 65536 10.2 (12.7 with a first time that only counts): 16 waves of a CU read and
+// rank 64 ids in about 18 clocks each, no more workgroups than CUs.
+constexpr int PLAN_LIST = 1024;
+
 // Keys of a wave's next rows from plane p on: an id, `none` for one of no expert,
 // -1 past the last.
 template <int ROWS>
@@ -30,62 +31,80 @@ __device__ __forceinline__ void plan_keys(const int* __restrict__ ids, int p, in
     }
 }
 
-template <int ROWS, bool ONCE>
+// Lists a wave's planes with key `mine` from rows of keys (the first of them plane
+// `off` of the run), `found` of them being there.
+template <int ROWS>
+__device__ __forceinline__ void plan_list(const uint32_t (&key)[ROWS], uint32_t mine, int off, uint16_t* list, int& found) {
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+        const uint64_t m = __ballot(key[i] == mine);
+        const int at = found + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+        if (key[i] == mine && at < PLAN_LIST) list[at] = (uint16_t)(off + 64 * i + (int)__lane_id());
+        found += __builtin_popcountll(m);
+    }
+}
+
+template <int ROWS>
 __global__ __launch_bounds__(1024) void k_expert_plan(const int* __restrict__ ids, int planes, uint64_t per_topk,
                                                       int experts, int* __restrict__ starts, int* __restrict__ sorted,
                                                       int* __restrict__ tokens, int* __restrict__ flags) {
     __shared__ int s_less[16], s_same[16];
-    __shared__ uint16_t s_list[16][64 * ROWS];
+    __shared__ uint16_t s_list[16][PLAN_LIST];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const uint32_t mine = blockIdx.x, none = (uint32_t)experts;
     const int run = ((planes + waves - 1) / waves + 63) & ~63, first = min(planes, wave * run), last = min(planes, first + run);
+    uint16_t* list = s_list[wave];
     int less = 0, same = 0;
     uint32_t key[ROWS], next[ROWS];
     plan_keys(ids, first, last, none, key);
     for (int p = first; p < last; p += 64 * ROWS) {
-        if (!ONCE) plan_keys(ids, p + 64 * ROWS, last, none, next);
+        plan_keys(ids, p + 64 * ROWS, last, none, next);
+        plan_list(key, mine, p - first, list, same);
 #pragma unroll
         for (int i = 0; i < ROWS; i++) {
             less += key[i] < mine;
-            same += key[i] == mine;
-            if (!ONCE) key[i] = next[i];
+            key[i] = next[i];
         }
     }
     less = __builtin_amdgcn_readlane(wave_scan(less), 63);
-    same = __builtin_amdgcn_readlane(wave_scan(same), 63);
     if (lane == 0) s_less[wave] = less, s_same[wave] = same;
     __syncthreads();
-    int at = 0, before = 0;
+    int at = 0, before = 0, all = 0, others = 0;  // planes: own ahead, of smaller experts, own, of none ahead
     for (int w = 0; w < waves; w++) {
-        before += s_less[w];
-        if (w < wave) at += s_same[w];
+        const int count = s_same[w], smaller = s_less[w];
+        before += smaller;
+        all += count;
+        if (w < wave) at += count, others += run - count - smaller;  // the runs ahead are whole
     }
     if (threadIdx.x == 0) starts[mine] = before;
     at += before;
-    if (!same) return;
-    uint16_t* list = s_list[wave];
     bool bad = false;
-    if (!ONCE) plan_keys(ids, first, last, none, key);
-    for (int p = first; p < last; p += 64 * ROWS) {
-        if (!ONCE) plan_keys(ids, p + 64 * ROWS, last, none, next);
-        int found = 0;
-#pragma unroll
-        for (int i = 0; i < ROWS; i++) {
-            const uint64_t m = __ballot(key[i] == mine);
-            if (key[i] == mine)
-                list[found + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] =
-                    (uint16_t)(64 * i + lane);
-            found += __builtin_popcountll(m);
-            if (!ONCE) key[i] = next[i];
-        }
-        // a wave's own list: its LDS operations are in order
-        for (int i = lane; i < found; i += 64) {
-            const int plane = p + list[i];
+    auto place = [&](int from, int count, uint32_t whose) {  // a wave's own list: its LDS operations are in order
+        for (int i = lane; i < count; i += 64) {
+            const int plane = from + list[i];
             sorted[at + i] = plane;
             tokens[at + i] = (int)((uint64_t)plane * per_topk >> 40);
-            if (mine == none) bad |= ids[plane] >= experts;
+            if (whose == none) bad |= ids[plane] >= experts;
         }
-        at += found;
+        at += count;
+    };
+    auto again = [&](uint32_t whose) {
+        static_assert(64 * ROWS <= PLAN_LIST, "rows loaded at a time fit the list");
+        for (int p = first; p < last; p += 64 * ROWS) {
+            int found = 0;
+            plan_keys(ids, p, last, none, key);
+            plan_list(key, whose, 0, list, found);
+            place(p, found, whose);
+        }
+    };
+    if (same <= PLAN_LIST && run <= 65536) place(first, same, mine);
+    else again(mine);
+    if (mine + 1 == none) {
+        if (threadIdx.x == 0) starts[none] = before + all;
+        if (before + all < planes) {
+            at = before + all + min(others, planes);
+            again(none);
+        }
     }
     if (bad) flags[0] = 1;
 }
@@ -96,13 +115,11 @@ hipError_t launch_expert_plan(const int* ids, int64_t planes, int topk, int expe
     const uint64_t per = (1ull << 40) / (uint32_t)topk + 1;
     const int p = (int)planes;
     if (planes <= 1024)
-        k_expert_plan<4, true><<<experts + 1, 256, 0, s>>>(ids, p, per, experts, starts, sorted, tokens, flags);
+        k_expert_plan<4><<<experts, 256, 0, s>>>(ids, p, per, experts, starts, sorted, tokens, flags);
     else if (planes <= 4096)
-        k_expert_plan<4, true><<<experts + 1, 1024, 0, s>>>(ids, p, per, experts, starts, sorted, tokens, flags);
-    else if (planes <= 16384)
-        k_expert_plan<16, true><<<experts + 1, 1024, 0, s>>>(ids, p, per, experts, starts, sorted, tokens, flags);
+        k_expert_plan<4><<<experts, 1024, 0, s>>>(ids, p, per, experts, starts, sorted, tokens, flags);
     else
-        k_expert_plan<16, false><<<experts + 1, 1024, 0, s>>>(ids, p, per, experts, starts, sorted, tokens, flags);
+        k_expert_plan<16><<<experts, 1024, 0, s>>>(ids, p, per, experts, starts, sorted, tokens, flags);
     return hipGetLastError();
 }
 

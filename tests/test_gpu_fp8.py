@@ -279,6 +279,19 @@ def test_plan(L, tokens, topk, experts):
     L.paged_check()
 
 
+@pytest.mark.parametrize("tokens,hot", [(3000, 1.0), (40000, 1.0), (40000, 0.9), (40000, 0.5), (200000, 0.2)])
+def test_plan_of_one_liked_expert(L, tokens, hot):
+    """More planes of one expert than a wave lists at once, in all waves or in some, and many of none."""
+    g = torch.Generator().manual_seed(tokens)
+    ids = torch.randint(-2, 7, (tokens, 2), generator=g, dtype=torch.int32)
+    ids[torch.rand(tokens, 2, generator=g) < hot] = 3
+    ids[tokens // 3: tokens // 2] = -1
+    p = L.expert_plan(ids.cuda(), 7)
+    for got, want in zip(p, plan_of(ids, 7)):
+        assert torch.equal(got.cpu().long(), want)
+    L.paged_check()
+
+
 def test_plan_reports_ids_past_the_last_expert(L):
     L.paged_check()
     ids = torch.tensor([[0, 7], [3, -5], [2 ** 31 - 1, 1]], dtype=torch.int32)
