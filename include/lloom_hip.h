@@ -340,10 +340,15 @@ int lloom_hip_paged_attention_workspace_bytes(int64_t tokens, int64_t requests, 
  *   y[m][n] = sum_b sx[m][b] sw[n / 128][b] sum_{k in b} qx[m][k] qw[n][k]
  * over blocks b of 128 values of k (the last one may be shorter).  The weight is
  * [n][k] of bytes with scales [ceil(n / 128)][ceil(k / 128)], as checkpoints
- * hold them; k is a multiple of 16.  Activations are F32, F16 or BF16, or E4M3
- * with a scale for each block of a row.  Rows and weights 16-byte aligned.  The
- * scales of a block are multiplied in f32: products of the two below 2^-126
- * lose bits.  The calls neither synchronize nor copy; what only the GPU can
+ * hold them; k is a multiple of 16, at most 2^22.  Activations are F32, F16 or
+ * BF16, or E4M3 with a scale for each block of a row.  Rows and weights 16-byte
+ * aligned; at most 2^24 rows and n, 4096 experts; x that is gathered from, in 8
+ * bits, and the scales are under 2^31 bytes.  A block's sum is formed first and the
+ * product of its two scales, rounded to f32, meets it: scales whose product is below
+ * 2^-126 lose bits, and over f32's largest a sum of zero gives NaN.  Sums are f32.
+ * Products are exact, but where many rows go into F16 or BF16 y: there the matrix
+ * cores cut off what is under 2^-13 of the largest of eight neighbours' products
+ * (1.5e-5 of the result in the 2-norm).  The calls neither synchronize nor copy; what only the GPU can
  * see is left out of the result as said below and reported by the next
  * lloom_hip_ctx_sync as LLOOM_HIP_EEXPERT.
  *

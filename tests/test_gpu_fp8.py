@@ -135,6 +135,18 @@ def test_gate_is_the_formula_in_f32(L):
     assert torch.equal(s, s2) and (q.view(torch.uint8) != q2.view(torch.uint8)).float().mean().item() < 1e-4
 
 
+def test_gate_near_the_end_of_the_exponential(L):
+    """Gates of -88.5 to -60, sixteen neighbours of one value, with an `up` that brings them to the middle of f32: the
+    formula's few roundings (as in test_gate) and e4m3's."""
+    g = torch.linspace(-88.5, -60, 64 * 512).reshape(64, 512, 1).expand(64, 512, 16).reshape(64, 8192).contiguous()
+    u = torch.full_like(g, 2.0 ** 100)
+    q, s = L.fp8_silu_mul(g.cuda(), u.cuda())
+    h = f64(g) / (1 + np.exp(-f64(g))) * 2.0 ** 100
+    got = R.values(q) * np.repeat(f64(s), 128, 1)
+    # eight values of 16 a block, at most e^.007 apart: all in one or two steps of e4m3, half a step of at most 2^-3 off
+    assert np.all(np.abs(got - h) <= (2.0 ** -4 + 2.0 ** -20) * np.abs(h))
+
+
 # ----------------------------------------------------------------- weights --
 
 @pytest.mark.parametrize("dtype", ACTS)
