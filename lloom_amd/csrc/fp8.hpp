@@ -45,10 +45,11 @@ hipError_t launch_fp8_weights(int type, const void* w, int64_t planes, int64_t n
 hipError_t launch_expert_plan(const int* ids, int64_t planes, int topk, int experts, int* starts, int* sorted,
                               int* tokens, int* flags, hipStream_t s);
 // Whether fp8_few.hip serves a call (else fp8_tile.hip).  Its workgroups' tiles
-// meet no other's, so it keeps all CUs busy with small outputs: 128 rows of [4096,
-// 4096] 15.1 against 19.0 us, 192 26 / 19, 64 rows of [8192, 2048] 9.7 / 11.1, 96 12.7
-// / 11.6, 192 22 / 12.5.  Grouped, us with 4, 8 and 12 rows an expert on average: [128, 1536, 2048]
-// 67, 79, 88 against 67, 72, 75, [128, 2048, 768] 41, 50, 55 / 41, 46, 49.
+// meet no other's, so it keeps all CUs busy with small outputs.  us of the two into
+// bf16: 64 rows of [4096, 4096] 10.8 / 13.5, 128 15.0 / 13.6 (into f32 14.9 / 18.3), 32 of
+// [8192, 8192] 21.0 / 29.3, 64 30.6 / 29.0, 96 of [8192, 2048] 12.7 / 8.9.  Grouped, with
+// 4, 8 and 12 rows an expert on average: [128, 1536, 2048] 67, 79, 88 against 67, 72, 75,
+// [128, 2048, 768] 41, 50, 55 / 41, 46, 49.
 inline bool fp8_few_rows(int64_t rows, int64_t n, int64_t experts, bool grouped) {
     return rows <= 16 || (grouped ? rows <= 4 * experts : rows * n <= 128 * 4096);
 }

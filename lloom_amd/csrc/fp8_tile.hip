@@ -20,6 +20,11 @@ namespace lloom {
 // weight is the matrix instructions' A: a lane's sums are of one row of x, so one
 // factor (its scale times the weight block's) serves them all.
 //
+// Where there are few tiles, KS parts of k are summed side by side, each by its own
+// waves in its own stages, and meet in LDS at the end.  A step is a wave's way from a
+// barrier through its reads to its products, about 0.5 us whatever the tile and
+// the stages; two waves a SIMD go it at once.
+//
 // Into F16 and BF16 a block of a 16 x 16 tile is one v_mfma_f32_16x16x128_f8f6f4.
 // It adds groups of eight products with 14 bits from the group's largest on (what
 // is under 2^-13 of that is cut), the groups and the blocks in f32: 1.5e-5 of the
@@ -33,18 +38,18 @@ namespace lloom {
 // barriers too 382, with zeros for data 493, 354 and 301: the clock falls with the
 // data's bits, and the loads cost a fifth, nearly all of it though every tile come
 // from one place of the L2 (490).
-template <int WM_, int WN_, int MF_, int NF_, int S_>
+template <int WM_, int WN_, int MF_, int NF_, int S_, int KS_ = 1>
 struct Fp8Cfg {
-    static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_, S = S_;
-    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+    static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_, S = S_, KS = KS_;
+    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES * KS;  // WAVES: of a part of k
     static constexpr int BM = 32 * WM * MF, BN = 32 * WN * NF;
     static constexpr int SHIFT = BM == 32 ? 5 : BM == 64 ? 6 : BM == 128 ? 7 : 8;
     static constexpr int W = BN * 128, X = BM * 128, XS = BM * 4 < 256 ? 256 : BM * 4, STAGE = W + X + XS;
     static constexpr int W_LOADS = BN / 8 / WAVES, X_LOADS = BM / 8 / WAVES;
     static constexpr int XS_LOADS = (BM / 64 + WAVES - 1) / WAVES < 1 ? 1 : (BM / 64 + WAVES - 1) / WAVES;
     static constexpr int PITCH = 32 * NF * 4 + 16;  // a row of a wave's part of y on its way out, f32 at most
-    static constexpr int OUT = WAVES * 32 * PITCH, RING = S * STAGE;
-    static constexpr int LDS = RING + BM * 4 > OUT ? RING + BM * 4 : OUT;
+    static constexpr int OUT = WAVES * 32 * PITCH, RING = S * STAGE, SUMS = (KS - 1) * BM * BN * 4;
+    static constexpr int LDS = KS * RING + BM * 4 > OUT + SUMS ? KS * RING + BM * 4 : OUT + SUMS;
     static_assert(BM == 1 << SHIFT && W_LOADS * WAVES * 8 == BN && X_LOADS * WAVES * 8 == BM, "whole loads");
     static_assert(128 % (32 * NF) == 0, "a wave's weight rows share their scales");
     static constexpr int DMA = W_LOADS + X_LOADS + XS_LOADS;  // a wave's loads of a stage
@@ -123,8 +128,8 @@ struct Fp8Sums<false> {
 template <class C, bool EXACT, int YT>
 __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nbn) {
     extern __shared__ __align__(16) uint8_t smem[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wv = __builtin_amdgcn_readfirstlane(wave), wm = wv / C::WN, wn = wv % C::WN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int part_k = C::KS > 1 ? wave / C::WAVES : 0, wv = wave - part_k * C::WAVES, wm = wv / C::WN, wn = wv % C::WN;
     int t, bn;
     const Fp8Tile tile = fp8_tile<C::SHIFT>(c, [&](int tiles) {
         if (!c.starts) tile_of(tiles, nbn, t, bn);
@@ -133,7 +138,9 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
         return t;
     });
     if (tile.count <= 0) return;
-    const int n0 = bn * C::BN, steps = tile.zero ? 0 : c.kb;
+    // block s of this part of k is block `base + s` of the rows; parts are of one
+    // length, and what the last has past kb is zeros
+    const int n0 = bn * C::BN, steps = tile.zero ? 0 : (c.kb + C::KS - 1) / C::KS, base = part_k * steps;
 
     const uint8_t* wbase = c.w + ((int64_t)tile.group * c.n + n0) * c.k;
     const fp8_v4i wbuf = fp8_buffer(wbase);
@@ -143,13 +150,14 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
     // A wave's loads of an operand are WAVES * 8 rows apart, so its lanes' pieces
     // are alike in all of them.  Rows of x are looked up in LDS, where they wait
     // for their step (-1: none): held in registers their offsets would spill.
-    int* s_from = (int*)(smem + C::RING);
+    int* s_from = (int*)(smem + C::KS * C::RING);
     for (int row = threadIdx.x; row < C::BM; row += C::THREADS)
         s_from[row] = row < tile.count && steps ? fp8_x_row(c, tile.first + row) - (int)x0 : -1;
     __syncthreads();
     const int row0 = 8 * wv + (lane >> 3), byte = 16 * ((lane & 7) ^ fp8_swizzle(row0));
     const uint32_t wlast = (uint32_t)min(C::BN, c.n - n0) - 1;
-    const uint32_t lds0 = lds_addr(smem);
+    uint8_t* ring = smem + part_k * C::RING;
+    const uint32_t lds0 = lds_addr(ring);
     constexpr int XS_PARTS = C::BM < 64 ? 1 : C::BM / 64;
     struct From {
         int x[C::X_LOADS], s[C::XS_LOADS];
@@ -162,7 +170,7 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
     };
     // loads lo .. hi - 1 of the wave's share of a stage
     auto issue = [&](int s, int slot, const From& from, int lo, int hi) {
-        const uint32_t st = lds0 + slot * C::STAGE, at = 128u * s;
+        const uint32_t st = lds0 + slot * C::STAGE, block = base + s, at = 128u * block;
         const bool past = (int)at + byte >= c.k;  // the last block's pieces past the end of the rows
 #pragma unroll
         for (int j = 0; j < C::DMA; j++) {
@@ -173,8 +181,8 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
                           st + C::W + 1024 * (wv + C::WAVES * i));
             } else if (j < C::X_LOADS + C::XS_LOADS) {
                 const int i = j - C::X_LOADS, r = from.s[i];
-                fp8_dma4(sbuf, r < 0 ? FP8_OUT : (uint32_t)r * (uint32_t)c.xs_row * 4u,
-                         (uint32_t)s * (uint32_t)c.xs_block * 4u, st + C::W + C::X + 256 * ((wv + C::WAVES * i) % XS_PARTS));
+                fp8_dma4(sbuf, r < 0 || (C::KS > 1 && (int)block >= c.kb) ? FP8_OUT : (uint32_t)r * (uint32_t)c.xs_row * 4u,
+                         (C::KS > 1 ? min(block, (uint32_t)c.kb - 1) : block) * (uint32_t)c.xs_block * 4u, st + C::W + C::X + 256 * ((wv + C::WAVES * i) % XS_PARTS));
             } else {
                 const int i = j - C::X_LOADS - C::XS_LOADS;
                 const uint32_t off = min((uint32_t)(row0 + 8 * C::WAVES * i), wlast) * (uint32_t)c.k + byte;
@@ -196,11 +204,14 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
     const float* ws = c.ws + ((int64_t)tile.group * c.nb + min((n0 + wn * 32 * C::NF) >> 7, c.nb - 1)) * c.kb;
     float wscale = 0.0f;  // lane l: of block 64 i + l
     auto weight_scale = [&](int s) {
-        if ((s & 63) == 0) wscale = fp8_load_now(ws + min(s + lane, c.kb - 1));
+        if ((s & 63) == 0) {
+            wscale = fp8_load_now(ws + min(base + s + lane, c.kb - 1));
+            if (C::KS > 1 && base + s + lane >= c.kb) wscale = 0.0f;
+        }
         return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wscale), s & 63));
     };
     auto read_s = [&](int slot, int a) {
-        return *(const float*)(smem + slot * C::STAGE + C::W + C::X + 4 * ((wm * MT + a) * T + ct));
+        return *(const float*)(ring + slot * C::STAGE + C::W + C::X + 4 * ((wm * MT + a) * T + ct));
     };
     // Everything of a step's stage is read before its last weight rows are
     // multiplied: there the next stage has had S - 1 steps' time to land, a barrier
@@ -237,8 +248,8 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
         for (int a = 0; a < MT; a++) f[a] = read_s(0, a);
         int slot = 0;
         if constexpr (EXACT) {
-            auto read_w = [&](int slot, int b) { return fp8_read(smem + slot * C::STAGE, (wn * NT + b) * 32 + ct, ht); };
-            auto read_x = [&](int slot, int a) { return fp8_read(smem + slot * C::STAGE + C::W, (wm * MT + a) * 32 + ct, ht); };
+            auto read_w = [&](int slot, int b) { return fp8_read(ring + slot * C::STAGE, (wn * NT + b) * 32 + ct, ht); };
+            auto read_x = [&](int slot, int a) { return fp8_read(ring + slot * C::STAGE + C::W, (wm * MT + a) * 32 + ct, ht); };
             Fp8Row x[MT], w = read_w(0, 0);
 #pragma unroll
             for (int a = 0; a < MT; a++) x[a] = read_x(0, a);
@@ -292,8 +303,8 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
             // a wave's tiles in turn, the sums of the one LAG before brought home
             // under a tile's products; weight rows are read two tiles' rows ahead
             constexpr int LAG = 2, TILES = NT * MT, TURN = (NT - 3) * MT;
-            auto read_w = [&](int slot, int b) { return fp8_read16(smem + slot * C::STAGE, (wn * NT + b) * 16 + ct, ht); };
-            auto read_x = [&](int slot, int a) { return fp8_read16(smem + slot * C::STAGE + C::W, (wm * MT + a) * 16 + ct, ht); };
+            auto read_w = [&](int slot, int b) { return fp8_read16(ring + slot * C::STAGE, (wn * NT + b) * 16 + ct, ht); };
+            auto read_x = [&](int slot, int a) { return fp8_read16(ring + slot * C::STAGE + C::W, (wm * MT + a) * 16 + ct, ht); };
             v8i x[MT], w[3] = {read_w(0, 0), read_w(0, 1), v8i{}};
 #pragma unroll
             for (int a = 0; a < MT; a++) x[a] = read_x(0, a);
@@ -336,6 +347,36 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
     // every wave has read its last operands before y passes through the ring
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
+
+    // the parts' sums meet in the first's waves
+    if constexpr (C::KS > 1) {
+        constexpr int QUADS = T * T / 256;
+        float4* sums = (float4*)(smem + C::OUT) + wv * 64 + lane;
+        auto at = [&](int p, int b, int a, int r) { return (((p * NT + b) * MT + a) * QUADS + r) * 64 * C::WAVES; };
+#pragma unroll
+        for (int b = 0; b < NT; b++)
+#pragma unroll
+            for (int a = 0; a < MT; a++)
+#pragma unroll
+                for (int r = 0; r < QUADS; r++) {
+                    const Sums& v = acc[b][a];
+                    if (part_k) sums[at(part_k - 1, b, a, r)] = make_float4(v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]);
+                }
+        __syncthreads();
+        if (part_k) return;
+#pragma unroll
+        for (int p = 0; p < C::KS - 1; p++)
+#pragma unroll
+            for (int b = 0; b < NT; b++)
+#pragma unroll
+                for (int a = 0; a < MT; a++)
+#pragma unroll
+                    for (int r = 0; r < QUADS; r++) {
+                        const float4 d = sums[at(p, b, a, r)];
+                        Sums& v = acc[b][a];
+                        v[4 * r] += d.x, v[4 * r + 1] += d.y, v[4 * r + 2] += d.z, v[4 * r + 3] += d.w;
+                    }
+    }
 
     // y: a wave's 32 rows at a time through LDS, so that stores run along n
     constexpr int SIZE = YT == T_F32 ? 4 : 2, PER = 16 / SIZE, LANES = 32 * C::NF / PER, ROWS = 64 / LANES;
@@ -403,16 +444,18 @@ static hipError_t tile_with(const Fp8Call& c, hipStream_t s) {
     }
 }
 
-// The largest tile that is mostly full and leaves workgroups for all CUs; us by
-// (rows of x, of the weight) a tile:
-//   (32, 128) / (64, 128) / (128, 128): 256 rows of [4096, 4096] 19 / 21 / 27, 192 of
-//     [8192, 2048] 13.8 / 12.9 / 16.6, 128 of [8192, 8192] 36 / 55 / 61 (with two
-//     stages; three in the first)
+// The largest tile that is mostly full and leaves workgroups for all CUs; where the
+// small ones are one round, k in two parts.  us by (rows of x, of the weight) a tile:
+//   (32, 128) / the same, two parts / (64, 128), two parts / (64, 128): 128 rows of
+//     [8192, 8192] 36 / 30 / 34 / 55, 256 of [4096, 4096] 18.4 / 14.4 / 16.2 / 21, into f32
+//     26 / 19 / 23 / 27, 192 of [6144, 2048] 13.4 / 16.1 / 10.2 / 12.6, 320 of [4096, 4096]
+//     - / 26 / 16 / 19, 509 22 / - / 16.7; six stages for three 36.4 in the first
 //   (64, 128) / (128, 128) / (256, 256): 509 rows of [8192, 2048] 15.8 / 17.8 / -, into
 //     f32 24.7 / 25.8; 2048 rows 59 / 48 / 41; 4096 of [4096, 4096] into f32 152 / 136
 //   grouped, top 8 of 128 experts [1536, 2048], 8, 12 and 32 rows an expert on
-//     average: 71 / 73 / 82, 77 / 75 / 81, 92 / 85 / 94; of 64 [2048, 2048], 256 and
-//     1024: - / 141 / 128 and (256, 256) 134, - / 451 / 402 / 368
+//     average, (32, 128) / (64, 128) / (128, 128): 71 / 73 / 82, 77 / 75 / 81, 92 / 85 /
+//     94; of 64 [2048, 2048], 256 and 1024: - / 141 / 128 and (256, 256) 134, - / 451 /
+//     402 / 368
 hipError_t launch_fp8_tile(const Fp8Call& c, hipStream_t s) {
     if (!c.xs && c.x_rows) return hipErrorInvalidValue;  // rows that are not in 8 bits
     auto count = [&](int rows, int cols) { return (int64_t)((c.m + rows - 1) / rows) * ((c.n + cols - 1) / cols); };
@@ -421,8 +464,10 @@ hipError_t launch_fp8_tile(const Fp8Call& c, hipStream_t s) {
         return c.y_type == T_F16 ? tile_of_type<Fp8Cfg<4, 2, 2, 4, 2>, false, T_F16>(c, s)
                                  : tile_of_type<Fp8Cfg<4, 2, 2, 4, 2>, false, T_BF16>(c, s);
     if (c.starts ? each >= 96 : count(128, 128) >= 300) return tile_with<Fp8Cfg<2, 2, 2, 2, 2>>(c, s);
-    if (c.starts ? each >= 10 : count(64, 128) >= 180) return tile_with<Fp8Cfg<2, 2, 1, 2, 2>>(c, s);
-    return tile_with<Fp8Cfg<1, 2, 1, 2, 3>>(c, s);
+    if (c.starts ? each >= 10 : count(64, 128) > 256) return tile_with<Fp8Cfg<2, 2, 1, 2, 2>>(c, s);
+    if (c.starts) return tile_with<Fp8Cfg<1, 2, 1, 2, 3>>(c, s);
+    if (count(64, 128) > 128) return tile_with<Fp8Cfg<2, 2, 1, 2, 3, 2>>(c, s);
+    return tile_with<Fp8Cfg<1, 2, 1, 2, 3, 2>>(c, s);
 }
 
 }  // namespace lloom

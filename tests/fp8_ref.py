@@ -73,7 +73,7 @@ def product(x, sx, w, sw, dtype, groups8):
     far it may be off.  A block's products (exact: 8 bits each) are added in f32 in fewer than 128 steps, each of which
     rounds or cuts at 2^-23 of what is there at most; the scales' product and the step that adds the block round once each,
     the parts of up to 8 waves are added once more; then y is rounded.  groups8: groups of eight products are added with
-    each cut at 2^-13 of the largest's power of two."""
+    each cut at 2^-13 of the largest's power of two.  F16 has steps of 2^-24 below 2^-14, so a y there is up to 2^-25 off."""
     (m, k), n = x.shape, w.shape[0]
     y, size, cut = np.zeros((m, n)), np.zeros((m, n)), np.zeros((m, n))
     for b in range(sx.shape[1]):
@@ -85,4 +85,4 @@ def product(x, sx, w, sw, dtype, groups8):
             # eight products of at most the block's largest each, sixteen groups
             cut += 16 * 8 * 2.0 ** -13 * np.abs(a).max(1)[:, None] * np.abs(c).max(1)[None] * np.abs(f)
     steps = 128 + sx.shape[1] + 8 + 3
-    return y, steps * 2.0 ** -23 * size + cut + EPS[dtype] * np.abs(y) + 2.0 ** -126
+    return y, steps * 2.0 ** -23 * size + cut + EPS[dtype] * np.abs(y) + (2.0 ** -25 if dtype is torch.float16 else 2.0 ** -126)

@@ -197,6 +197,23 @@ SIZES = [(1, 16, 16), (1, 6152, 912), (1, 80, 8208), (4, 16400, 272), (12, 4104,
 
 
 @pytest.mark.parametrize("out", ACTS)
+@pytest.mark.parametrize("m,n,k", [(2100, 264, 16), (2100, 264, 272), (540, 1000, 1152), (1100, 1000, 16), (1100, 1000, 528),
+                                   (700, 1500, 2064)])
+def test_matmul_of_an_odd_number_of_blocks(L, m, n, k, out):
+    w, ws = weights(n + k, n, k)
+    q, sx = (t.cpu() for t in L.fp8_quantize(normal(m, m, k).cuda()))
+    ws[0, -1] = 3e38  # past the end of the rows nothing may meet it
+    sx[0, -1] = 3e38
+    sx, ws = sx * 2.0 ** -64, ws * 2.0 ** -64
+    y = L.fp8_matmul(q.cuda(), w.cuda(), ws.cuda(), x_scales=sx.cuda(), out_dtype=out).cpu()
+    check_product(y[1:], q[1:], sx[1:], w, ws)
+    check_product(y[:1, 128:], q[:1], sx[:1], w[128:], ws[1:])
+    # where the two scales meet (2.6e38, in f32's range) sums of 1.4 and more are past its largest, 3.4e38
+    d = R.values(q)[0, -((k - 1) % 128 + 1):] @ R.values(w)[:128, -((k - 1) % 128 + 1):].T
+    assert np.array_equal(f64(y)[0, :128][np.abs(d) > 1.4], np.copysign(np.inf, d[np.abs(d) > 1.4]))
+
+
+@pytest.mark.parametrize("out", ACTS)
 @pytest.mark.parametrize("m,n,k", SIZES)
 def test_matmul(L, m, n, k, out):
     w, ws = weights(n + k, n, k)
