@@ -449,7 +449,12 @@ static hipError_t tile_with(const Fp8Call& c, hipStream_t s) {
 //   (32, 128) / the same, two parts / (64, 128), two parts / (64, 128): 128 rows of
 //     [8192, 8192] 36 / 30 / 34 / 55, 256 of [4096, 4096] 18.4 / 14.4 / 16.2 / 21, into f32
 //     26 / 19 / 23 / 27, 192 of [6144, 2048] 13.4 / 16.1 / 10.2 / 12.6, 320 of [4096, 4096]
-//     - / 26 / 16 / 19, 509 22 / - / 16.7; six stages for three 36.4 in the first
+//     - / 26 / 16 / 19, 509 22 / - / 16.7, 130 of [8192, 1024] 9.0 / 11.3 / 7.7 / 8.2, 128
+//     of [8192, 512] 5.7 / 5.9 / 6.5 / 6.1, 192 of [6144, 512] 6.4 / 9.4 / 6.2 / 5.8; six
+//     stages for three 36.4 in the first
+//   (64, 128) / (128, 128), two parts, into bf16 and into f32: 260 rows of [8192, 2048]
+//     15.1 / 15.6, 24.0 / 22.3; 400 of [6144, 4096] 24.9 / 23.8, 38.3 / 34.9; 384 of [8192,
+//     8192] 57 / 49, 76 / 66; 640 of [4096, 1024] 9.5 / 10.5, 14.6 / 15.0
 //   (64, 128) / (128, 128) / (256, 256): 509 rows of [8192, 2048] 15.8 / 17.8 / -, into
 //     f32 24.7 / 25.8; 2048 rows 59 / 48 / 41; 4096 of [4096, 4096] into f32 152 / 136
 //   grouped, top 8 of 128 experts [1536, 2048], 8, 12 and 32 rows an expert on
@@ -464,8 +469,11 @@ hipError_t launch_fp8_tile(const Fp8Call& c, hipStream_t s) {
         return c.y_type == T_F16 ? tile_of_type<Fp8Cfg<4, 2, 2, 4, 2>, false, T_F16>(c, s)
                                  : tile_of_type<Fp8Cfg<4, 2, 2, 4, 2>, false, T_BF16>(c, s);
     if (c.starts ? each >= 96 : count(128, 128) >= 300) return tile_with<Fp8Cfg<2, 2, 2, 2, 2>>(c, s);
-    if (c.starts ? each >= 10 : count(64, 128) > 256) return tile_with<Fp8Cfg<2, 2, 1, 2, 2>>(c, s);
-    if (c.starts) return tile_with<Fp8Cfg<1, 2, 1, 2, 3>>(c, s);
+    if (!c.starts && count(64, 128) > 256 && count(128, 128) <= 256 && c.kb >= (c.y_type == T_F32 ? 16 : 32))
+        return tile_with<Fp8Cfg<2, 2, 2, 2, 2, 2>>(c, s);
+    const bool parts = c.kb >= 8;
+    if (c.starts ? each >= 10 : count(64, 128) > (parts ? 256 : 128)) return tile_with<Fp8Cfg<2, 2, 1, 2, 2>>(c, s);
+    if (c.starts || !parts) return tile_with<Fp8Cfg<1, 2, 1, 2, 3>>(c, s);
     if (count(64, 128) > 128) return tile_with<Fp8Cfg<2, 2, 1, 2, 3, 2>>(c, s);
     return tile_with<Fp8Cfg<1, 2, 1, 2, 3, 2>>(c, s);
 }
