@@ -12,22 +12,23 @@ namespace lloom {
 // between workgroups; what it costs is that each reads all ids.  ROWS rows of 64
 // are loaded at a time, the next ones under those in work.  A wave whose list is
 // too short (over PLAN_LIST planes of one expert in its run) goes through its run
-// again, a list at a time.  128 experts, 256 planes 2.9 us (a launch), 16384 5.4,
-// 65536 10.2 (12.7 with a first time that only counts): 16 waves of a CU read and
-// rank 64 ids in about 18 clocks each, no more workgroups than CUs.
+// again, a list at a time.  Rows without a plane of the expert are skipped: 800000
+// planes 73 us, 77 without.  128 experts, 256 planes 2.8 us (a launch), 16384 5.2, 65536
+// 9.9 (12.7 with a first time that only counts), 256 experts 9.8; 4096 experts, 16000
+// planes 35.5.
 constexpr int PLAN_LIST = 1024;
 
-// Keys of a wave's next rows from plane p on: an id, `none` for one of no expert,
-// -1 past the last.
-template <int ROWS>
+// Keys of a wave's next rows from plane p on: an id (CLAMP: `none` for one of no
+// expert), -1 past the last.
+template <bool CLAMP, int ROWS>
 __device__ __forceinline__ void plan_keys(const int* __restrict__ ids, int p, int last, uint32_t none, uint32_t (&key)[ROWS]) {
     const int at = p + (int)__lane_id();
     if (p + 64 * ROWS <= last) {
 #pragma unroll
-        for (int i = 0; i < ROWS; i++) key[i] = min((uint32_t)ids[at + 64 * i], none);
+        for (int i = 0; i < ROWS; i++) key[i] = CLAMP ? min((uint32_t)ids[at + 64 * i], none) : (uint32_t)ids[at + 64 * i];
     } else {
 #pragma unroll
-        for (int i = 0; i < ROWS; i++) key[i] = at + 64 * i < last ? min((uint32_t)ids[at + 64 * i], none) : ~0u;
+        for (int i = 0; i < ROWS; i++) key[i] = at + 64 * i >= last ? ~0u : CLAMP ? min((uint32_t)ids[at + 64 * i], none) : (uint32_t)ids[at + 64 * i];
     }
 }
 
@@ -38,6 +39,7 @@ __device__ __forceinline__ void plan_list(const uint32_t (&key)[ROWS], uint32_t 
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
         const uint64_t m = __ballot(key[i] == mine);
+        if (m == 0) continue;
         const int at = found + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
         if (key[i] == mine && at < PLAN_LIST) list[at] = (uint16_t)(off + 64 * i + (int)__lane_id());
         found += __builtin_popcountll(m);
@@ -56,9 +58,9 @@ __global__ __launch_bounds__(1024) void k_expert_plan(const int* __restrict__ id
     uint16_t* list = s_list[wave];
     int less = 0, same = 0;
     uint32_t key[ROWS], next[ROWS];
-    plan_keys(ids, first, last, none, key);
+    plan_keys<false>(ids, first, last, none, key);
     for (int p = first; p < last; p += 64 * ROWS) {
-        plan_keys(ids, p + 64 * ROWS, last, none, next);
+        plan_keys<false>(ids, p + 64 * ROWS, last, none, next);
         plan_list(key, mine, p - first, list, same);
 #pragma unroll
         for (int i = 0; i < ROWS; i++) {
@@ -92,7 +94,7 @@ __global__ __launch_bounds__(1024) void k_expert_plan(const int* __restrict__ id
         static_assert(64 * ROWS <= PLAN_LIST, "rows loaded at a time fit the list");
         for (int p = first; p < last; p += 64 * ROWS) {
             int found = 0;
-            plan_keys(ids, p, last, none, key);
+            plan_keys<true>(ids, p, last, none, key);
             plan_list(key, whose, 0, list, found);
             place(p, found, whose);
         }
