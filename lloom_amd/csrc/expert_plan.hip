@@ -28,7 +28,10 @@ __device__ __forceinline__ void plan_keys(const int* __restrict__ ids, int p, in
         for (int i = 0; i < ROWS; i++) key[i] = CLAMP ? min((uint32_t)ids[at + 64 * i], none) : (uint32_t)ids[at + 64 * i];
     } else {
 #pragma unroll
-        for (int i = 0; i < ROWS; i++) key[i] = at + 64 * i >= last ? ~0u : CLAMP ? min((uint32_t)ids[at + 64 * i], none) : (uint32_t)ids[at + 64 * i];
+        for (int i = 0; i < ROWS; i++) {
+            key[i] = at + 64 * i < last ? (uint32_t)ids[at + 64 * i] : ~0u;
+            if (CLAMP && at + 64 * i < last) key[i] = min(key[i], none);
+        }
     }
 }
 

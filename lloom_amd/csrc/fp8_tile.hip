@@ -181,8 +181,10 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
                           st + C::W + 1024 * (wv + C::WAVES * i));
             } else if (j < C::X_LOADS + C::XS_LOADS) {
                 const int i = j - C::X_LOADS, r = from.s[i];
-                fp8_dma4(sbuf, r < 0 || (C::KS > 1 && (int)block >= c.kb) ? FP8_OUT : (uint32_t)r * (uint32_t)c.xs_row * 4u,
-                         (C::KS > 1 ? min(block, (uint32_t)c.kb - 1) : block) * (uint32_t)c.xs_block * 4u, st + C::W + C::X + 256 * ((wv + C::WAVES * i) % XS_PARTS));
+                const bool none = r < 0 || (C::KS > 1 && block >= (uint32_t)c.kb);
+                const uint32_t sb = C::KS > 1 ? min(block, (uint32_t)c.kb - 1) : block;
+                fp8_dma4(sbuf, none ? FP8_OUT : (uint32_t)r * (uint32_t)c.xs_row * 4u, sb * (uint32_t)c.xs_block * 4u,
+                         st + C::W + C::X + 256 * ((wv + C::WAVES * i) % XS_PARTS));
             } else {
                 const int i = j - C::X_LOADS - C::XS_LOADS;
                 const uint32_t off = min((uint32_t)(row0 + 8 * C::WAVES * i), wlast) * (uint32_t)c.k + byte;

@@ -191,7 +191,8 @@ def check_product(y, x, xs, w, ws):
     assert np.all(np.abs(got - want) <= off), np.max(np.abs(got - want) / off)
 
 
-SIZES = [(1, 16, 16), (1, 6152, 912), (1, 80, 8208), (4, 16400, 272), (12, 4104, 2064), (1, 64, 128), (2, 24, 144), (5, 130, 272), (16, 128, 2048), (17, 257, 1040), (33, 96, 96), (64, 384, 640),
+SIZES = [(1, 16, 16), (1, 6152, 912), (1, 80, 8208), (4, 16400, 272), (12, 4104, 2064), (1, 64, 128), (2, 24, 144),
+         (5, 130, 272), (16, 128, 2048), (17, 257, 1040), (33, 96, 96), (64, 384, 640),
          (65, 200, 1376), (129, 127, 512), (255, 264, 768), (300, 520, 256), (1030, 1000, 400),
          (2100, 264, 144), (2049, 300, 912)]
 
