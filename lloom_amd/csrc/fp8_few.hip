@@ -169,10 +169,9 @@ __global__ __launch_bounds__(64 * W) void k_fp8_few(const Fp8Call c, int nblocks
         const int yr = fp8_y_row(c, tile.first + row), col = n0 + 16 * j + 4 * g;
         if (yr < 0) continue;
         const int64_t at = (int64_t)yr * c.n + col;
-        const bool wide = c.n % 4 == 0;
-        if (c.y_type == T_F32) fp8_store4<T_F32>(c.y, at, v, c.n - col, wide);
-        else if (c.y_type == T_F16) fp8_store4<T_F16>(c.y, at, v, c.n - col, wide);
-        else fp8_store4<T_BF16>(c.y, at, v, c.n - col, wide);
+        if (c.y_type == T_F32) fp8_store4<T_F32>(c.y, at, v, c.n - col);
+        else if (c.y_type == T_F16) fp8_store4<T_F16>(c.y, at, v, c.n - col);
+        else fp8_store4<T_BF16>(c.y, at, v, c.n - col);
     }
 }
 

@@ -384,7 +384,6 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
     constexpr int SIZE = YT == T_F32 ? 4 : 2, PER = 16 / SIZE, LANES = 32 * C::NF / PER, ROWS = 64 / LANES;
     uint8_t* part = smem + wv * 32 * C::PITCH;
     const int col0 = n0 + wn * 32 * C::NF, cl = lane % LANES * PER;
-    const bool wide = c.n % PER == 0;
 #pragma unroll
     for (int a = 0; a < C::MF; a++) {
 #pragma unroll
@@ -412,8 +411,8 @@ __global__ __launch_bounds__(C::THREADS) void k_fp8_tile(const Fp8Call c, int nb
             const int yr = fp8_y_row(c, tile.first + row);
             if (yr < 0) continue;
             uint8_t* y = (uint8_t*)c.y + ((int64_t)yr * c.n + col) * SIZE;
-            if (wide) {
-                *(uint4*)y = v;
+            if (col + PER <= c.n) {
+                fp8_store16(y, v);
             } else {
                 const uint32_t e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -458,7 +457,8 @@ static hipError_t tile_with(const Fp8Call& c, hipStream_t s) {
 //     15.1 / 15.6, 24.0 / 22.3; 400 of [6144, 4096] 24.9 / 23.8, 38.3 / 34.9; 384 of [8192,
 //     8192] 57 / 49, 76 / 66; 640 of [4096, 1024] 9.5 / 10.5, 14.6 / 15.0
 //   (64, 128) / (128, 128) / (256, 256): 509 rows of [8192, 2048] 15.8 / 17.8 / -, into
-//     f32 24.7 / 25.8; 2048 rows 59 / 48 / 41; 4096 of [4096, 4096] into f32 152 / 136
+//     f32 24.7 / 25.8; 1200 34 / 35 / 32, 1400 38 / 39 / 33, 2048 59 / 48 / 41, 2304 (a round of
+//     256 large tiles and 32 more) 62 / 58 / 63, 2560 67 / 60 / 63, 3000 77 / 68 / 65; 4096 of [4096, 4096] into f32 152 / 136
 //   grouped, top 8 of 128 experts [1536, 2048], 8, 12 and 32 rows an expert on
 //     average, (32, 128) / (64, 128) / (128, 128): 71 / 73 / 82, 77 / 75 / 81, 92 / 85 /
 //     94; of 64 [2048, 2048], 256 and 1024: - / 141 / 128 and (256, 256) 134, - / 451 /
@@ -467,7 +467,8 @@ hipError_t launch_fp8_tile(const Fp8Call& c, hipStream_t s) {
     if (!c.xs && c.x_rows) return hipErrorInvalidValue;  // rows that are not in 8 bits
     auto count = [&](int rows, int cols) { return (int64_t)((c.m + rows - 1) / rows) * ((c.n + cols - 1) / cols); };
     const int64_t each = c.m / c.experts;
-    if (c.y_type != T_F32 && (c.starts ? each >= 512 : count(256, 256) >= 200))
+    const int64_t large = count(256, 256);
+    if (c.y_type != T_F32 && (c.starts ? each >= 512 : large >= 160 && (large <= 256 || large > 320)))
         return c.y_type == T_F16 ? tile_of_type<Fp8Cfg<4, 2, 2, 4, 2>, false, T_F16>(c, s)
                                  : tile_of_type<Fp8Cfg<4, 2, 2, 4, 2>, false, T_BF16>(c, s);
     if (c.starts ? each >= 96 : count(128, 128) >= 300) return tile_with<Fp8Cfg<2, 2, 2, 2, 2>>(c, s);

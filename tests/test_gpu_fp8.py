@@ -199,7 +199,8 @@ SIZES = [(1, 16, 16), (1, 6152, 912), (1, 80, 8208), (4, 16400, 272), (12, 4104,
 
 @pytest.mark.parametrize("out", ACTS)
 @pytest.mark.parametrize("m,n,k", [(2100, 264, 16), (2100, 264, 272), (540, 1000, 1152), (1100, 1000, 16), (1100, 1000, 528),
-                                   (700, 1500, 2064), (1030, 2900, 4112), (520, 4200, 2064)])
+                                   (700, 1500, 2064), (1030, 2900, 4112), (520, 4200, 2064), (3400, 3101, 144),
+                                   (40, 4103, 272), (70, 9001, 144)])
 def test_matmul_of_an_odd_number_of_blocks(L, m, n, k, out):
     w, ws = weights(n + k, n, k)
     q, sx = (t.cpu() for t in L.fp8_quantize(normal(m, m, k).cuda()))
