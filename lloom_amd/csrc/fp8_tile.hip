@@ -458,7 +458,8 @@ static hipError_t tile_with(const Fp8Call& c, hipStream_t s) {
 //     8192] 57 / 49, 76 / 66; 640 of [4096, 1024] 9.5 / 10.5, 14.6 / 15.0
 //   (64, 128) / (128, 128) / (256, 256): 509 rows of [8192, 2048] 15.8 / 17.8 / -, into
 //     f32 24.7 / 25.8; 1200 34 / 35 / 32, 1400 38 / 39 / 33, 2048 59 / 48 / 41, 2304 (a round of
-//     256 large tiles and 32 more) 62 / 58 / 63, 2560 67 / 60 / 63, 3000 77 / 68 / 65; 4096 of [4096, 4096] into f32 152 / 136
+//     256 large tiles and 32 more) 62 / 58 / 63, 2560 67 / 60 / 63, 3000 77 / 68 / 65; 44000 of [112, 1264] -
+//     / 27 / 32, 20000 of [300, 4096] - / 44 / 45; 4096 of [4096, 4096] into f32 152 / 136
 //   grouped, top 8 of 128 experts [1536, 2048], 8, 12 and 32 rows an expert on
 //     average, (32, 128) / (64, 128) / (128, 128): 71 / 73 / 82, 77 / 75 / 81, 92 / 85 /
 //     94; of 64 [2048, 2048], 256 and 1024: - / 141 / 128 and (256, 256) 134, - / 451 /
@@ -468,7 +469,7 @@ hipError_t launch_fp8_tile(const Fp8Call& c, hipStream_t s) {
     auto count = [&](int rows, int cols) { return (int64_t)((c.m + rows - 1) / rows) * ((c.n + cols - 1) / cols); };
     const int64_t each = c.m / c.experts;
     const int64_t large = count(256, 256);
-    if (c.y_type != T_F32 && (c.starts ? each >= 512 : large >= 160 && (large <= 256 || large > 320)))
+    if (c.y_type != T_F32 && c.nb > 1 && (c.starts ? each >= 512 : large >= 160 && (large <= 256 || large > 320)))
         return c.y_type == T_F16 ? tile_of_type<Fp8Cfg<4, 2, 2, 4, 2>, false, T_F16>(c, s)
                                  : tile_of_type<Fp8Cfg<4, 2, 2, 4, 2>, false, T_BF16>(c, s);
     if (c.starts ? each >= 96 : count(128, 128) >= 300) return tile_with<Fp8Cfg<2, 2, 2, 2, 2>>(c, s);
