@@ -88,8 +88,17 @@ int lloom_hip_ctx_set_mv_rows_max(lloom_hip_ctx* ctx, int rows);
  *   faster there).
  * LLOOM_HIP_PREFILL_MMA=f16|int8|auto sets the default of new contexts.
  * No counterpart in the reference (its CUDA arm has one MMQ kernel). */
-enum { LLOOM_HIP_MMA_F16 = 0, LLOOM_HIP_MMA_INT8 = 1, LLOOM_HIP_MMA_AUTO = 2 };
+enum { LLOOM_HIP_MMA_F16 = 0, LLOOM_HIP_MMA_INT8 = 1, LLOOM_HIP_MMA_AUTO = 2, LLOOM_HIP_MMA_FP8 = 3 };
 int lloom_hip_ctx_set_prefill_mma(lloom_hip_ctx* ctx, int mode);
+/* Matrix-core family of the 8-bit floating-point products of many rows into
+ * F16 and BF16 y (into F32, and of few rows, it is always F16):
+ * LLOOM_HIP_MMA_F16 (default): the e4m3 numbers, exact in fp16, on
+ *   v_mfma_f32_32x32x16_f16: exact products, f32 sums;
+ * LLOOM_HIP_MMA_FP8: v_mfma_f32_16x16x128_f8f6f4, at twice the rate.  It cuts
+ *   off what is under 2^-13 of the largest of eight neighbours' products: 1.5e-5 of
+ *   the result in the 2-norm for normal values, and all that is left where large
+ *   neighbours cancel. */
+int lloom_hip_ctx_set_fp8_mma(lloom_hip_ctx* ctx, int mode);
 
 /* Wait for the device; report a device-side error (an out-of-range expert
  * id seen by a routed matmul, or an out-of-range embedding id: EEXPERT; a page,
@@ -345,10 +354,9 @@ int lloom_hip_paged_attention_workspace_bytes(int64_t tokens, int64_t requests, 
  * aligned; at most 2^24 rows and n, 4096 experts; x that is gathered from, in 8
  * bits, and the scales are under 2^31 bytes.  A block's sum is formed first and the
  * product of its two scales, rounded to f32, meets it: scales whose product is below
- * 2^-126 lose bits, and over f32's largest a sum of zero gives NaN.  Sums are f32.
- * Products are exact, but where many rows go into F16 or BF16 y: there the matrix
- * cores cut off what is under 2^-13 of the largest of eight neighbours' products
- * (1.5e-5 of the result in the 2-norm).  The calls neither synchronize nor copy; what only the GPU can
+ * 2^-126 lose bits, and over f32's largest a sum of zero gives NaN.  Products are
+ * exact and sums f32 into every type of y (but for lloom_hip_ctx_set_fp8_mma), which
+ * rounds once.  The calls neither synchronize nor copy; what only the GPU can
  * see is left out of the result as said below and reported by the next
  * lloom_hip_ctx_sync as LLOOM_HIP_EEXPERT.
  *

@@ -30,6 +30,8 @@ from .paged import (  # noqa: F401
     paged_plan,
 )
 from .fp8 import (  # noqa: F401
+    MMA_F16,
+    MMA_FP8,
     ExpertPlan,
     expert_plan,
     fp8_grouped_matmul,
@@ -38,4 +40,5 @@ from .fp8 import (  # noqa: F401
     fp8_quantize_weight,
     fp8_silu_mul,
     fp8_workspace_bytes,
+    set_fp8_mma,
 )

@@ -175,6 +175,14 @@ int lloom_hip_ctx_set_prefill_mma(lloom_hip_ctx* ctx, int mode) {
     return LLOOM_HIP_OK;
 }
 
+int lloom_hip_ctx_set_fp8_mma(lloom_hip_ctx* ctx, int mode) {
+    if (!ctx) return fail(LLOOM_HIP_EINVAL, "set_fp8_mma: null context");
+    if (mode != LLOOM_HIP_MMA_F16 && mode != LLOOM_HIP_MMA_FP8)
+        return fail(LLOOM_HIP_EINVAL, "set_fp8_mma: mode %d is none of F16 (0), FP8 (3)", mode);
+    ctx->fp8_cut = mode == LLOOM_HIP_MMA_FP8;
+    return LLOOM_HIP_OK;
+}
+
 int lloom_hip_ctx_sync(lloom_hip_ctx* ctx) {
     if (!ctx) return fail(LLOOM_HIP_EINVAL, "ctx_sync: null context");
     HIP_OK(hipSetDevice(ctx->device));

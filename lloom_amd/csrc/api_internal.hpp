@@ -34,6 +34,7 @@ struct lloom_hip_ctx {
     int* call_flag = nullptr;
     int mv_rows_max = 16;
     int prefill_mma = lloom::GEMM_AUTO;
+    bool fp8_cut = false;  // MMA_FP8
     std::mutex mu;
 };
 

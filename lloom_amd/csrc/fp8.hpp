@@ -31,6 +31,7 @@ struct Fp8Call {
     int* flags;  // [0]: rows, starts or ids out of range
     int64_t x_stride, xs_row, xs_block;
     int n, k, kb, nb, m, x_rows, y_rows, experts, y_type;
+    bool cut;  // halves of many rows by the 8-bit matrix instructions, whose sums are cut
 };
 
 // fp8_rows.hip: rows of x (F32, F16, BF16; x_stride elements apart) into e4m3 q

@@ -196,7 +196,8 @@ int lloom_hip_fp8_matmul(lloom_hip_ctx* ctx, const void* w_dev, const float* w_s
     HIP_OK(hipSetDevice(ctx->device));
     const Fp8Call c = {(const uint8_t*)w_dev, w_scales_dev, x_dev, x_scales_dev, y_dev, nullptr, nullptr, nullptr,
                        ctx->flags, x_stride, xs_row, xs_block, (int)n, (int)k, (int)((k + 127) / 128),
-                       (int)((n + 127) / 128), (int)m, (int)m, (int)m, 1, y_dtype};
+                       (int)((n + 127) / 128), (int)m, (int)m, (int)m, 1, y_dtype,
+                       y_dtype != T_F32 && ctx->fp8_cut};
     return run_product(ctx, x_dtype, c, (hipStream_t)stream);
 }
 
@@ -223,7 +224,7 @@ int lloom_hip_fp8_grouped_matmul(lloom_hip_ctx* ctx, const void* w_dev, const fl
     const Fp8Call c = {(const uint8_t*)w_dev, w_scales_dev, x_dev, x_scales_dev, y_dev, (const int*)starts_dev,
                        (const int*)gather_dev, (const int*)scatter_dev, ctx->flags, x_stride, xs_row, xs_block, (int)n,
                        (int)k, (int)((k + 127) / 128), (int)((n + 127) / 128), (int)rows, (int)x_rows, (int)y_rows,
-                       (int)experts, y_dtype};
+                       (int)experts, y_dtype, y_dtype != T_F32 && ctx->fp8_cut};
     return run_product(ctx, x_dtype, c, (hipStream_t)stream);
 }
 

@@ -25,16 +25,18 @@ namespace lloom {
 // barrier through its reads to its products, about 0.5 us whatever the tile and
 // the stages; two waves a SIMD go it at once.
 //
-// Into F16 and BF16 a block of a 16 x 16 tile is one v_mfma_f32_16x16x128_f8f6f4.
-// It adds groups of eight products with 14 bits from the group's largest on (what
-// is under 2^-13 of that is cut), the groups and the blocks in f32: 1.5e-5 of the
-// result in the 2-norm for normal values, where F16's own rounding is 2.1e-4 and
-// BF16's 1.7e-3.  Into F32 (EXACT) the numbers go as halves to v_mfma_f32_32x32x16_
-// f16, whose products are exact and whose sums are f32, at half the rate (8192^3:
-// 527 us and 1030).  Tiles of 32 x 32 for the former: 543, their sums waiting for
-// two chained instructions.
+// The numbers go as halves to v_mfma_f32_32x32x16_f16 (EXACT), whose products are
+// exact and whose sums are f32, into every type of y.  All 8-bit instructions of
+// this chip add groups of eight products with 14 bits from the group's largest on:
+// what is under 2^-13 of that is cut, so that where 448 * 448 and its negative meet,
+// neighbours of up to 24 vanish.  They have twice the rate (8192^3: 483 us and 961), and
+// a caller who would rather have that for F16 and BF16 y says so (MMA_FP8): a block of
+// a 16 x 16 tile is then one v_mfma_f32_16x16x128_f8f6f4, the groups and the blocks
+// are added in f32, and it is 1.5e-5 of the result in the 2-norm for normal values,
+// where F16's own rounding is 2.1e-4 and BF16's 1.7e-3.  Tiles of 32 x 32 for it: 543 us
+// for 527, their sums waiting for two chained instructions.
 //
-// 8192^3 into BF16 is 2090 TFLOP/s; without the loads 424 us, without LDS and
+// 8192^3 into BF16 by MMA_FP8 is 2090 to 2280 TFLOP/s; without the loads 424 us, without LDS and
 // barriers too 382, with zeros for data 493, 354 and 301: the clock falls with the
 // data's bits, and the loads cost a fifth, nearly all of it though every tile come
 // from one place of the L2 (490).
@@ -440,8 +442,8 @@ template <class C>
 static hipError_t tile_with(const Fp8Call& c, hipStream_t s) {
     switch (c.y_type) {
         case T_F32: return tile_of_type<C, true, T_F32>(c, s);
-        case T_F16: return tile_of_type<C, false, T_F16>(c, s);
-        default: return tile_of_type<C, false, T_BF16>(c, s);
+        case T_F16: return c.cut ? tile_of_type<C, false, T_F16>(c, s) : tile_of_type<C, true, T_F16>(c, s);
+        default: return c.cut ? tile_of_type<C, false, T_BF16>(c, s) : tile_of_type<C, true, T_BF16>(c, s);
     }
 }
 
@@ -469,11 +471,11 @@ hipError_t launch_fp8_tile(const Fp8Call& c, hipStream_t s) {
     auto count = [&](int rows, int cols) { return (int64_t)((c.m + rows - 1) / rows) * ((c.n + cols - 1) / cols); };
     const int64_t each = c.m / c.experts;
     const int64_t large = count(256, 256);
-    if (c.y_type != T_F32 && c.nb > 1 && (c.starts ? each >= 512 : large >= 160 && (large <= 256 || large > 320)))
+    if (c.cut && c.nb > 1 && (c.starts ? each >= 512 : large >= 160 && (large <= 256 || large > 320)))
         return c.y_type == T_F16 ? tile_of_type<Fp8Cfg<4, 2, 2, 4, 2>, false, T_F16>(c, s)
                                  : tile_of_type<Fp8Cfg<4, 2, 2, 4, 2>, false, T_BF16>(c, s);
     if (c.starts ? each >= 96 : count(128, 128) >= 300) return tile_with<Fp8Cfg<2, 2, 2, 2, 2>>(c, s);
-    if (!c.starts && count(64, 128) > 256 && count(128, 128) <= 256 && c.kb >= (c.y_type == T_F32 ? 16 : 32))
+    if (!c.starts && count(64, 128) > 256 && count(128, 128) <= 256 && c.kb >= (c.cut ? 32 : 16))
         return tile_with<Fp8Cfg<2, 2, 2, 2, 2, 2>>(c, s);
     const bool parts = c.kb >= 8;
     if (c.starts ? each >= 10 : count(64, 128) > (parts ? 256 : 128)) return tile_with<Fp8Cfg<2, 2, 1, 2, 2>>(c, s);

@@ -44,10 +44,11 @@ pub const LLOOM_HIP_Q8K: c_int = 15;
 pub const LLOOM_HIP_BF16: c_int = 30;
 pub const LLOOM_HIP_E4M3: c_int = 100;
 
-// Prefill operand mode (lloom_hip_ctx_set_prefill_mma).
+// Prefill operand modes (lloom_hip_ctx_set_prefill_mma, lloom_hip_ctx_set_fp8_mma).
 pub const LLOOM_HIP_MMA_F16: c_int = 0;
 pub const LLOOM_HIP_MMA_INT8: c_int = 1;
 pub const LLOOM_HIP_MMA_AUTO: c_int = 2;
+pub const LLOOM_HIP_MMA_FP8: c_int = 3;
 
 // Fused stores (MvStore: none / Silu / MulInto).
 pub const LLOOM_HIP_STORE_PLAIN: c_int = 0;
@@ -65,6 +66,7 @@ extern "C" {
     pub fn lloom_hip_ctx_stream(ctx: *mut lloom_hip_ctx) -> *mut c_void;
     pub fn lloom_hip_ctx_set_mv_rows_max(ctx: *mut lloom_hip_ctx, rows: c_int) -> c_int;
     pub fn lloom_hip_ctx_set_prefill_mma(ctx: *mut lloom_hip_ctx, mode: c_int) -> c_int;
+    pub fn lloom_hip_ctx_set_fp8_mma(ctx: *mut lloom_hip_ctx, mode: c_int) -> c_int;
     pub fn lloom_hip_ctx_sync(ctx: *mut lloom_hip_ctx) -> c_int;
 
     // Device memory (Device::qzeros, load_quantized, QCudaStorage::data).
