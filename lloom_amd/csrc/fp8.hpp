@@ -60,6 +60,11 @@ bool fp8_few_fuses(int x_type, int64_t rows, int64_t k, int64_t experts, bool gr
 hipError_t launch_fp8_few(int x_type, const Fp8Call& c, hipStream_t s);
 // fp8_tile.hip: x E4M3.
 hipError_t launch_fp8_tile(const Fp8Call& c, hipStream_t s);
+// Whether such a launch has fewer threads than the 2^32 that one may have (of a call
+// its sizes and y_type, cut, and whether it has starts).
+constexpr int64_t FP8_THREADS = (int64_t)1 << 32;
+bool fp8_few_fits(int x_type, const Fp8Call& c);
+bool fp8_tile_fits(const Fp8Call& c);
 
 #if defined(__HIP_DEVICE_COMPILE__) || defined(__HIPCC__)
 

@@ -67,17 +67,6 @@ int check_product(const char* what, const void* w, const float* ws, int64_t expe
     return LLOOM_HIP_OK;
 }
 
-// A launch has fewer than 2^32 threads: fp8_few.hip's at most 512 for 16 rows of x
-// and of the weight, fp8_tile.hip's 128 for 32 rows of x and 128 of the weight.
-int check_grid(const char* what, int64_t rows, int64_t n, int64_t experts, bool grouped) {
-    const int64_t more = experts < rows ? experts : rows;
-    const bool fits = fp8_few_rows(rows, n, experts, grouped)
-                          ? (rows / 16 + more + 1) * ((n + 15) / 16) < ((int64_t)1 << 23)
-                          : (rows / 32 + more + 1) * ((n + 127) / 128) < ((int64_t)1 << 25);
-    if (fits) return LLOOM_HIP_OK;
-    return fail(LLOOM_HIP_ESHAPE, "%s: %lld rows by n %lld", what, (long long)rows, (long long)n);
-}
-
 // x in 8 bits, where a call brings it there in a launch before the product's:
 // q [rows][k], then the scales, block by block.
 struct XCopy {
@@ -104,6 +93,24 @@ int check_offsets(const char* what, int x_type, int64_t rows, int64_t x_rows, in
         return LLOOM_HIP_OK;
     return fail(LLOOM_HIP_ESHAPE, "%s: %lld rows of x, %lld bytes apart, or their scales, are past 2^31 bytes", what,
                 (long long)reach, (long long)stride);
+}
+
+// A product's launch, in either mode of lloom_hip_ctx_set_fp8_mma.
+int check_grid(const char* what, int x_type, int64_t rows, int64_t n, int64_t k, int64_t experts, bool grouped) {
+    static const int none = 0;
+    Fp8Call c = {};
+    c.n = (int)n, c.k = (int)k, c.kb = (int)((k + 127) / 128), c.nb = (int)((n + 127) / 128), c.m = (int)rows;
+    c.experts = (int)experts, c.starts = grouped ? &none : nullptr;
+    if (x_type != T_E4M3 && !fp8_few_fuses(x_type, rows, k, experts, grouped)) x_type = T_E4M3;
+    bool fits = true;
+    if (fp8_few_rows(rows, n, experts, grouped)) {
+        fits = fp8_few_fits(x_type, c);
+    } else {
+        for (bool cut : {false, true}) c.cut = cut, c.y_type = cut ? T_F16 : T_F32, fits = fits && fp8_tile_fits(c);
+    }
+    if (fits) return LLOOM_HIP_OK;
+    return fail(LLOOM_HIP_ESHAPE, "%s: %lld rows by n %lld are over the threads of a launch", what, (long long)rows,
+                (long long)n);
 }
 
 int run_product(lloom_hip_ctx* ctx, int x_type, Fp8Call c, hipStream_t s) {
@@ -191,7 +198,7 @@ int lloom_hip_fp8_matmul(lloom_hip_ctx* ctx, const void* w_dev, const float* w_s
                                xs_block, m, y_dev, y_dtype))
         return rc;
     if (int rc = check_offsets("fp8_matmul", x_dtype, m, m, x_stride, xs_row, xs_block, k, 1, false, false)) return rc;
-    if (int rc = check_grid("fp8_matmul", m, n, 1, false)) return rc;
+    if (int rc = check_grid("fp8_matmul", x_dtype, m, n, k, 1, false)) return rc;
     if (m == 0) return LLOOM_HIP_OK;
     HIP_OK(hipSetDevice(ctx->device));
     const Fp8Call c = {(const uint8_t*)w_dev, w_scales_dev, x_dev, x_scales_dev, y_dev, nullptr, nullptr, nullptr,
@@ -218,7 +225,7 @@ int lloom_hip_fp8_grouped_matmul(lloom_hip_ctx* ctx, const void* w_dev, const fl
     if (int rc = check_offsets("fp8_grouped_matmul", x_dtype, rows, x_rows, x_stride, xs_row, xs_block, k, experts, true,
                                gather_dev != nullptr))
         return rc;
-    if (int rc = check_grid("fp8_grouped_matmul", rows, n, experts, true)) return rc;
+    if (int rc = check_grid("fp8_grouped_matmul", x_dtype, rows, n, k, experts, true)) return rc;
     if (rows == 0) return LLOOM_HIP_OK;
     HIP_OK(hipSetDevice(ctx->device));
     const Fp8Call c = {(const uint8_t*)w_dev, w_scales_dev, x_dev, x_scales_dev, y_dev, (const int*)starts_dev,

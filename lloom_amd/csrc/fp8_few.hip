@@ -191,12 +191,18 @@ bool fp8_few_fuses(int x_type, int64_t rows, int64_t k, int64_t experts, bool gr
     return rows <= 16 && rows * ((k + 127) / 128) <= 64 && few_lds(rows, k) <= 65536;
 }
 
-template <int XT, int W, int MT, int NT, int D>
+// W waves, MT tiles of 16 rows of x, NT of the weight, loads of D blocks under way.
+template <int W_, int MT_, int NT_, int D_>
+struct FewCfg {
+    static constexpr int W = W_, MT = MT_, NT = NT_, D = D_;
+};
+template <int XT, class C>
 static hipError_t few_of(const Fp8Call& c, hipStream_t s) {
+    constexpr int W = C::W, MT = C::MT, NT = C::NT;
     const int nblocks = (c.n + 16 * NT - 1) / (16 * NT);
     int lds = W * NT * MT * 64 * 16;
     if (XT != T_E4M3 && few_lds(c.m, c.k) > lds) lds = (int)few_lds(c.m, c.k);
-    k_fp8_few<XT, W, MT, NT, D><<<dim3((uint32_t)(fp8_tiles(c, 16 * MT) * nblocks)), 64 * W, lds, s>>>(c, nblocks);
+    k_fp8_few<XT, W, MT, NT, C::D><<<dim3((uint32_t)(fp8_tiles(c, 16 * MT) * nblocks)), 64 * W, lds, s>>>(c, nblocks);
     return hipGetLastError();
 }
 
@@ -212,22 +218,35 @@ static hipError_t few_of(const Fp8Call& c, hipStream_t s) {
 //   grouped, (16, 16) / (16, 32) / (16, 64): 32 tokens top 8 of 128 experts, [1536,
 //     2048] 85 / 57 / 55 and [2048, 768] 76 / 43 / 33; 4 tokens (29 experts) 24 / 20 /
 //     23; (32, 64) is slower (67), most tiles being far from full
-template <int XT>
-static hipError_t few_with(const Fp8Call& c, hipStream_t s) {
+template <bool E4M3, class F>
+static auto few_choice(const Fp8Call& c, F with) {
     const int64_t groups = c.starts ? (c.experts < c.m ? c.experts : c.m) : 1, tiles = groups * ((c.n + 15) / 16);
-    if constexpr (XT == T_E4M3) {
+    if constexpr (E4M3) {
         if (!c.starts && c.m > 16) {
             auto enough = [&](int rows, int cols) {
                 return (int64_t)((c.m + rows - 1) / rows) * ((c.n + cols - 1) / cols) >= 200;
             };
-            if (enough(32, 64)) return few_of<XT, 4, 2, 4, 1>(c, s);
-            if (enough(32, 32)) return few_of<XT, 4, 2, 2, 1>(c, s);
-            return few_of<XT, 4, 1, 2, 2>(c, s);
+            if (enough(32, 64)) return with(FewCfg<4, 2, 4, 1>{});
+            if (enough(32, 32)) return with(FewCfg<4, 2, 2, 1>{});
+            return with(FewCfg<4, 1, 2, 2>{});
         }
     }
-    if (tiles >= 4096) return few_of<XT, 4, 1, 4, 1>(c, s);
-    if (tiles >= 1024 || (tiles >= 256 && c.m > 4)) return few_of<XT, 4, 1, 2, 2>(c, s);
-    return few_of<XT, 8, 1, 1, 2>(c, s);
+    if (tiles >= 4096) return with(FewCfg<4, 1, 4, 1>{});
+    if (tiles >= 1024 || (tiles >= 256 && c.m > 4)) return with(FewCfg<4, 1, 2, 2>{});
+    return with(FewCfg<8, 1, 1, 2>{});
+}
+
+template <int XT>
+static hipError_t few_with(const Fp8Call& c, hipStream_t s) {
+    return few_choice<XT == T_E4M3>(c, [&](auto cfg) { return few_of<XT, decltype(cfg)>(c, s); });
+}
+
+bool fp8_few_fits(int x_type, const Fp8Call& c) {
+    auto fits = [&](auto cfg) {
+        typedef decltype(cfg) C;
+        return fp8_tiles(c, 16 * C::MT) * ((c.n + 16 * C::NT - 1) / (16 * C::NT)) < FP8_THREADS / (64 * C::W);
+    };
+    return x_type == T_E4M3 ? few_choice<true>(c, fits) : few_choice<false>(c, fits);
 }
 
 hipError_t launch_fp8_few(int x_type, const Fp8Call& c, hipStream_t s) {

@@ -440,11 +440,11 @@ static hipError_t tile_of_type(const Fp8Call& c, hipStream_t s) {
 
 template <class C>
 static hipError_t tile_with(const Fp8Call& c, hipStream_t s) {
-    switch (c.y_type) {
-        case T_F32: return tile_of_type<C, true, T_F32>(c, s);
-        case T_F16: return c.cut ? tile_of_type<C, false, T_F16>(c, s) : tile_of_type<C, true, T_F16>(c, s);
-        default: return c.cut ? tile_of_type<C, false, T_BF16>(c, s) : tile_of_type<C, true, T_BF16>(c, s);
+    if constexpr (C::BM < 256) {  // the large tile's sums and halves of both operands would not fit the registers
+        if (c.y_type == T_F32) return tile_of_type<C, true, T_F32>(c, s);
+        if (!c.cut) return c.y_type == T_F16 ? tile_of_type<C, true, T_F16>(c, s) : tile_of_type<C, true, T_BF16>(c, s);
     }
+    return c.y_type == T_F16 ? tile_of_type<C, false, T_F16>(c, s) : tile_of_type<C, false, T_BF16>(c, s);
 }
 
 // The largest tile that is mostly full and leaves workgroups for all CUs; where the
@@ -466,22 +466,33 @@ static hipError_t tile_with(const Fp8Call& c, hipStream_t s) {
 //     average, (32, 128) / (64, 128) / (128, 128): 71 / 73 / 82, 77 / 75 / 81, 92 / 85 /
 //     94; of 64 [2048, 2048], 256 and 1024: - / 141 / 128 and (256, 256) 134, - / 451 /
 //     402 / 368
-hipError_t launch_fp8_tile(const Fp8Call& c, hipStream_t s) {
-    if (!c.xs && c.x_rows) return hipErrorInvalidValue;  // rows that are not in 8 bits
+template <class F>
+static auto tile_choice(const Fp8Call& c, F with) {
     auto count = [&](int rows, int cols) { return (int64_t)((c.m + rows - 1) / rows) * ((c.n + cols - 1) / cols); };
     const int64_t each = c.m / c.experts;
     const int64_t large = count(256, 256);
     if (c.cut && c.nb > 1 && (c.starts ? each >= 512 : large >= 160 && (large <= 256 || large > 320)))
-        return c.y_type == T_F16 ? tile_of_type<Fp8Cfg<4, 2, 2, 4, 2>, false, T_F16>(c, s)
-                                 : tile_of_type<Fp8Cfg<4, 2, 2, 4, 2>, false, T_BF16>(c, s);
-    if (c.starts ? each >= 96 : count(128, 128) >= 300) return tile_with<Fp8Cfg<2, 2, 2, 2, 2>>(c, s);
+        return with(Fp8Cfg<4, 2, 2, 4, 2>{});
+    if (c.starts ? each >= 96 : count(128, 128) >= 300) return with(Fp8Cfg<2, 2, 2, 2, 2>{});
     if (!c.starts && count(64, 128) > 256 && count(128, 128) <= 256 && c.kb >= (c.cut ? 32 : 16))
-        return tile_with<Fp8Cfg<2, 2, 2, 2, 2, 2>>(c, s);
+        return with(Fp8Cfg<2, 2, 2, 2, 2, 2>{});
     const bool parts = c.kb >= 8;
-    if (c.starts ? each >= 10 : count(64, 128) > (parts ? 256 : 128)) return tile_with<Fp8Cfg<2, 2, 1, 2, 2>>(c, s);
-    if (c.starts || !parts) return tile_with<Fp8Cfg<1, 2, 1, 2, 3>>(c, s);
-    if (count(64, 128) > 128) return tile_with<Fp8Cfg<2, 2, 1, 2, 3, 2>>(c, s);
-    return tile_with<Fp8Cfg<1, 2, 1, 2, 3, 2>>(c, s);
+    if (c.starts ? each >= 10 : count(64, 128) > (parts ? 256 : 128)) return with(Fp8Cfg<2, 2, 1, 2, 2>{});
+    if (c.starts || !parts) return with(Fp8Cfg<1, 2, 1, 2, 3>{});
+    if (count(64, 128) > 128) return with(Fp8Cfg<2, 2, 1, 2, 3, 2>{});
+    return with(Fp8Cfg<1, 2, 1, 2, 3, 2>{});
+}
+
+hipError_t launch_fp8_tile(const Fp8Call& c, hipStream_t s) {
+    if (!c.xs && c.x_rows) return hipErrorInvalidValue;  // rows that are not in 8 bits
+    return tile_choice(c, [&](auto cfg) { return tile_with<decltype(cfg)>(c, s); });
+}
+
+bool fp8_tile_fits(const Fp8Call& c) {
+    return tile_choice(c, [&](auto cfg) {
+        typedef decltype(cfg) C;
+        return fp8_tiles(c, C::BM) * ((c.n + C::BN - 1) / C::BN) < FP8_THREADS / C::THREADS;
+    });
 }
 
 }  // namespace lloom

@@ -196,3 +196,16 @@ def test_modes_that_are_none_are_refused(L):
         with pytest.raises(L.LloomHipError) as e:
             L.set_fp8_mma(mode)
         assert e.value.name == "EINVAL"
+
+
+# ------------------------------------------------------------------- sizes --
+
+def test_many_experts_of_few_rows_by_a_long_n(L):
+    """4096 experts of four rows each by 32768 columns: within a launch's threads with the tiles that serve them."""
+    E, n, k = 4096, 32768, 16
+    w = torch.randint(0, 0x60, (E, n, k), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    ws = torch.rand(E, n // 128, 1, device="cuda")
+    q, sx = L.fp8_quantize(normal(1, 4 * E, k).cuda())
+    y = L.fp8_grouped_matmul(q, w, ws, (4 * torch.arange(E + 1)).int().cuda(), x_scales=sx, out_dtype=F16)
+    for e in (0, 1, 2047, E - 1):
+        check_rows(y[4 * e:4 * e + 4].cpu(), q[4 * e:4 * e + 4].cpu(), sx[4 * e:4 * e + 4], w[e].cpu(), ws[e], torch.arange(4))
