@@ -46,13 +46,15 @@ hipError_t launch_fp8_weights(int type, const void* w, int64_t planes, int64_t n
 hipError_t launch_expert_plan(const int* ids, int64_t planes, int topk, int experts, int* starts, int* sorted,
                               int* tokens, int* flags, hipStream_t s);
 // Whether fp8_few.hip serves a call (else fp8_tile.hip).  Its workgroups' tiles
-// meet no other's, so it keeps all CUs busy with small outputs.  us of the two into
-// bf16: 64 rows of [4096, 4096] 10.8 / 13.5, 128 15.0 / 13.6 (into f32 14.9 / 18.3), 32 of
-// [8192, 8192] 21.0 / 29.3, 64 30.6 / 29.0, 96 of [8192, 2048] 12.7 / 8.9.  Grouped, with
-// 4, 8 and 12 rows an expert on average: [128, 1536, 2048] 67, 79, 88 against 67, 72, 75,
-// [128, 2048, 768] 41, 50, 55 / 41, 46, 49.
+// meet no other's, so it keeps all CUs busy with small outputs.  us of the two: 64 rows
+// of [4096, 4096] 10.9 / 17.0, 128 14.9 / 17.2, 256 25.9 / 17.8; 32 of [8192, 8192] 21 / 32, 64 30.6 / 32.3,
+// 128 52 / 33; 64 of [8192, 2048] 9.6 / 10.5, 96 15.2 / 10.9, 64 of [8192, 512] 5.4 / 5.8, 96 7.0 / 6.0;
+// 256 of [2048, 8192] 25 / 30 (by MMA_FP8 the other is up to a tenth faster at the limit, 128 of [4096,
+// 4096] 13.6).  Grouped, with 4, 6 and 8 rows an expert on average: [128, 1536, 2048] 67, 71, 77
+// against 73, 74, 75, [128, 2048, 768] 4: 41.7 / 40.6; of small outputs 4 experts of 64 rows by 264
+// 8.6 / 11.1, 64 of 8 by 256 12.9 / 12.5, by 512 19.7 / 16.1, 16 of 10 by 2048 13.1 / 11.0.
 inline bool fp8_few_rows(int64_t rows, int64_t n, int64_t experts, bool grouped) {
-    return rows <= 16 || (grouped ? rows <= 4 * experts : rows * n <= 128 * 4096);
+    return rows <= 16 || (grouped ? rows <= 4 * experts || rows * n <= 128 * 1024 : rows * n <= 128 * 4096);
 }
 // fp8_few.hip: x E4M3, or any type where fp8_few_fuses (it is brought into 8 bits
 // by each workgroup; only calls that fp8_few_rows gives to it).

@@ -448,38 +448,45 @@ static hipError_t tile_with(const Fp8Call& c, hipStream_t s) {
 }
 
 // The largest tile that is mostly full and leaves workgroups for all CUs; where the
-// small ones are one round, k in two parts.  us by (rows of x, of the weight) a tile:
-//   (32, 128) / the same, two parts / (64, 128), two parts / (64, 128): 128 rows of
-//     [8192, 8192] 36 / 30 / 34 / 55, 256 of [4096, 4096] 18.4 / 14.4 / 16.2 / 21, into f32
-//     26 / 19 / 23 / 27, 192 of [6144, 2048] 13.4 / 16.1 / 10.2 / 12.6, 320 of [4096, 4096]
-//     - / 26 / 16 / 19, 509 22 / - / 16.7, 130 of [8192, 1024] 9.0 / 11.3 / 7.7 / 8.2, 128
-//     of [8192, 512] 5.7 / 5.9 / 6.5 / 6.1, 192 of [6144, 512] 6.4 / 9.4 / 6.2 / 5.8; six
-//     stages for three 36.4 in the first
-//   (64, 128) / (128, 128), two parts, into bf16 and into f32: 260 rows of [8192, 2048]
-//     15.1 / 15.6, 24.0 / 22.3; 400 of [6144, 4096] 24.9 / 23.8, 38.3 / 34.9; 384 of [8192,
-//     8192] 57 / 49, 76 / 66; 640 of [4096, 1024] 9.5 / 10.5, 14.6 / 15.0
-//   (64, 128) / (128, 128) / (256, 256): 509 rows of [8192, 2048] 15.8 / 17.8 / -, into
-//     f32 24.7 / 25.8; 1200 34 / 35 / 32, 1400 38 / 39 / 33, 2048 59 / 48 / 41, 2304 (a round of
-//     256 large tiles and 32 more) 62 / 58 / 63, 2560 67 / 60 / 63, 3000 77 / 68 / 65; 44000 of [112, 1264] -
-//     / 27 / 32, 20000 of [300, 4096] - / 44 / 45; 4096 of [4096, 4096] into f32 152 / 136
-//   grouped, top 8 of 128 experts [1536, 2048], 8, 12 and 32 rows an expert on
-//     average, (32, 128) / (64, 128) / (128, 128): 71 / 73 / 82, 77 / 75 / 81, 92 / 85 /
-//     94; of 64 [2048, 2048], 256 and 1024: - / 141 / 128 and (256, 256) 134, - / 451 /
-//     402 / 368
+// small ones are one round, k in two parts.  The rule is one for all types of y and
+// for grouped calls, whose groups' last tiles are taken as half full (a group's rows
+// are known on the GPU alone).  us by (rows of x, of the weight) a tile, into bf16:
+//   (32, 128) / two parts / (64, 128) / two parts / (128, 128) / two parts:
+//     256 rows of [4096, 4096] 25.9 / 17.8 / 26.0 / 22.0 / 36 / 31, 509 36 / 33 / 27.5 / 24.3 / 37 / 32,
+//     1000 67 / 63 / 43 / 45 / 40 / 36; 384 of [8192, 8192] 110 / 89 / 77 / 80 / 71 / 65; 96 of [8192,
+//     2048] 14.7 / 10.9 / 15.0 / 13.4 / 20.6 / 18.5, 509 37 / 38 / 24.2 / 27.2 / 23.6 / 22.1, 1200 83 /
+//     90 / 53 / 64 / 54 / 58, 2048 133 / 150 / 80 / 106 / 71 / 83; 96 of [8192, 512] 6.2 / 6.0 / 6.6 /
+//     7.0 / 8.5 / 8.8; 2000 of [264, 2048] 14.6 / 10.8 / 14.9 / 13.2 / 20.6 / 18.5, 44000 of [112, 1264] 42 /
+//     52 / 28 / 38 / 30 / 37, 20000 of [300, 4096] 126 / 131 / 79 / 91 / 70 / 78
+//   grouped, the same: top 8 of 128 experts [1536, 2048], 8, 32 and 128 rows an expert on
+//     average, 75 / 84 / 75 / 92 / 98 / 114, 100 / 116 / 91 / 110 / 111 / 132, 241 / 295 / 167 / 222 /
+//     172 / 209; of 64 [2048, 2048], 1024 rows 1098 / 1326 / 636 / 860 / 580 / 693; of 4
+//     [264, 2048], 256 rows 15.4 / 11.7 / 15.9 / 13.9 / 21.5 / 19.4, 2048 38 / 41 / 24.5 / 29 / 24.6 /
+//     22.8; of 8 [1024, 1024], 128 rows 12.8 / 14.5 / 10.5 / 10.1 / 13.6 / 13.4, [512, 4096], 512 rows
+//     57 / 53 / 40 / 46 / 39 / 36; of 64 [512, 2048], 8 rows 17.6 / 16.1 / 20.0 / 17.5 / - / -
+// With MMA_FP8, and (256, 256) where its rounds of 256 are full by 5 / 8 on average:
+//   (64, 128) / (128, 128) / (256, 256): 1200 rows of [8192, 2048] 34 / 35 / 34, 1400 40 / 39 / 34,
+//     2304 (288 large tiles) 65 / 61 / 63, 3000 77 / 69 / 66, 4160 (544 of them) 109 / 99 / 94,
+//     4400 110 / 97 / 98, 6200 154 / 136 / 131, 8192^3 704 / 601 / 483; grouped, of 8 experts, 2048
+//     rows by 2048, [512, 2048] 36 / 39 / 36, [1024, 2048] (272 tiles) 64 / 61 / 63, [1536, 2048] 94 /
+//     84 / 70; of 64 [2048, 2048], 1024 rows 462 / 405 / 346
 template <class F>
 static auto tile_choice(const Fp8Call& c, F with) {
-    auto count = [&](int rows, int cols) { return (int64_t)((c.m + rows - 1) / rows) * ((c.n + cols - 1) / cols); };
-    const int64_t each = c.m / c.experts;
-    const int64_t large = count(256, 256);
-    if (c.cut && c.nb > 1 && (c.starts ? each >= 512 : large >= 160 && (large <= 256 || large > 320)))
-        return with(Fp8Cfg<4, 2, 2, 4, 2>{});
-    if (c.starts ? each >= 96 : count(128, 128) >= 300) return with(Fp8Cfg<2, 2, 2, 2, 2>{});
-    if (!c.starts && count(64, 128) > 256 && count(128, 128) <= 256 && c.kb >= (c.cut ? 32 : 16))
+    const int64_t groups = c.experts < c.m ? c.experts : c.m, each = c.starts ? c.m / c.experts : c.m;
+    auto count = [&](int rows, int cols) {
+        const int64_t tiles = c.starts ? c.m / rows + (groups + 1) / 2 : (c.m + rows - 1) / rows;
+        return tiles * ((c.n + cols - 1) / cols);
+    };
+    const int64_t large = count(256, 256), rounds = (large + 255) / 256;
+    if (c.cut && c.nb > 1 && (!c.starts || each >= 512) && 8 * large >= 5 * 256 * rounds) return with(Fp8Cfg<4, 2, 2, 4, 2>{});
+    const bool full = !c.starts || each >= 96, half = !c.starts || each >= 10;  // tiles of 128 rows, of 64
+    if (full && count(128, 128) >= 300) return with(Fp8Cfg<2, 2, 2, 2, 2>{});
+    if (full && count(64, 128) > 256 && count(128, 128) <= 256 && c.kb >= (c.cut ? 32 : 16))
         return with(Fp8Cfg<2, 2, 2, 2, 2, 2>{});
     const bool parts = c.kb >= 8;
-    if (c.starts ? each >= 10 : count(64, 128) > (parts ? 256 : 128)) return with(Fp8Cfg<2, 2, 1, 2, 2>{});
-    if (c.starts || !parts) return with(Fp8Cfg<1, 2, 1, 2, 3>{});
-    if (count(64, 128) > 128) return with(Fp8Cfg<2, 2, 1, 2, 3, 2>{});
+    if (half && count(64, 128) > (parts ? 256 : 128)) return with(Fp8Cfg<2, 2, 1, 2, 2>{});
+    if (!parts || count(64, 128) > 256) return with(Fp8Cfg<1, 2, 1, 2, 3>{});
+    if (half && count(64, 128) > 128) return with(Fp8Cfg<2, 2, 1, 2, 3, 2>{});
     return with(Fp8Cfg<1, 2, 1, 2, 3, 2>{});
 }
 

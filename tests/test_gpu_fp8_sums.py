@@ -67,10 +67,10 @@ def test_neighbours_that_cancel_by_expert(L, each, out):
 # (m, n, k) of every kernel and tile by number of steps: few rows; 32 x 128 and 64 x 128 with k in one part and in two; 128 x 128
 # in two parts and in one, with one step, some, and past the 64 blocks whose scales a wave holds; ends inside tiles
 SHAPES = [(3, 264, 656), (16, 4104, 2064), (64, 4096, 656), (17, 257, 1040), (128, 2050, 8336),  # few rows
-          (300, 3001, 400), (1030, 1000, 400),       # 32 x 128
-          (300, 3001, 1040), (200, 4100, 8336),      # 32 x 128, two parts
-          (1400, 1500, 656), (700, 5000, 400),       # 64 x 128
-          (540, 2900, 1168), (400, 5200, 1424),      # 64 x 128, two parts
+          (300, 3001, 400), (700, 1000, 400), (600, 1000, 16),  # 32 x 128
+          (300, 3001, 1040), (200, 3100, 8336),      # 32 x 128, two parts
+          (1400, 1500, 656), (700, 5000, 400), (1030, 1000, 272),  # 64 x 128
+          (540, 2900, 1168), (400, 4200, 8208),      # 64 x 128, two parts
           (700, 4100, 4112), (1000, 4001, 2192),     # 128 x 128, two parts
           (3400, 3101, 656), (2304, 8200, 1168), (2500, 2100, 8336), (20000, 300, 1264), (5000, 1300, 16), (3000, 1800, 272)]
 
@@ -111,14 +111,20 @@ def grouped_sums(L, counts, extra, n, k, out, groups8):
     return plain
 
 
-# ragged groups, some empty, by rows of an expert on average and n: few rows; 32 x 128; 64 x 128; 128 x 128; and what is 256 x 256
-# with MMA_FP8 (513 and more rows), whose tiles are no multiple of 4 or 8 and whose last blocks of n are not full
 COUNTS = [[1, 0, 2, 1, 0, 4, 3], [3, 9, 0, 14, 2, 7, 5], [16, 40, 0, 33, 64, 65, 15, 1], [250, 0, 129, 128, 127, 1],
           [513, 0, 700, 1030, 1, 900], [2049, 0, 3, 256], [600, 600, 600, 600, 512, 513, 511, 1025, 0]]
+LONG = [[6000, 0, 9000, 13001, 512, 12600], [3000, 0, 5001, 4100, 700, 1500]]
+# (groups, some empty and some that end inside a tile; n, k) of every kernel and tile, with one step, some, and over 64
+GROUPED = [(COUNTS[0], 700, 656), (COUNTS[1], 264, 1168), (COUNTS[2], 257, 8336), (COUNTS[3], 129, 656), ([3] * 300, 600, 272),  # few
+           (COUNTS[1], 4100, 400), (COUNTS[3], 700, 656), (COUNTS[5], 264, 16), ([7, 0, 9] * 90, 1500, 2064),  # 32 x 128
+           (COUNTS[1], 4100, 1168), (COUNTS[3], 264, 1168), (COUNTS[5], 257, 8336),  # the same, two parts
+           (COUNTS[4], 264, 656), (COUNTS[6], 700, 400), (COUNTS[3], 2200, 16), (COUNTS[4], 1280, 8336),  # 64 x 128
+           (COUNTS[6], 257, 1168), (COUNTS[4], 384, 8336),  # the same, two parts
+           (COUNTS[4], 2200, 400), (COUNTS[6], 2200, 1168), (LONG[0], 200, 272), (LONG[1], 700, 656),  # 128 x 128
+           (COUNTS[4], 700, 2192), (COUNTS[5], 900, 8336)]  # the same, two parts
 
 
-@pytest.mark.parametrize("n,k", [(264, 656), (129, 1168), (700, 656), (2200, 400), (257, 8336)])
-@pytest.mark.parametrize("counts", COUNTS)
+@pytest.mark.parametrize("counts,n,k", GROUPED)
 def test_one_sum_for_all_types_by_expert(L, counts, n, k):
     y = grouped_sums(L, counts, 9, n, k, F32, False)
     for out in (F16, BF16):
@@ -162,24 +168,31 @@ def test_cut_sums(L, fp8_mma, m, n, k, out):
     assert 0 < far <= (3e-5 * 2 * R.EPS[out]) ** 0.5
 
 
+# by expert, with MMA_FP8: a tile of each size, and (256, 256) by one, three and nine tiles of n, whose tiles of rows are no
+# multiple of the four that are walked together nor of the eight XCDs, with 1, 2, 3, 6 and over 64 steps
+CUT_GROUPED = [(COUNTS[3], 700, 656), (COUNTS[3], 264, 1168), (COUNTS[4], 264, 656), (COUNTS[6], 257, 1168), (COUNTS[4], 2200, 400),
+               (COUNTS[5], 900, 8336), (LONG[0], 200, 272), (LONG[0], 256, 16), (LONG[1], 700, 656), (LONG[1], 641, 256),
+               (COUNTS[6], 2200, 656), (COUNTS[6], 2200, 8336)]
+
+
 @pytest.mark.parametrize("out", [F16, BF16])
-@pytest.mark.parametrize("n,k", [(264, 656), (129, 1168), (700, 656), (257, 8336)])
-@pytest.mark.parametrize("counts", COUNTS[2:])
+@pytest.mark.parametrize("counts,n,k", CUT_GROUPED)
 def test_cut_sums_by_expert(L, fp8_mma, counts, n, k, out):
     grouped_sums(L, counts, 9, n, k, out, True)
 
 
-@pytest.mark.parametrize("counts", COUNTS[4:])
+@pytest.mark.parametrize("counts,n", [(COUNTS[6], 2200), (LONG[0], 200), (LONG[1], 700)])
 @pytest.mark.parametrize("starts", [[1, 2, 3], [0, 5, 3], [0, -1, 3], [0, 2, 1 << 30]])
-def test_cut_sums_of_starts_out_of_order(L, fp8_mma, counts, starts):
-    w, ws = weights(2, len(counts), 700, 272)
+def test_cut_sums_of_starts_out_of_order(L, fp8_mma, counts, n, starts):
+    """On tiles of (256, 256)."""
+    w, ws = weights(2, len(counts), n, 272)
     rows = sum(counts)
     bad = torch.tensor([0] + np.cumsum(counts).tolist(), dtype=torch.int32)
     bad[:3] = torch.tensor(starts, dtype=torch.int32)
     y = L.fp8_grouped_matmul(normal(3, rows, 272, dtype=F16).cuda(), w.cuda(), ws.cuda(), bad.cuda())
     with pytest.raises(L.LloomHipError) as e:
         L.paged_check()
-    assert e.value.name == "EEXPERT" and y.shape == (rows, 700) and not y.any()
+    assert e.value.name == "EEXPERT" and y.shape == (rows, n) and not y.any()
     L.paged_check()
 
 
