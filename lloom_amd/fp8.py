@@ -222,8 +222,10 @@ def expert_plan(ids, experts):
 
 
 def _index(t, i, what):
-    if t is None:
+    if t is None and what != "starts":
         return 0
+    if not isinstance(t, torch.Tensor):
+        raise LloomHipError(1, f"fp8_grouped_matmul: {what} is a {type(t).__name__}, no tensor")
     if t.dtype is not torch.int32 or t.dim() != 1 or t.get_device() != i or not t.is_contiguous():
         raise LloomHipError(2, f"fp8_grouped_matmul: {what} {tuple(t.shape)} {t.dtype} on {t.device} is not a dense int32 "
                                f"tensor of one dimension on GPU {i}")

@@ -1,0 +1,24 @@
+"""Calls of the 8-bit floating-point operators that are refused by name, whatever is wrong with them, and values that are held
+to the last bit."""
+import pytest
+import torch
+
+from .test_gpu_fp8 import ACTS, F16, F32, L, check_product, normal, weights  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def refused(L, name, call):
+    with pytest.raises(L.LloomHipError) as e:
+        call()
+    assert e.value.name == name, str(e.value)
+
+
+def test_starts_that_are_no_tensor(L):
+    w, ws = (t.cuda() for t in weights(1, 3, 200, 256))
+    x = torch.zeros(5, 256, device="cuda")
+    for starts in (None, [0, 1, 2, 5], 0):
+        refused(L, "EINVAL", lambda: L.fp8_grouped_matmul(x, w, ws, starts))
+    starts = torch.tensor([0, 1, 2, 5], dtype=torch.int32, device="cuda")
+    refused(L, "EINVAL", lambda: L.fp8_grouped_matmul(x, w, ws, starts, gather=[0, 1, 2, 3, 4]))
+    refused(L, "EINVAL", lambda: L.fp8_grouped_matmul(x, w, ws, starts, scatter=[0, 1, 2, 3, 4]))
