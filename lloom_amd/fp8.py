@@ -28,6 +28,7 @@ E4M3 = torch.float8_e4m3fn
 _IDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30, E4M3: 100}
 BLOCK = 128
 MMA_FP8 = 3
+MAX_EXPERTS = 4096  # the library refuses more
 
 
 class ExpertPlan(NamedTuple):
@@ -211,7 +212,7 @@ def expert_plan(ids, experts):
         ids = ids.contiguous()
     tokens, topk = ids.shape
     p = tokens * topk
-    buf = ids.new_empty(2 * p + max(experts, 0) + 1)
+    buf = ids.new_empty(2 * p + min(max(experts, 0), MAX_EXPERTS) + 1)
     base = buf.data_ptr()
     rc = lib().lloom_hip_expert_plan(ctx, ids.data_ptr(), tokens, topk, experts, base + 8 * p, base, base + 4 * p,
                                      _stream_of(ids.get_device()))

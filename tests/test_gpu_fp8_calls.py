@@ -22,3 +22,14 @@ def test_starts_that_are_no_tensor(L):
     starts = torch.tensor([0, 1, 2, 5], dtype=torch.int32, device="cuda")
     refused(L, "EINVAL", lambda: L.fp8_grouped_matmul(x, w, ws, starts, gather=[0, 1, 2, 3, 4]))
     refused(L, "EINVAL", lambda: L.fp8_grouped_matmul(x, w, ws, starts, scatter=[0, 1, 2, 3, 4]))
+
+
+def test_more_experts_than_there_may_be(L):
+    """Refused by their number, before memory for so many starts is asked for."""
+    ids = torch.zeros(4, 2, dtype=torch.int32, device="cuda")
+    free = torch.cuda.memory_reserved()
+    for experts in (4097, 1 << 34, 1 << 45):
+        refused(L, "ESHAPE", lambda: L.expert_plan(ids, experts))
+    refused(L, "EINVAL", lambda: L.expert_plan(ids, -(1 << 45)))
+    assert torch.cuda.memory_reserved() - free <= 2 << 20
+    assert L.expert_plan(ids, 4096).starts.shape == (4097,)
