@@ -351,9 +351,10 @@ int lloom_hip_paged_attention_workspace_bytes(int64_t tokens, int64_t requests, 
  * [n][k] of bytes with scales [ceil(n / 128)][ceil(k / 128)], as checkpoints
  * hold them; k is a multiple of 16, at most 2^22.  Activations are F32, F16 or
  * BF16, or E4M3 with a scale for each block of a row.  Rows and weights 16-byte
- * aligned; at most 2^24 rows and n, 4096 experts, and 2^32 threads a launch (as a
- * rule one for 64 values of y, in tiles that a group's few rows do not fill); x that is gathered from, in 8
- * bits, and the scales are under 2^31 bytes.  A block's sum is formed first and the
+ * aligned; at most 2^24 rows and n, 4096 experts, and under 2^32 threads a launch
+ * (about one for 64 values of y, in tiles that a group's few rows do not fill); x
+ * that is gathered from, in 8 bits, and the scales are under 2^31 bytes.  An output
+ * shares no memory with an input or another output (EINVAL).  A block's sum is formed first and the
  * product of its two scales, rounded to f32, meets it: scales whose product is below
  * 2^-126 lose bits, and over f32's largest a sum of zero gives NaN.  Products are
  * exact and sums f32 into every type of y (but for lloom_hip_ctx_set_fp8_mma), which

@@ -42,6 +42,35 @@ int check_rows(const char* what, int type, const void* x, int64_t stride, int64_
     return LLOOM_HIP_OK;
 }
 
+// Bytes that a call reads or writes: rows of `row` bytes, `apart` from each other.
+struct Span {
+    const void* at;
+    int64_t rows, apart, row;
+};
+// Workgroups read what others have written already where an output shares memory
+// with an input or another output.
+int check_apart(const char* what, const Span* out, int outs, const Span* in, int ins) {
+    auto meet = [](const Span& a, const Span& b) {
+        if (!a.at || !b.at || a.rows < 1 || b.rows < 1) return false;
+        typedef unsigned __int128 Address;  // rows may be any number of bytes apart
+        auto end = [](const Span& s) { return (Address)(uintptr_t)s.at + (Address)(s.rows - 1) * s.apart + s.row; };
+        return (uintptr_t)a.at < end(b) && (uintptr_t)b.at < end(a);
+    };
+    for (int i = 0; i < outs; i++) {
+        for (int j = 0; j < ins; j++)
+            if (meet(out[i], in[j])) return fail(LLOOM_HIP_EINVAL, "%s: an output overlaps an input", what);
+        for (int j = 0; j < i; j++)
+            if (meet(out[i], out[j])) return fail(LLOOM_HIP_EINVAL, "%s: outputs overlap", what);
+    }
+    return LLOOM_HIP_OK;
+}
+Span rows_span(int type, const void* x, int64_t stride, int64_t rows, int64_t k) {
+    return {x, rows, stride * type_bytes(type), k * type_bytes(type)};
+}
+Span scales_span(const float* s, int64_t rows, int64_t row, int64_t blocks, int64_t block) {
+    return {rows > 0 ? s : nullptr, blocks, 4 * block, 4 * ((rows - 1) * row + 1)};
+}
+
 int check_product(const char* what, const void* w, const float* ws, int64_t experts, int64_t n, int64_t k, const void* x,
                   int x_type, int64_t x_stride, const float* xs, int64_t xs_row, int64_t xs_block, int64_t x_rows,
                   const void* y, int y_type) {
@@ -145,6 +174,9 @@ int lloom_hip_fp8_quantize(lloom_hip_ctx* ctx, const void* x_dev, int x_dtype, i
                     (long long)scales_stride);
     if ((uintptr_t)q_dev % 8 || (uintptr_t)scales_dev % 4)
         return fail(LLOOM_HIP_EINVAL, "fp8_quantize: q must be 8-byte, scales 4-byte aligned");
+    const Span out[] = {{q_dev, rows, k, k}, scales_span(scales_dev, rows, 1, (k + 127) / 128, scales_stride)};
+    const Span in = rows_span(x_dtype, x_dev, x_stride, rows, k);
+    if (int rc = check_apart("fp8_quantize", out, 2, &in, 1)) return rc;
     if (rows == 0) return LLOOM_HIP_OK;
     HIP_OK(hipSetDevice(ctx->device));
     HIP_OK(launch_fp8_rows(x_dtype, x_dev, x_stride, nullptr, 0, rows, k, q_dev, scales_dev, scales_stride,
@@ -166,6 +198,9 @@ int lloom_hip_fp8_silu_mul(lloom_hip_ctx* ctx, const void* gate_dev, int64_t gat
                     (long long)scales_stride);
     if ((uintptr_t)q_dev % 8 || (uintptr_t)scales_dev % 4)
         return fail(LLOOM_HIP_EINVAL, "fp8_silu_mul: q must be 8-byte, scales 4-byte aligned");
+    const Span out[] = {{q_dev, rows, k, k}, scales_span(scales_dev, rows, 1, (k + 127) / 128, scales_stride)};
+    const Span in[] = {rows_span(dtype, gate_dev, gate_stride, rows, k), rows_span(dtype, up_dev, up_stride, rows, k)};
+    if (int rc = check_apart("fp8_silu_mul", out, 2, in, 2)) return rc;
     if (rows == 0) return LLOOM_HIP_OK;
     HIP_OK(hipSetDevice(ctx->device));
     HIP_OK(launch_fp8_rows(dtype, gate_dev, gate_stride, up_dev, up_stride, rows, k, q_dev, scales_dev, scales_stride,
@@ -185,6 +220,10 @@ int lloom_hip_fp8_quantize_weight(lloom_hip_ctx* ctx, const void* w_dev, int w_d
                     (long long)k);
     if ((uintptr_t)w_dev % 16 || (uintptr_t)q_dev % 8 || (uintptr_t)scales_dev % 4)
         return fail(LLOOM_HIP_EINVAL, "fp8_quantize_weight: the weight must be 16-byte, q 8-byte, scales 4-byte aligned");
+    const int64_t blocks = experts * ((n + 127) / 128) * ((k + 127) / 128);
+    const Span out[] = {{q_dev, experts * n, k, k}, {scales_dev, blocks, 4, 4}};
+    const Span in = rows_span(w_dtype, w_dev, k, experts * n, k);
+    if (int rc = check_apart("fp8_quantize_weight", out, 2, &in, 1)) return rc;
     HIP_OK(hipSetDevice(ctx->device));
     HIP_OK(launch_fp8_weights(w_dtype, w_dev, experts, n, k, q_dev, scales_dev, (hipStream_t)stream));
     return LLOOM_HIP_OK;
@@ -199,6 +238,11 @@ int lloom_hip_fp8_matmul(lloom_hip_ctx* ctx, const void* w_dev, const float* w_s
         return rc;
     if (int rc = check_offsets("fp8_matmul", x_dtype, m, m, x_stride, xs_row, xs_block, k, 1, false, false)) return rc;
     if (int rc = check_grid("fp8_matmul", x_dtype, m, n, k, 1, false)) return rc;
+    const int64_t kb = (k + 127) / 128;
+    const Span out = {y_dev, m, n * type_bytes(y_dtype), n * type_bytes(y_dtype)};
+    const Span in[] = {rows_span(x_dtype, x_dev, x_stride, m, k), {w_dev, n, k, k}, {w_scales_dev, (n + 127) / 128, 4 * kb, 4 * kb},
+                       scales_span(x_dtype == T_E4M3 ? x_scales_dev : nullptr, m, xs_row, kb, xs_block)};
+    if (int rc = check_apart("fp8_matmul", &out, 1, in, 4)) return rc;
     if (m == 0) return LLOOM_HIP_OK;
     HIP_OK(hipSetDevice(ctx->device));
     const Fp8Call c = {(const uint8_t*)w_dev, w_scales_dev, x_dev, x_scales_dev, y_dev, nullptr, nullptr, nullptr,
@@ -226,6 +270,13 @@ int lloom_hip_fp8_grouped_matmul(lloom_hip_ctx* ctx, const void* w_dev, const fl
                                gather_dev != nullptr))
         return rc;
     if (int rc = check_grid("fp8_grouped_matmul", x_dtype, rows, n, k, experts, true)) return rc;
+    const int64_t kb = (k + 127) / 128;
+    const Span out = {y_dev, y_rows, n * type_bytes(y_dtype), n * type_bytes(y_dtype)};
+    const Span in[] = {rows_span(x_dtype, x_dev, x_stride, x_rows, k), {w_dev, experts * n, k, k},
+                       {w_scales_dev, experts * ((n + 127) / 128), 4 * kb, 4 * kb},
+                       scales_span(x_dtype == T_E4M3 ? x_scales_dev : nullptr, x_rows, xs_row, kb, xs_block),
+                       {starts_dev, experts + 1, 4, 4}, {gather_dev, rows, 4, 4}, {scatter_dev, rows, 4, 4}};
+    if (int rc = check_apart("fp8_grouped_matmul", &out, 1, in, 7)) return rc;
     if (rows == 0) return LLOOM_HIP_OK;
     HIP_OK(hipSetDevice(ctx->device));
     const Fp8Call c = {(const uint8_t*)w_dev, w_scales_dev, x_dev, x_scales_dev, y_dev, (const int*)starts_dev,
@@ -245,6 +296,10 @@ int lloom_hip_expert_plan(lloom_hip_ctx* ctx, const uint32_t* ids_dev, int64_t t
     if (topk > MOE_MAX_EXPERTS || experts > MOE_MAX_EXPERTS || tokens > MAX_ROWS || tokens * topk >= MAX_ROWS)
         return fail(LLOOM_HIP_ESHAPE, "expert_plan: %lld tokens of %lld (under %lld planes), %lld experts (at most %d)",
                     (long long)tokens, (long long)topk, (long long)MAX_ROWS, (long long)experts, MOE_MAX_EXPERTS);
+    const int64_t planes = tokens * topk;
+    const Span out[] = {{starts_dev, experts + 1, 4, 4}, {planes_dev, planes, 4, 4}, {tokens_dev, planes, 4, 4}};
+    const Span in = {ids_dev, planes, 4, 4};
+    if (int rc = check_apart("expert_plan", out, 3, &in, 1)) return rc;
     HIP_OK(hipSetDevice(ctx->device));
     HIP_OK(launch_expert_plan((const int*)ids_dev, tokens * topk, (int)topk, (int)experts, (int*)starts_dev,
                               (int*)planes_dev, (int*)tokens_dev, ctx->flags, (hipStream_t)stream));

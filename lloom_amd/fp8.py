@@ -182,7 +182,8 @@ def _check_out(out, shape, dtype, i, what):
 def fp8_matmul(x, weight, weight_scales, x_scales=None, out_dtype=None, out=None):
     """x . W^T for a weight e4m3 [n, k] with f32 scales [ceil(n / 128), ceil(k / 128)]; x [.., k] f32, f16 or bf16 (brought
     into 8 bits as fp8_quantize does), or e4m3 with x_scales [rows, ceil(k / 128)].  The result [.., n] is of out_dtype (x's
-    own by default, f32 for e4m3 x): exact products, sums in f32 (but for set_fp8_mma), rounded once."""
+    own by default, f32 for e4m3 x): exact products, sums in f32 (but for set_fp8_mma), rounded once.  `out`
+    shares no memory with what the call reads."""
     ctx = _gpu(weight, "fp8_matmul")
     i = weight.get_device()
     n, k = _weight(weight, weight_scales, 2, "fp8_matmul")
