@@ -15,7 +15,6 @@ namespace lloom {
 
 // Type ids beside those of kq_common.hpp: BF16 is GGUF's, E4M3 has none there.
 constexpr int T_BF16 = 30, T_E4M3 = 100;
-constexpr int FP8_BLOCK = 128;
 
 // A product's operands.  Rows of x are x_stride elements apart, its scales
 // (e4m3 x) at [row * xs_row + block * xs_block].  starts (null: one group of
@@ -138,11 +137,6 @@ __device__ __forceinline__ fp8_h8 fp8_halves(uint32_t lo, uint32_t hi) {
 }
 
 // ---------------------------------------------------------------- types --
-template <int TYPE>
-struct Fp8Size {
-    static constexpr int V = TYPE == T_F32 ? 4 : TYPE == T_E4M3 ? 1 : 2;
-};
-
 // Eight values from element i (16-byte aligned) as f32.
 template <int TYPE>
 __device__ __forceinline__ void fp8_load8(const void* p, int64_t i, float (&v)[8]) {

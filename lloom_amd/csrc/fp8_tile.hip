@@ -104,7 +104,7 @@ __device__ __forceinline__ v8i fp8_read16(const uint8_t* rows, int row, int g) {
 
 // Place of a workgroup among a grouped call's tiles: a run of them an XCD, walked
 // in groups of four, as tile_of walks another call's: what an XCD's workgroups
-// have in flight then shares rows of x and of the weight in its L2 (8192 tokens top
+// have in flight then shares rows of x and of the weight in its L2 (MMA_FP8, 8192 tokens top
 // 8 of 64 experts, [2048, 2048]: 389 us in launch order, 377 so; smaller tiles have
 // fewer rows of one expert to share, (128, 128) 129 and 140).  t is -1 where none is
 // left.
