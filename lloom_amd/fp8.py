@@ -12,7 +12,9 @@ An expert layer of a step is
     q, s = fp8_silu_mul(h[:, :inner], h[:, inner:])
     y = fp8_grouped_matmul(q, w_down, s_down, plan.starts, x_scales=s, scatter=plan.planes, out_dtype=x.dtype)
 
-with y [tokens * topk, n] in the order of ids, as QTensor.indexed_moe_forward has it.  Nothing here waits for the GPU: what
+with y [tokens * topk, n] in the order of ids, as QTensor.indexed_moe_forward has it.  A product that brings x into 8 bits in a
+launch before its own does so in the workspace of the GPU's context, which serves one stream at a time: calls on another stream
+wait for them first, or take e4m3 x (fp8_quantize's).  Nothing here waits for the GPU: what
 only the GPU can see (an id, a start or a row out of range) is left out of the result and raised by the next paged_check()
 as EEXPERT.
 """
