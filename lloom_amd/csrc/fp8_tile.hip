@@ -458,7 +458,9 @@ static hipError_t tile_with(const Fp8Call& c, hipStream_t s) {
 //     2048] 14.7 / 10.9 / 15.0 / 13.4 / 20.6 / 18.5, 509 37 / 38 / 24.2 / 27.2 / 23.6 / 22.1, 1200 83 /
 //     90 / 53 / 64 / 54 / 58, 2048 133 / 150 / 80 / 106 / 71 / 83; 96 of [8192, 512] 6.2 / 6.0 / 6.6 /
 //     7.0 / 8.5 / 8.8; 2000 of [264, 2048] 14.6 / 10.8 / 14.9 / 13.2 / 20.6 / 18.5, 44000 of [112, 1264] 42 /
-//     52 / 28 / 38 / 30 / 37, 20000 of [300, 4096] 126 / 131 / 79 / 91 / 70 / 78
+//     52 / 28 / 38 / 30 / 37, 20000 of [300, 4096] 126 / 131 / 79 / 91 / 70 / 78; long outputs of few
+//     rows: 32 of [65536, 4096] 64 / 54 / 67 / 60 / 70 / -, 64 76 / 75 / 68 / 64 / 74 / -, 96 104 / 105 /
+//     86 / 102 / 77 / -, 64 of [128256, 2048] 83 / 96 / 59 / 71 / 75 / -, 20 of [32768, 8192] 63 / 67 / 70 / 68 / 75 / -
 //   grouped, the same: top 8 of 128 experts [1536, 2048], 8, 32 and 128 rows an expert on
 //     average, 75 / 84 / 75 / 92 / 98 / 114, 100 / 116 / 91 / 110 / 111 / 132, 241 / 295 / 167 / 222 /
 //     172 / 209; of 64 [2048, 2048], 1024 rows 1098 / 1326 / 636 / 860 / 580 / 693; of 4
@@ -479,8 +481,9 @@ static auto tile_choice(const Fp8Call& c, F with) {
         return tiles * ((c.n + cols - 1) / cols);
     };
     const int64_t large = count(256, 256), rounds = (large + 255) / 256;
-    if (c.cut && c.nb > 1 && (!c.starts || each >= 512) && 8 * large >= 5 * 256 * rounds) return with(Fp8Cfg<4, 2, 2, 4, 2>{});
-    const bool full = !c.starts || each >= 96, half = !c.starts || each >= 10;  // tiles of 128 rows, of 64
+    if (c.cut && c.nb > 1 && (c.starts ? each >= 512 : each > 128) && 8 * large >= 5 * 256 * rounds) return with(Fp8Cfg<4, 2, 2, 4, 2>{});
+    // enough rows for tiles of 128, of 64
+    const bool full = c.starts ? each >= 96 : each > 64, half = c.starts ? each >= 10 : each > 32;
     if (full && count(128, 128) >= 300) return with(Fp8Cfg<2, 2, 2, 2, 2>{});
     if (full && count(64, 128) > 256 && count(128, 128) <= 256 && c.kb >= (c.cut ? 32 : 16))
         return with(Fp8Cfg<2, 2, 2, 2, 2, 2>{});

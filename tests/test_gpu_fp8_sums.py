@@ -67,12 +67,12 @@ def test_neighbours_that_cancel_by_expert(L, each, out):
 # (m, n, k) of every kernel and tile by number of steps: few rows; 32 x 128 and 64 x 128 with k in one part and in two; 128 x 128
 # in two parts and in one, with one step, some, and past the 64 blocks whose scales a wave holds; ends inside tiles
 SHAPES = [(3, 264, 656), (16, 4104, 2064), (64, 4096, 656), (17, 257, 1040), (128, 2050, 8336),  # few rows
-          (300, 3001, 400), (700, 1000, 400), (600, 1000, 16),  # 32 x 128
+          (300, 3001, 400), (700, 1000, 400), (600, 1000, 16), (20, 35000, 1040),  # 32 x 128
           (300, 3001, 1040), (200, 3100, 8336),      # 32 x 128, two parts
-          (1400, 1500, 656), (700, 5000, 400), (1030, 1000, 272),  # 64 x 128
+          (1400, 1500, 656), (700, 5000, 400), (1030, 1000, 272), (50, 40000, 272),  # 64 x 128
           (540, 2900, 1168), (400, 4200, 8208),      # 64 x 128, two parts
           (700, 4100, 4112), (1000, 4001, 2192),     # 128 x 128, two parts
-          (3400, 3101, 656), (2304, 8200, 1168), (2500, 2100, 8336), (20000, 300, 1264), (5000, 1300, 16), (3000, 1800, 272)]
+          (3400, 3101, 656), (2304, 8200, 1168), (2500, 2100, 8336), (20000, 300, 1264), (5000, 1300, 16), (3000, 1800, 272), (100, 40000, 272)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
