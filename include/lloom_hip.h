@@ -354,13 +354,13 @@ int lloom_hip_paged_attention_workspace_bytes(int64_t tokens, int64_t requests, 
  * aligned; at most 2^24 rows and n, 4096 experts, and under 2^32 threads a launch
  * (about one for 64 values of y, in tiles that a group's few rows do not fill); x
  * that is gathered from, in 8 bits, and the scales are under 2^31 bytes.  An output
- * shares no memory with an input or another output (EINVAL).  A block's sum is formed first and the
- * product of its two scales, rounded to f32, meets it: scales whose product is below
- * 2^-126 lose bits, and over f32's largest a sum of zero gives NaN.  Products are
- * exact and sums f32 into every type of y (but for lloom_hip_ctx_set_fp8_mma), which
- * rounds once.  The calls neither synchronize nor copy; what only the GPU can
- * see is left out of the result as said below and reported by the next
- * lloom_hip_ctx_sync as LLOOM_HIP_EEXPERT.
+ * shares no memory with an input or another output (EINVAL).  A block's sum is
+ * formed first and the product of its two scales, rounded to f32, meets it: scales
+ * whose product is below 2^-126 lose bits, and over f32's largest a sum of zero
+ * gives NaN.  Products are exact and sums f32 into every type of y (but for
+ * lloom_hip_ctx_set_fp8_mma), which rounds once.  The calls neither synchronize nor
+ * copy; what only the GPU can see is left out of the result as said below and
+ * reported by the next lloom_hip_ctx_sync as LLOOM_HIP_EEXPERT.
  *
  * lloom_hip_fp8_quantize: rows of x [rows][k], x_stride elements apart, into
  * q [rows][k] and scales [ceil(k / 128)][scales_stride] (a block's rows side by

@@ -481,9 +481,10 @@ static auto tile_choice(const Fp8Call& c, F with) {
         return tiles * ((c.n + cols - 1) / cols);
     };
     const int64_t large = count(256, 256), rounds = (large + 255) / 256;
-    if (c.cut && c.nb > 1 && (c.starts ? each >= 512 : each > 128) && 8 * large >= 5 * 256 * rounds) return with(Fp8Cfg<4, 2, 2, 4, 2>{});
-    // enough rows for tiles of 128, of 64
-    const bool full = c.starts ? each >= 96 : each > 64, half = c.starts ? each >= 10 : each > 32;
+    // enough rows for tiles of 256, of 128, of 64
+    const bool whole = c.starts ? each >= 512 : each > 128, full = c.starts ? each >= 96 : each > 64,
+               half = c.starts ? each >= 10 : each > 32;
+    if (c.cut && c.nb > 1 && whole && 8 * large >= 5 * 256 * rounds) return with(Fp8Cfg<4, 2, 2, 4, 2>{});
     if (full && count(128, 128) >= 300) return with(Fp8Cfg<2, 2, 2, 2, 2>{});
     if (full && count(64, 128) > 256 && count(128, 128) <= 256 && c.kb >= (c.cut ? 32 : 16))
         return with(Fp8Cfg<2, 2, 2, 2, 2, 2>{});
